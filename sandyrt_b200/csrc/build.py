@@ -51,7 +51,10 @@ LIBRARIES: Dict[str, List[str]] = {
     "attention_prefill_tc": [],
     "attention_prefill_f32": [],
     "attention_prefill_f32_tc": [],
+    "kv_8bit": [],
+    "attention_8bit": [],
     "sampling": [],
+    "logprobs": [],
     "rmsnorm": [],
     "elementwise": [],
     "attention_prepare": [],

@@ -1,0 +1,290 @@
+// The paged key/value cache in 8 bits: a step's keys and values quantised as they are written, and cached rows read back.
+//
+// Formulas (blocks, codes and scales in kv_8bit.cuh).  A step's new tokens of a request touch pages kv_before / page_size to
+// (kv_before + n - 1) / page_size of it.  For each touched block:
+//   need = the scale for the largest |x| of the step's values in it;
+//   s'   = need, if the block's first position is among the new ones; else max(s, need), and the codes c of the positions
+//          before the step become round(c * s / s') where s' > s;
+//   the new codes are round(x / s').
+// A page that starts with the step's tokens is thus a fresh one, whatever it held before; slots behind the new tokens are left
+// as they are.
+//
+// What bounds it.  2 (keys, values) x 2 bytes in and 1 byte out a value: a copy's work.  One warp owns one block and holds the
+// block's new values in registers between the maximum and the rounding (up to 1,024 values; larger blocks are read twice,
+// the second time from the caches), so each value crosses the memory bus once.
+#include "kv_8bit.cuh"
+
+namespace {
+
+constexpr int WARPS = 8;
+constexpr int HELD = 4;            // pieces of 8 values that a lane holds: 32 lanes x 4 x 8 = 1,024 values
+
+struct Planes {
+    uint8_t *k, *v;
+    float *k_scale, *v_scale;
+    long long page_stride, scale_stride;
+};
+
+// Eight values as floats; ALIGNED: they start on 16 bytes.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void load8(const T* __restrict__ p, float (&x)[8]) {
+    if (ALIGNED) {
+        if (sizeof(T) == 4) {
+            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+            x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        } else {
+            const uint4 raw = *reinterpret_cast<const uint4*>(p);
+            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 f = __bfloat1622float2(h[i]);
+                x[2 * i] = f.x;
+                x[2 * i + 1] = f.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = to_f32(p[i]);
+    }
+}
+
+template <int CODE>
+__device__ __forceinline__ uint2 encode8(const float (&x)[8], float inv) {
+    const float most = __uint_as_float(LARGEST_KEPT_BITS);
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = fminf(fmaxf(x[i], -most), most) * inv;
+    return make_uint2(encode2<CODE>(y[0], y[1]) | encode2<CODE>(y[2], y[3]) << 16,
+                      encode2<CODE>(y[4], y[5]) | encode2<CODE>(y[6], y[7]) << 16);
+}
+
+template <typename T, int CODE, bool ALIGNED>
+__global__ void __launch_bounds__(WARPS * 32)
+append_kernel(const T* __restrict__ k_src, const T* __restrict__ v_src, long long ld_k, long long ld_v, Planes cache,
+              const int* __restrict__ block_table, int max_blocks, const int* __restrict__ q_start,
+              const int* __restrict__ kv_before, int n_rows, int n_kv_heads, int head_dim, int page_size, int num_pages,
+              int groups_of_heads, int* __restrict__ status) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int s = blockIdx.y;
+    const int nth = blockIdx.x / groups_of_heads;                   // which of the request's touched pages
+    const int unit = (blockIdx.x % groups_of_heads) * WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int first_row = q_start[s], n = q_start[s + 1] - first_row, before = kv_before[s];
+    if (unit >= 2 * n_kv_heads || n <= 0) return;
+    if (first_row < 0 || n > n_rows - first_row) {                  // rows that are not there
+        if (lane == 0 && status) atomicOr(status, 8);
+        return;
+    }
+    const int block = before / page_size + nth;
+    const int lo = max(before, block * page_size), hi = min(before + n, (block + 1) * page_size);     // new positions in the block
+    if (lo >= hi && before >= 0) return;
+    const int page = before >= 0 && block < max_blocks ? block_table[(size_t)s * max_blocks + block] : -1;
+    if (page < 0 || page >= num_pages) {                            // no page behind these positions: nothing may be written
+        if (lane == 0 && unit == 0 && status) atomicOr(status, 8);
+        return;
+    }
+    const int h = unit >> 1, plane = unit & 1;                      // neighbouring warps: keys and values of one head
+    const T* src = (plane ? v_src : k_src) + (size_t)(first_row + lo - before) * (plane ? ld_v : ld_k) + (size_t)h * head_dim;
+    const long long ld = plane ? ld_v : ld_k;
+    uint8_t* codes = (plane ? cache.v : cache.k) + (size_t)page * cache.page_stride + (size_t)h * page_size * head_dim;
+    float* scale_at = (plane ? cache.v_scale : cache.k_scale) + (size_t)page * cache.scale_stride + h;
+    const int kept = lo - block * page_size;                        // positions of the block that were there before
+    const float old = kept > 0 ? *scale_at : 0.0f;
+    const int per_row = head_dim >> 3, pieces = (hi - lo) * per_row;
+
+    // the largest |x|: as unsigned numbers floats without their sign keep their order, with infinities and NaN above all
+    float x[HELD][8];
+    unsigned amax = 0;
+#pragma unroll
+    for (int k = 0; k < HELD; k++) {
+        const int i = lane + 32 * k;
+        if (i < pieces) {
+            load8<T, ALIGNED>(src + (size_t)(i / per_row) * ld + (i % per_row) * 8, x[k]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[k][e] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < HELD; k++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) amax = max(amax, __float_as_uint(x[k][e]) & 0x7fffffffu);
+    for (int i = lane + 32 * HELD; i < pieces; i += 32) {
+        float y[8];
+        load8<T, ALIGNED>(src + (size_t)(i / per_row) * ld + (i % per_row) * 8, y);
+#pragma unroll
+        for (int e = 0; e < 8; e++) amax = max(amax, __float_as_uint(y[e]) & 0x7fffffffu);
+    }
+    amax = __reduce_max_sync(0xffffffffu, amax);
+
+    const float nan = __uint_as_float(0x7fffffffu);
+    float now = amax >= 0x7f800000u ? nan : scale_for<CODE>(min(amax, LARGEST_KEPT_BITS));
+    if (kept > 0 && !(old <= now)) now = old;                       // the old one is larger, or one of the two is NaN
+    if (amax >= 0x7f800000u) now = nan;
+    const bool sound = now == now;
+    const float inv = sound ? 1.0f / now : 0.0f;                    // of a power of two: exact
+
+    if (kept > 0 && sound && now > old) {                           // the block's earlier codes at its new scale
+        const float shrink = old * inv;
+        for (int i = lane; i < kept * (head_dim >> 2); i += 32) {
+            unsigned* w = reinterpret_cast<unsigned*>(codes) + i;
+            unsigned a, b;
+            decode4<CODE>(*w, a, b);
+            const float2 p = half2_floats(a), q = half2_floats(b);
+            *w = encode2<CODE>(p.x * shrink, p.y * shrink) | encode2<CODE>(q.x * shrink, q.y * shrink) << 16;
+        }
+    }
+    uint2* dst = reinterpret_cast<uint2*>(codes + (size_t)kept * head_dim);      // the new rows follow one another in a block
+#pragma unroll
+    for (int k = 0; k < HELD; k++) {
+        const int i = lane + 32 * k;
+        if (i < pieces) dst[i] = sound ? encode8<CODE>(x[k], inv) : make_uint2(0u, 0u);
+    }
+    for (int i = lane + 32 * HELD; i < pieces; i += 32) {
+        float y[8];
+        load8<T, ALIGNED>(src + (size_t)(i / per_row) * ld + (i % per_row) * 8, y);
+        dst[i] = sound ? encode8<CODE>(y, inv) : make_uint2(0u, 0u);
+    }
+    if (lane == 0) *scale_at = now;
+}
+
+// Sixteen codes times their scale, rounded to T (exact in bfloat16 and float32 for the scales that appending gives).
+template <typename T, int CODE>
+__device__ __forceinline__ void store16(uint4 raw, float scale, T* dst, bool aligned) {
+    const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        unsigned a, b;
+        decode4<CODE>(w[i], a, b);
+        const float2 p = half2_floats(a), q = half2_floats(b);
+        x[4 * i] = p.x * scale; x[4 * i + 1] = p.y * scale; x[4 * i + 2] = q.x * scale; x[4 * i + 3] = q.y * scale;
+    }
+    if (aligned) {
+        if (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                reinterpret_cast<float4*>(dst)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+        } else {
+            __nv_bfloat162 h[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(h)[0];
+            reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(h)[1];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++) dst[i] = from_f32<T>(x[i]);
+    }
+}
+
+constexpr int READ_THREADS = 256;
+constexpr int READ_ROWS = 8;       // rows of a request that a block reads
+
+// A lane takes 16 codes of the keys and as many of the values; neighbouring lanes follow the output row, which is written
+// whole lines at a time.
+template <typename T, int CODE>
+__global__ void __launch_bounds__(READ_THREADS)
+read_kernel(Planes cache, const int* __restrict__ block_table, int max_blocks, const int* __restrict__ first,
+            const int* __restrict__ out_start, T* __restrict__ k_out, T* __restrict__ v_out, long long ld_k, long long ld_v,
+            int n_rows, int n_kv_heads, int head_dim, int page_size, int num_pages, bool aligned, int* __restrict__ status) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int s = blockIdx.y;
+    const int row0 = out_start[s], n = out_start[s + 1] - row0, from = first[s];
+    const int r0 = blockIdx.x * READ_ROWS, rows = min(READ_ROWS, n - r0);
+    if (rows <= 0) return;
+    if (row0 < 0 || n > n_rows - row0) {                            // rows that are not there
+        if (threadIdx.x == 0 && status) atomicOr(status, 16);
+        return;
+    }
+    const int per_head = head_dim >> 4, per_row = n_kv_heads * per_head;
+    for (int i = threadIdx.x; i < rows * per_row; i += READ_THREADS) {
+        const int r = i / per_row, at = i % per_row, h = at / per_head, d = at % per_head * 16;
+        const int pos = from + r0 + r;
+        const int block = pos >= 0 ? pos / page_size : max_blocks;
+        const int page = block < max_blocks ? block_table[(size_t)s * max_blocks + block] : -1;
+        if (page < 0 || page >= num_pages) {                        // no page behind this position: its row is left as it was
+            if (at == 0 && status) atomicOr(status, 16);
+            continue;
+        }
+        const size_t code_at = (size_t)page * cache.page_stride + ((size_t)h * page_size + (pos - block * page_size)) * head_dim + d;
+        const size_t scale_at = (size_t)page * cache.scale_stride + h;
+        const uint4 kc = *reinterpret_cast<const uint4*>(cache.k + code_at);
+        const uint4 vc = *reinterpret_cast<const uint4*>(cache.v + code_at);
+        const float ks = cache.k_scale[scale_at], vs = cache.v_scale[scale_at];
+        store16<T, CODE>(kc, ks, k_out + (size_t)(row0 + r0 + r) * ld_k + (size_t)h * head_dim + d, aligned);
+        store16<T, CODE>(vc, vs, v_out + (size_t)(row0 + r0 + r) * ld_v + (size_t)h * head_dim + d, aligned);
+    }
+}
+
+bool bad_cache(const void* k, const void* v, const float* ks, const float* vs, long long page_stride, int n_kv_heads, int head_dim,
+               int page_size) {
+    return !k || !v || !ks || !vs || n_kv_heads < 1 || head_dim < 16 || page_size < 1 || page_stride < 1;
+}
+
+}  // namespace
+
+// k_src, v_src: [n_rows, Hkv * D] of dtype with row pitches ld_k, ld_v (elements).  Request s brings rows q_start[s] .. q_start[s + 1] - 1,
+// which go to positions kv_before[s] on; max_q_len: the most that one brings.  k, v: codes [num_pages][Hkv][page_size][D], page pitch
+// page_stride (bytes); k_scale, v_scale: [num_pages][Hkv], row pitch scale_stride.  Pages that two requests of one call both
+// write are not allowed.  Bit 3 of *status: a position without a page, or rows past n_rows.
+SANDY_API int sandy_kv_append_8bit(const void* k_src, const void* v_src, long long ld_k, long long ld_v, void* k, void* v,
+                                   float* k_scale, float* v_scale, long long page_stride, long long scale_stride,
+                                   const int* block_table, int max_blocks, const int* q_start, const int* kv_before, int n_seqs,
+                                   int n_rows, int max_q_len, int n_kv_heads, int head_dim, int page_size, int num_pages, int dtype, int code,
+                                   int* status, cudaStream_t stream) {
+    if (n_seqs == 0 || max_q_len == 0) return SANDY_OK;
+    if (!k_src || !v_src || !block_table || !q_start || !kv_before || n_seqs < 0 || max_q_len < 0 ||
+        bad_cache(k, v, k_scale, v_scale, page_stride, n_kv_heads, head_dim, page_size))
+        return SANDY_ERR_ARGUMENT;
+    if (head_dim % 16 || page_stride % 16 || (((uintptr_t)k | (uintptr_t)v) & 15) || n_seqs > 65535) return SANDY_ERR_UNSUPPORTED;
+    const int groups = (2 * n_kv_heads + WARPS - 1) / WARPS;
+    const long long touched = ((long long)max_q_len + page_size - 2) / page_size + 1;      // by one request, wherever it starts
+    if (touched * groups > 0x7fffffffll) return SANDY_ERR_UNSUPPORTED;
+    const Planes cache = {(uint8_t*)k, (uint8_t*)v, k_scale, v_scale, page_stride, scale_stride};
+    const dim3 grid((unsigned)(touched * groups), n_seqs), block(WARPS * 32);
+#define APPEND(T, CODE)                                                                                                         \
+    do {                                                                                                                        \
+        const size_t any = (uintptr_t)k_src | (uintptr_t)v_src | (size_t)(ld_k * (long long)sizeof(T)) | (size_t)(ld_v * (long long)sizeof(T)); \
+        return sandy_launch(any % 16 == 0 ? append_kernel<T, CODE, true> : append_kernel<T, CODE, false>, grid, block, 0, stream, \
+                            (const T*)k_src, (const T*)v_src, ld_k, ld_v, cache, block_table, max_blocks, q_start, kv_before,   \
+                            n_rows, n_kv_heads, head_dim, page_size, num_pages, groups, status);                                        \
+    } while (0)
+    if (dtype == SANDY_F32 && code == SANDY_E4M3) APPEND(float, SANDY_E4M3);
+    if (dtype == SANDY_F32 && code == SANDY_INT8) APPEND(float, SANDY_INT8);
+    if (dtype == SANDY_BF16 && code == SANDY_E4M3) APPEND(bf16, SANDY_E4M3);
+    if (dtype == SANDY_BF16 && code == SANDY_INT8) APPEND(bf16, SANDY_INT8);
+#undef APPEND
+    return SANDY_ERR_UNSUPPORTED;
+}
+
+// Rows out_start[s] .. out_start[s + 1] - 1 of k_out and v_out ([n_rows, Hkv * D] of dtype, row pitches ld_k, ld_v) become the cached
+// positions first[s] on of request s; max_len: the most rows of one request.  Bit 4 of *status: a position without a page, or rows past
+// n_rows.
+SANDY_API int sandy_kv_read_8bit(const void* k, const void* v, const float* k_scale, const float* v_scale, long long page_stride,
+                                 long long scale_stride, const int* block_table, int max_blocks, const int* first,
+                                 const int* out_start, void* k_out, void* v_out, long long ld_k, long long ld_v, int n_seqs,
+                                 int n_rows, int max_len, int n_kv_heads, int head_dim, int page_size, int num_pages, int dtype, int code,
+                                 int* status, cudaStream_t stream) {
+    if (n_seqs == 0 || max_len == 0) return SANDY_OK;
+    if (!k_out || !v_out || !block_table || !first || !out_start || n_seqs < 0 || max_len < 0 ||
+        bad_cache(k, v, k_scale, v_scale, page_stride, n_kv_heads, head_dim, page_size))
+        return SANDY_ERR_ARGUMENT;
+    if (head_dim % 16 || page_stride % 16 || (((uintptr_t)k | (uintptr_t)v) & 15) || n_seqs > 65535) return SANDY_ERR_UNSUPPORTED;
+    const Planes cache = {(uint8_t*)k, (uint8_t*)v, (float*)k_scale, (float*)v_scale, page_stride, scale_stride};
+    const dim3 grid((max_len - 1) / READ_ROWS + 1, n_seqs), block(READ_THREADS);
+#define READ(T, CODE)                                                                                                           \
+    do {                                                                                                                        \
+        const size_t any = (uintptr_t)k_out | (uintptr_t)v_out | (size_t)(ld_k * (long long)sizeof(T)) | (size_t)(ld_v * (long long)sizeof(T)); \
+        return sandy_launch(read_kernel<T, CODE>, grid, block, 0, stream, cache, block_table, max_blocks, first, out_start,     \
+                            (T*)k_out, (T*)v_out, ld_k, ld_v, n_rows, n_kv_heads, head_dim, page_size, num_pages, any % 16 == 0, status); \
+    } while (0)
+    if (dtype == SANDY_F32 && code == SANDY_E4M3) READ(float, SANDY_E4M3);
+    if (dtype == SANDY_F32 && code == SANDY_INT8) READ(float, SANDY_INT8);
+    if (dtype == SANDY_BF16 && code == SANDY_E4M3) READ(bf16, SANDY_E4M3);
+    if (dtype == SANDY_BF16 && code == SANDY_INT8) READ(bf16, SANDY_INT8);
+#undef READ
+    return SANDY_ERR_UNSUPPORTED;
+}

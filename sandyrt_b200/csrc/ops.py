@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
+import functools
 from typing import Optional
 
 import torch
@@ -498,6 +499,247 @@ def prefill_attention_f32(q, k_cache, v_cache, block_table, q_start, kv_before, 
         _check(code, f"decode_attention_single(H={n_heads},Hkv={hkv},D={d},splits={single_splits})")
 
 
+# ---- a cache in 8 bits (kv_8bit.cu, attention_8bit.cu) -----------------------------------------------------------------
+CODE_CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
+_V, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(library: str, name: str, argtypes: tuple, restype=ctypes.c_int):
+    """A typed entry point: it takes Python numbers and addresses as they are, without an object for each."""
+    f = getattr(load_library(library), name)
+    f.argtypes, f.restype = argtypes, restype
+    return f
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _device_of(what: str, *tensors) -> torch.device:
+    """The one CUDA device all tensors are on."""
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise KernelError(f"{what}: tensors on {device} and {t.device}")
+    if device.type != "cuda":
+        raise KernelError("kernel arguments must be CUDA tensors (there is no CPU path)")
+    return device
+
+
+def _status_word(device: torch.device) -> int:
+    """The address of the device's status word.  It is made by the first call on the device, which must not be a recorded one: a
+    graph's memory would hold it."""
+    t = _kernel_status.get(device.index)
+    if t is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise KernelError("the device's status word is made by its first kernel call; call once before capturing a graph")
+        t = kernel_status(device)
+    return t.data_ptr()
+
+
+def _run_on(device: torch.device, entry, args: tuple, what: str) -> None:
+    """One typed call on the device's current stream, whichever device is the current one."""
+    if device.index == torch.cuda.current_device():
+        code = entry(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            code = entry(*args, torch.cuda.current_stream().cuda_stream)
+    _check(code, what)
+
+
+@dataclasses.dataclass
+class Cache8:
+    """Keys and values of one layer in 8 bits: codes [num_pages, Hkv, page_size, D] (float8_e4m3fn or int8, dense inside a page) and
+    float32 scales [num_pages, Hkv], one for each page and head; a cached number is its code times its block's scale.  Pages
+    need no initial values: a page's scales are set when its first position is written.  kv_append_8bit is what writes it;
+    codes that are NaN are not for it (a block with a value that is not finite has a scale of NaN)."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+    @classmethod
+    def empty(cls, num_pages: int, n_kv_heads: int, page_size: int, head_dim: int, dtype=torch.float8_e4m3fn, device="cuda") -> "Cache8":
+        codes = lambda: torch.empty(num_pages, n_kv_heads, page_size, head_dim, dtype=dtype, device=device)
+        scales = lambda: torch.empty(num_pages, n_kv_heads, dtype=torch.float32, device=device)
+        return cls(codes(), codes(), scales(), scales())
+
+    def check(self, what: str):
+        """(Hkv, page_size, D, page pitch, scale pitch, num_pages, code) or KernelError."""
+        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
+        if k.dtype not in CODE_CODES or v.dtype != k.dtype:
+            raise UnsupportedShape(f"{what}: codes are float8_e4m3fn or int8, got {k.dtype} and {v.dtype}")
+        if k.dim() != 4 or k.shape != v.shape:
+            raise KernelError(f"{what}: codes must be [num_pages, Hkv, page_size, D], keys and values alike")
+        n, hkv, ps, d = k.shape
+        stride = k.stride()
+        if stride != v.stride() or stride[1:] != (ps * d, d, 1):
+            raise KernelError(f"{what}: codes must be dense inside a page, keys and values with one page stride")
+        if d % 16 or not 16 <= d <= 256 or stride[0] % 16 or k.data_ptr() % 16 or v.data_ptr() % 16:
+            raise UnsupportedShape(f"{what}: head sizes 16..256 in steps of 16, pages on 16-byte boundaries")
+        for s in (ks, vs):
+            if s.dtype != torch.float32 or s.shape != (n, hkv) or s.stride(1) != 1 or s.stride(0) != ks.stride(0):
+                raise KernelError(f"{what}: scales must be float32 [num_pages, Hkv]")
+        if n > 1 and (stride[0] < hkv * ps * d or ks.stride(0) < hkv):
+            raise KernelError(f"{what}: pages overlap")
+        return hkv, ps, d, stride[0], ks.stride(0), n, CODE_CODES[k.dtype]
+
+
+def _indices(what: str, **arrays) -> None:
+    for name, t in arrays.items():
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise KernelError(f"{what}: {name} must be a contiguous int32 tensor")
+
+
+def _portions(what: str, table, starts, befores) -> int:
+    """The number of requests of block table, row starts [S + 1] and first positions [S]."""
+    _indices(what, block_table=table, starts=starts, positions=befores)
+    S = befores.numel()
+    if table.dim() != 2 or table.shape[0] != S or starts.numel() != S + 1:
+        raise KernelError(f"{what}: the block table, the row starts and the first positions disagree on the requests")
+    if S > 65535:
+        raise UnsupportedShape(f"{what}: at most 65535 requests")
+    return S
+
+
+def _rows_of(what: str, hkv: int, d: int, *tensors) -> None:
+    first = tensors[0]
+    for t in tensors:
+        if t.dim() != 2 or t.shape != (first.shape[0], hkv * d) or t.dtype != first.dtype or (t.stride(1) != 1 and t.numel()):
+            raise KernelError(f"{what}: rows must be [T, Hkv * D] = [T, {hkv * d}] of one type, with an innermost stride of 1")
+
+
+_APPEND8 = (_V, _V, _L, _L, _V, _V, _V, _V, _L, _L, _V, _I, _V, _V, _I, _I, _I, _I, _I, _I, _I, _I, _I, _V, _V)
+_READ8 = (_V, _V, _V, _V, _L, _L, _V, _I, _V, _V, _V, _V, _L, _L, _I, _I, _I, _I, _I, _I, _I, _I, _I, _V, _V)
+_ATTEND8 = (_V, _L, _V, _V, _V, _V, _L, _L, _V, _I, _I, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _I, _I, _I, _F, _V, _I, _V, _I, _I, _V, _V)
+
+
+def kv_append_8bit(k_src, v_src, cache: Cache8, block_table, q_start, kv_before, *, max_q_len: int) -> None:
+    """Quantise the step's keys and values ([T, Hkv * D] views, float32 or bfloat16, a row pitch each) into their pages.
+    Request s of the block table's rows brings rows q_start[s] .. q_start[s + 1] - 1 (int32 [S + 1]) for its positions
+    kv_before[s] on (int32 [S]); max_q_len: the most that one request brings.  A block's scale is the smallest power of two by
+    which its largest value fits the code; a block that held earlier positions keeps its scale or, where the new values need a
+    larger one, has its earlier codes rounded again.  A block that is given a value that is not finite gets a scale of NaN.
+    Requests must not share a page that they write.  Rows in front of the first request and behind the last one are not read."""
+    hkv, ps, d, page_stride, scale_stride, pages, code = cache.check("kv_append_8bit")
+    _rows_of("kv_append_8bit", hkv, d, k_src, v_src)
+    dtype, S = _dt(k_src), _portions("kv_append_8bit", block_table, q_start, kv_before)
+    if max_q_len < 0:
+        raise KernelError("kv_append_8bit: max_q_len is negative")
+    device = _device_of("kv_append_8bit", k_src, v_src, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, q_start, kv_before)
+    if S == 0 or max_q_len == 0 or k_src.shape[0] == 0:
+        return
+    _run_on(device, _entry("kv_8bit", "sandy_kv_append_8bit", _APPEND8),
+            (k_src.data_ptr(), v_src.data_ptr(), k_src.stride(0), v_src.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
+             cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), page_stride, scale_stride, block_table.data_ptr(), block_table.shape[1],
+             q_start.data_ptr(), kv_before.data_ptr(), S, k_src.shape[0], max_q_len, hkv, d, ps, pages, dtype, code, _status_word(device)),
+            "kv_append_8bit")
+
+
+def kv_read_8bit(cache: Cache8, block_table, first, out_start, k_out, v_out, *, max_len: int) -> None:
+    """Cached rows back as numbers: rows out_start[s] .. out_start[s + 1] - 1 (int32 [S + 1]) of k_out and v_out ([N, Hkv * D], float32
+    or bfloat16, a row pitch each) become positions first[s] on (int32 [S]) of the block table's request s; max_len: the
+    most rows of one request.  Exact in both types.  Rows of no request, and of positions without a page, are left as they were."""
+    hkv, ps, d, page_stride, scale_stride, pages, code = cache.check("kv_read_8bit")
+    _rows_of("kv_read_8bit", hkv, d, k_out, v_out)
+    dtype, S = _dt(k_out), _portions("kv_read_8bit", block_table, out_start, first)
+    if max_len < 0:
+        raise KernelError("kv_read_8bit: max_len is negative")
+    device = _device_of("kv_read_8bit", k_out, v_out, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, out_start, first)
+    if S == 0 or max_len == 0 or k_out.shape[0] == 0:
+        return
+    _run_on(device, _entry("kv_8bit", "sandy_kv_read_8bit", _READ8),
+            (cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), page_stride, scale_stride,
+             block_table.data_ptr(), block_table.shape[1], first.data_ptr(), out_start.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
+             k_out.stride(0), v_out.stride(0), S, k_out.shape[0], max_len, hkv, d, ps, pages, dtype, code, _status_word(device)), "kv_read_8bit")
+
+
+def _attention_8bit(what, q, cache, block_table, token_seq, positions, q_start, out, n_z, max_n, n_heads, scale, num_splits, rules) -> None:
+    hkv, ps, d, page_stride, scale_stride, pages, code = cache.check(what)
+    if n_heads < 1 or n_heads % hkv:
+        raise UnsupportedShape(f"{what}: {n_heads} heads do not divide into {hkv} key/value heads")
+    if q.dim() != 2 or q.shape[1] != n_heads * d or out.shape != q.shape or out.dtype != q.dtype or \
+            (q.numel() and (q.stride(1) != 1 or out.stride(1) != 1)):
+        raise KernelError(f"{what}: q and out must be [T, H * D] = [T, {n_heads * d}] of one type, with an innermost stride of 1")
+    dtype, T = _dt(q), q.shape[0]
+    window, keep_first, softcap, chunk, sink, out_gate, dist_bias, elem_gate = (
+        rules.get(n, z) for n, z in (("window", 0), ("keep_first", 0), ("softcap", 0.0), ("chunk", 0), ("sink", None), ("out_gate", None),
+                                     ("dist_bias", None), ("elem_gate", None)))
+    if min(window, keep_first, chunk) < 0 or not softcap >= 0 or (keep_first and chunk):
+        raise UnsupportedShape(f"{what}: window, keep_first, softcap and chunk must not be negative, kept first keys and chunks not together")
+    if sink is not None and (sink.dtype != torch.float32 or sink.shape != (n_heads,) or not sink.is_contiguous()):
+        raise KernelError(f"{what}: a sink is a dense float32 [H]")
+    if out_gate is not None and (out_gate.dtype != torch.float32 or out_gate.shape != (T, n_heads) or not out_gate.is_contiguous()):
+        raise KernelError(f"{what}: a gate by head is a dense float32 [T, H]")
+    if dist_bias is not None and (dist_bias.dtype != torch.float32 or dist_bias.dim() != 2 or dist_bias.shape[0] != n_heads
+                                  or dist_bias.shape[1] < 1 or not dist_bias.is_contiguous()):
+        raise KernelError(f"{what}: a bias by distance is a dense float32 [H, n_dist]")
+    if elem_gate is not None and (elem_gate.dtype != q.dtype or elem_gate.dim() != 2 or elem_gate.shape[0] != T or elem_gate.shape[1] < n_heads
+                                  or elem_gate.shape[1] % n_heads or elem_gate.shape[1] > q.shape[1] or (T and elem_gate.stride(1) != 1)):
+        raise KernelError(f"{what}: a gate by element is [T, H * dim] of the queries' type, dim at most the head size")
+    if num_splits < 0 or num_splits > 256:
+        raise KernelError(f"{what}: num_splits must lie in 0 .. 256 (0: the kernel's choice)")
+    device = _device_of(what, q, out, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, token_seq, positions, q_start, sink,
+                        out_gate, dist_bias, elem_gate)
+    if n_z == 0 or max_n == 0 or T == 0:
+        return
+    if block_table.shape[0] == 0 or block_table.shape[1] == 0 or pages == 0:
+        raise KernelError(f"{what}: an empty block table or cache")
+    splits = num_splits or _entry("attention_8bit", "sandy_attention_8bit_splits", (_I,) * 7)(
+        n_z, max_n, n_heads, hkv, d, min(block_table.shape[1] * ps, window + keep_first + max_n if window else 1 << 30), dtype)
+    # partial results of the splits: memory of the stream the call is on, given back to the allocator when it returns
+    scratch = torch.empty(T * n_heads * splits * (d + 2), dtype=torch.float32, device=device) if splits > 1 else None
+    args = _AttentionRules(window, keep_first, softcap, chunk, _at(sink), _at(out_gate), _at(dist_bias),
+                           0 if dist_bias is None else dist_bias.shape[1], _at(elem_gate), 0 if elem_gate is None else elem_gate.stride(0),
+                           0 if elem_gate is None else elem_gate.shape[1] // n_heads)
+    _run_on(device, _entry("attention_8bit", "sandy_attention_8bit", _ATTEND8),
+            (q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), page_stride,
+             scale_stride, block_table.data_ptr(), block_table.shape[1], block_table.shape[0], _at(token_seq), positions.data_ptr(), _at(q_start),
+             out.data_ptr(), out.stride(0), T, n_z, max_n, n_heads, hkv, d, ps, pages, scale, ctypes.addressof(args), splits, _at(scratch),
+             dtype, code, _status_word(device)), f"{what}(H={n_heads},Hkv={hkv},D={d},page={ps},splits={splits})")
+    if splits > 1:
+        global LAUNCHES
+        LAUNCHES += 1
+
+
+def decode_attention_8bit(q, cache: Cache8, block_table, token_seq, positions, out, *, n_heads: int, scale: float, num_splits: int = 0,
+                          **rules) -> None:
+    """Attention of single tokens over a cache in 8 bits: token t (row t of q and out, [T, H * D], float32 or bfloat16) of request
+    token_seq[t] at positions[t] (int32 [T]) sees that request's cached positions up to its own, which kv_append_8bit has written.
+    Head sizes 16..256 in steps of 16, any page size.  num_splits: blocks that share a request's keys (0: the kernel's choice).
+    rules: window, keep_first, softcap, chunk, sink, out_gate, dist_bias, elem_gate as in paged_attention.  A token at a negative
+    position (a padded one) or of no visible key gets zeros."""
+    _known_rules("decode_attention_8bit", rules)
+    _indices("decode_attention_8bit", block_table=block_table, token_seq=token_seq, positions=positions)
+    T = q.shape[0]
+    if block_table.dim() != 2 or token_seq.numel() != T or positions.numel() != T:
+        raise KernelError("decode_attention_8bit: q, token_seq and positions disagree on the tokens")
+    if T > 65535:
+        raise UnsupportedShape("decode_attention_8bit: at most 65535 tokens")
+    _attention_8bit("decode_attention_8bit", q, cache, block_table, token_seq, positions, None, out, T, 1, n_heads, scale, num_splits, rules)
+
+
+def prefill_attention_8bit(q, cache: Cache8, block_table, q_start, kv_before, out, *, n_heads: int, max_q_len: int, scale: float,
+                           num_splits: int = 0, **rules) -> None:
+    """Attention of prompt portions over a cache in 8 bits: request s of the block table's rows brings rows q_start[s] ..
+    q_start[s + 1] - 1 (int32 [S + 1]) at its positions kv_before[s] on (int32 [S]), whose keys and values kv_append_8bit has
+    written; max_q_len: the most that one request brings.  Types, sizes and rules as in decode_attention_8bit; portions of one
+    token are allowed.  Rows of no request are left as they were."""
+    _known_rules("prefill_attention_8bit", rules)
+    S = _portions("prefill_attention_8bit", block_table, q_start, kv_before)
+    if max_q_len < 0:
+        raise KernelError("prefill_attention_8bit: max_q_len is negative")
+    _attention_8bit("prefill_attention_8bit", q, cache, block_table, None, kv_before, q_start, out, S, max_q_len, n_heads, scale, num_splits,
+                    rules)
+
+
+def _known_rules(what: str, rules: dict) -> None:
+    unknown = set(rules) - {"window", "keep_first", "softcap", "chunk", "sink", "out_gate", "dist_bias", "elem_gate"}
+    if unknown:
+        raise TypeError(f"{what}() got an unexpected keyword argument {sorted(unknown)[0]!r}")
+
+
 def _f32(t, name: str) -> None:
     if t is not None and (t.dtype != torch.float32 or not t.is_contiguous()):
         raise KernelError(f"{name} must be a contiguous float32 tensor")
@@ -944,6 +1186,45 @@ def gemm_skinny_groups(a, w, out, *, n_groups: int) -> None:
         _p(a), _p(w), _p(out), i(a.shape[0]), i(n_groups), i(w.shape[0] // n_groups), i(w.shape[1]), i(a.stride(0)), i(w.stride(0)),
         i(out.stride(0)), i(_dt(out)), _stream())
     _check(code, "gemm_skinny_groups")
+
+
+MAX_TOP_LOGPROBS = 32
+_LOGPROBS = (_V, _L, _I, _I, _V, _I, _V, _V, _V, _V, _I, _V, _V)
+
+
+def token_logprobs(logits, ids, logprob, *, entropy=None, top_ids=None, top_logprobs=None, status=None) -> None:
+    """Of every row of `logits` ([n, vocab], float32 or bfloat16, any row pitch): logprob (float32 [n]) of the token ids[r] (int32
+    [n]; -1: none, its logprob is 0), the row's entropy (float32 [n], in nats) and its k likeliest tokens, the likeliest first and of
+    equals the lower id (top_ids int32 [n, k], top_logprobs float32 [n, k], k at most 32).  ids and logprob may be None together, as
+    may each of the others.  A logit of minus infinity has probability 0.  A row with a NaN or plus infinity, or of minus
+    infinities alone, gives NaN; with a NaN its top_ids are -1.  status (int32 [1]): bit 0 is raised for a NaN and for an id that is
+    not in the vocabulary (its logprob is NaN)."""
+    what = "token_logprobs"
+    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise KernelError(f"{what}: logits must be [n, vocab] with an innermost stride of 1")
+    n, vocab = logits.shape
+    dtype = _dt(logits)
+    if (ids is None) != (logprob is None) or (top_ids is None) != (top_logprobs is None):
+        raise KernelError(f"{what}: ids go with logprob, top_ids with top_logprobs")
+    for name, t, dt in (("ids", ids, torch.int32), ("logprob", logprob, torch.float32), ("entropy", entropy, torch.float32)):
+        if t is not None and (t.dtype != dt or t.shape != (n,) or not t.is_contiguous()):
+            raise KernelError(f"{what}: {name} must be a contiguous {dt} tensor of one value per row")
+    top = 0
+    if top_ids is not None:
+        top = top_ids.shape[-1]
+        for name, t, dt in (("top_ids", top_ids, torch.int32), ("top_logprobs", top_logprobs, torch.float32)):
+            if t.dtype != dt or t.shape != (n, top) or not t.is_contiguous():
+                raise KernelError(f"{what}: {name} must be a contiguous {dt} tensor [n, k]")
+        if top > MAX_TOP_LOGPROBS or top > vocab:
+            raise UnsupportedShape(f"{what}: at most {MAX_TOP_LOGPROBS} likeliest tokens, and no more than the vocabulary has")
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+        raise KernelError(f"{what}: status must be an int32 tensor")
+    device = _device_of(what, logits, ids, logprob, entropy, top_ids, top_logprobs, status)
+    if n == 0:
+        return
+    _run_on(device, _entry("logprobs", "sandy_token_logprobs", _LOGPROBS),
+            (logits.data_ptr(), logits.stride(0), n, vocab, _at(ids), top, _at(logprob), _at(entropy), _at(top_ids), _at(top_logprobs), dtype,
+             _at(status)), f"{what}(vocab={vocab},top={top})")
 
 
 def sample(logits, out_tokens, *, temperature=None, top_k=None, top_p=None, uniform=None, status=None,

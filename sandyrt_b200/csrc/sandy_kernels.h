@@ -466,6 +466,29 @@ int sandy_sample(const float* logits, int ld, int n_rows, int vocab, const float
                  const float* top_p, const float* uniform, int* out_token, int* status, int* token_ids,
                  const int* logit_rows, int* positions, int* out_tokens, int* row_step, cudaStream_t stream);
 
+/* kv_8bit.cu */
+int sandy_kv_append_8bit(const void* k_src, const void* v_src, long long ld_k, long long ld_v, void* k, void* v, float* k_scale,
+                         float* v_scale, long long page_stride, long long scale_stride, const int* block_table, int max_blocks,
+                         const int* q_start, const int* kv_before, int n_seqs, int n_rows, int max_q_len, int n_kv_heads, int head_dim,
+                         int page_size, int num_pages, int dtype, int code, int* status, cudaStream_t stream);
+int sandy_kv_read_8bit(const void* k, const void* v, const float* k_scale, const float* v_scale, long long page_stride,
+                       long long scale_stride, const int* block_table, int max_blocks, const int* first, const int* out_start,
+                       void* k_out, void* v_out, long long ld_k, long long ld_v, int n_seqs, int n_rows, int max_len, int n_kv_heads,
+                       int head_dim, int page_size, int num_pages, int dtype, int code, int* status, cudaStream_t stream);
+
+/* attention_8bit.cu */
+int sandy_attention_8bit_splits(int n_z, int max_n, int n_heads, int n_kv_heads, int head_dim, int max_keys, int dtype);
+int sandy_attention_8bit(const void* q, long long ld_q, const void* k, const void* v, const float* k_scale, const float* v_scale,
+                         long long page_stride, long long scale_stride, const int* block_table, int max_blocks, int n_seqs,
+                         const int* token_seq, const int* positions, const int* q_start, void* out, long long ld_out, int n_rows, int n_z,
+                         int max_n, int n_heads, int n_kv_heads, int head_dim, int page_size, int num_pages, float scale,
+                         const SandyAttentionRules* rules, int num_splits, float* scratch, int dtype, int code, int* status,
+                         cudaStream_t stream);
+
+/* logprobs.cu */
+int sandy_token_logprobs(const void* logits, long long ld, int n_rows, int vocab, const int* ids, int top, float* logprob,
+                         float* entropy, int* top_ids, float* top_logprobs, int dtype, int* status, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
