@@ -34,7 +34,6 @@
 
 namespace {
 
-constexpr int WARPS = 4;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Args {
@@ -48,9 +47,10 @@ struct Args {
     const float *sink, *out_gate, *dist_bias;
     const void* elem_gate;
     long long ld_q, ld_out, page_stride, scale_stride;
-    int max_blocks, n_rows, n_seqs, n_heads, n_kv_heads, head_dim, page_size, num_pages, num_splits;
+    int max_blocks, n_rows, n_seqs, n_heads, n_kv_heads, head_dim, page_size, num_pages, num_splits, split_tiles;
     int window, keep_first, chunk, n_dist, ld_elem_gate, gate_dim;
     float scale, softcap;
+    bool q_aligned;                                                  // q's rows start on 16 bytes
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
@@ -83,6 +83,35 @@ __device__ __forceinline__ float sum_over_groups(float v) {
     v += __shfl_xor_sync(0xffffffffu, v, 4);
     v += __shfl_xor_sync(0xffffffffu, v, 8);
     return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+
+// Sixteen elements as floats, zeros where they are not there.
+template <typename T>
+__device__ __forceinline__ void load16(const T* __restrict__ p, bool there, bool aligned, float (&x)[16]) {
+    if (!there) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[e] = 0.0f;
+    } else if (!aligned) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[e] = to_f32(p[e]);
+    } else if (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float4 v = reinterpret_cast<const float4*>(p)[i];
+            x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+            const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[8 * i + 2 * e] = __uint_as_float(w[e] << 16);
+                x[8 * i + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+            }
+        }
+    }
 }
 
 // Where a block's queries stand: `n` new tokens from row `row0` on, the first at position `before` of request `seq`.
@@ -119,9 +148,35 @@ __device__ __forceinline__ void finish(const Args& a, float O, float L, float M,
     ((T*)a.out)[(size_t)row * a.ld_out + (size_t)h * a.head_dim + d] = from_f32<T>(y);
 }
 
-// DMAX: 64, 128 or 256, the head size rounded up; NT: column tiles of 8; KT: key tiles of 16 that a warp takes at a time.
-template <typename T, int CODE, int DMAX, int NT, int KT>
-__global__ void __launch_bounds__(WARPS * 32)
+constexpr float RESCALE = 8.0f;          // how far (in the exponent) a score may run ahead of the maximum its column refers to
+
+// What a warp has looked up about a run of keys in one page: where its rows start (page 0's, if it has no page), its block's scales
+// and what is made of them: ev = log2 of the value's scale, inv = 2^-ev.
+struct __align__(16) Run {
+    long long off;
+    float ks, ev;
+    float inv, vs;
+    unsigned flags, unused;
+};
+constexpr unsigned HAS_PAGE = 1;         // there is a page
+constexpr unsigned NO_POWER = 2;         // vs is not 2^ev: the weights are multiplied by it
+constexpr unsigned SEEN_BY_ALL = 4;      // every query of the block sees all keys of the tile, and scores are as they are
+constexpr unsigned SEEN_BY_ONE = 8;      // every key of the tile is seen by one query or more
+
+// ev and inv of a value's scale.  Of one that is not finite ev = 0, so that its weights are NaN and the others stay numbers.
+__device__ __forceinline__ unsigned power_of(float vs, float& ev, float& inv) {
+    const unsigned bits = __float_as_uint(vs);
+    const int e = (int)(bits >> 23) & 255;
+    ev = e == 255 ? 0.0f : (float)(e - 127);
+    inv = e == 255 ? 1.0f : e == 0 ? 1.7014118e38f : __uint_as_float((unsigned)max(254 - e, 0) << 23);
+    return e == 255 || e == 0 || (bits & 0x807fffffu) ? NO_POWER : 0u;
+}
+
+// WARPS: of a block; DMAX: 64, 128 or 256, the head size rounded up; DK: the head size, or 0 where it is known at run time only; NT: column tiles of
+// 8; KT: key tiles of 16 that a warp takes at a time; RUN: 16 or 8, pages are a multiple of it, so that a tile or half a tile lies in
+// one page; 0: every row is looked up by itself.
+template <typename T, int CODE, int WARPS, int DMAX, int DK, int NT, int KT, int RUN>
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 && RUN && DMAX < 256 ? DK ? 16 : 12 : 1)
 attention_8bit_kernel(const __grid_constant__ Args a) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1;            // pieces a number is split into
     constexpr int QT = 8 * NT / P;                       // queries of a block
@@ -129,78 +184,36 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
     constexpr int Q2 = 2 / P;                            // queries in a lane's two columns of a tile
     __shared__ float sm_o[WARPS][QT][DMAX + 1];
     __shared__ float sm_m[WARPS][QT], sm_l[WARPS][QT];
+    constexpr int HALVES = RUN == 16 ? 1 : 2;            // runs of a tile
+    __shared__ Run known[RUN ? WARPS : 1][RUN ? 32 * HALVES : 1];
 
     pdl_launch_dependents();
     pdl_wait();
-    const int z = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x % a.num_splits, tile = blockIdx.x / a.num_splits;
+    const int z = blockIdx.z, kvh = blockIdx.y;
+    const int tile = a.num_splits == 1 ? blockIdx.x : blockIdx.x / a.num_splits, split = blockIdx.x - tile * a.num_splits;
     const Portion at = portion_of(a, z);
     const int group = a.n_heads / a.n_kv_heads;
     const int n_queries = min(QT, at.n * group - tile * QT);         // of this block
     if (n_queries <= 0) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int D = a.head_dim, ps = a.page_size;
+    const int D = DK ? DK : a.head_dim, ps = a.page_size;
+    // query qi of the (request, key/value head): which of its tokens, which head of the group
+    const bool single = !a.q_start || group == 1;
+    auto token_of = [&](int qi) { return a.q_start ? single ? qi : qi / group : 0; };
+    auto head_of = [&](int qi) { return kvh * group + (a.q_start ? single ? 0 : qi % group : qi); };
 
-    // ---- q: column g of every tile, as the second operand ------------------------------------------------------
-    unsigned qf[NT][CH * 4][2];
-    float my_factor[NT];                                 // of column g
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int i = (n * 8 + g) / P, qi = tile * QT + i;
-        const bool there = i < n_queries;
-        const T* src = (const T*)a.q + (size_t)(at.row0 + (there ? qi / group : 0)) * a.ld_q + (size_t)(kvh * group + (there ? qi % group : 0)) * D;
-        unsigned amax = 0;
-#pragma unroll
-        for (int c = 0; c < CH; c++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int d = 64 * c + 16 * t + e;
-                if (there && 64 * c + 16 * t < D) amax = max(amax, __float_as_uint(to_f32(src[d])) & 0x7fffffffu);
-            }
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const int e2 = max(-100, min(120, (int)(amax >> 23) - 127));
-        const float down = __uint_as_float((unsigned)(127 - e2) << 23);
-        my_factor[n] = __uint_as_float((unsigned)(127 + e2) << 23) * a.scale;
-#pragma unroll
-        for (int c = 0; c < CH; c++)
-#pragma unroll
-            for (int w = 0; w < 8; w++) {                // word w: dims 64 c + 16 t + 2 w, + 1; k-step w / 2
-                float x0 = 0.0f, x1 = 0.0f;
-                if (there && 64 * c + 16 * t < D) {
-                    x0 = to_f32(src[64 * c + 16 * t + 2 * w]) * down;
-                    x1 = to_f32(src[64 * c + 16 * t + 2 * w + 1]) * down;
-                }
-                if (P == 2 && (g & 1)) {                 // the second piece: what the first one leaves
-                    x0 -= __half2float(__float2half_rn(x0));
-                    x1 -= __half2float(__float2half_rn(x1));
-                }
-                qf[n][c * 4 + (w >> 1)][w & 1] = pack_half(x0, x1);
-            }
-    }
-    // the lane's two columns 2t, 2t + 1 of every tile: one query each, or the two pieces of one
-    float factor[NT][Q2];
-    int pos[NT][Q2], lo[NT][Q2];
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int e = 0; e < Q2; e++) {
-            const int i = (n * 8 + 2 * t) / P + e;
-            factor[n][e] = __shfl_sync(0xffffffffu, my_factor[n], (2 * t + e) * 4);
-            pos[n][e] = i < n_queries ? at.before + (tile * QT + i) / group : -1;
-            lo[n][e] = first_key(a, max(pos[n][e], 0));
-        }
-
+    const bool plain = a.softcap == 0.0f && !a.dist_bias;            // a score is S times its factors
     // ---- the block's keys, as tiles of 16 positions: kept first ones, then from the first query's first to the last query's own ----
-    const int pos_first = at.before + tile * QT / group, pos_last = at.before + (tile * QT + n_queries - 1) / group;
-    const int lo_first = first_key(a, max(pos_first, 0));
+    const int pos_first = at.before + token_of(tile * QT), pos_last = at.before + token_of(tile * QT + n_queries - 1);
+    const int lo_first = first_key(a, max(pos_first, 0)), lo_last = first_key(a, max(pos_last, 0));
     const int kept_tiles = lo_first > 0 ? min((a.keep_first + 15) >> 4, lo_first >> 4) : 0;
-    const bool known = (unsigned)at.seq < (unsigned)a.n_seqs;
-    if (!known && tid == 0 && a.status) atomicOr(a.status, 16);
-    const int n_tiles = known && pos_last >= 0 ? kept_tiles + (pos_last >> 4) - (lo_first >> 4) + 1 : 0;
-    const int per_split = ((n_tiles + a.num_splits - 1) / a.num_splits + KT - 1) / KT * KT;
-    const int tile_end = min(n_tiles, (split + 1) * per_split);
-    const int* table = a.block_table + (size_t)(known ? at.seq : 0) * a.max_blocks;
-    const bool whole_pages = (ps & 15) == 0;             // a tile of 16 keys lies in one page
+    const bool request = (unsigned)at.seq < (unsigned)a.n_seqs;
+    if (!request && tid == 0 && a.status) atomicOr(a.status, 16);
+    const int n_tiles = request && pos_last >= 0 ? kept_tiles + (pos_last >> 4) - (lo_first >> 4) + 1 : 0;
+    const int tile_end = split == a.num_splits - 1 ? n_tiles : min(n_tiles, (split + 1) * a.split_tiles);
+    const int* table = a.block_table + (size_t)(request ? at.seq : 0) * a.max_blocks;
+    const size_t head_at = (size_t)kvh * ps * D;
+    auto seen = [&](int j) { return j <= pos_last && (j >= lo_first || j < a.keep_first); };      // by any of the block's queries
 
     float o[CH * 4][NT][4];
     float M[NT][Q2], l[NT][Q2];
@@ -216,68 +229,180 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
             l[n][e] = 0.0f;
         }
     }
-    const size_t head_at = (size_t)kvh * ps * D;
 
-    for (int it = split * per_split + warp * KT; it < tile_end; it += WARPS * KT) {
-        uint4 kw[KT][2][CH];                              // keys g, g + 8: dims 64 c + 16 t ..
-        uint2 vw[KT][4][CH];                              // keys 2t, 2t + 1, 2t + 8, 2t + 9: dims 64 c + 8 g ..
-        float ks[KT][2], vs[KT][2];                       // scales of keys g, g + 8
-        int key0[KT];                                     // the tile's first position
-        unsigned there = 0;                               // bit 2 kt + r: key g + 8 r of tile kt has a page
-        // A tile's loads: which key, its page, then codes and scales.  Rows that no query of the block sees are zeros.
+    // This warp's tiles: KT at a time, the first at `tile0`, then every WARPS * KT-th group.
+    const int tile0 = split * a.split_tiles + warp * KT;
+    const int n_groups = tile0 < tile_end ? (tile_end - tile0 + WARPS * KT - 1) / (WARPS * KT) : 0;
+    auto nth_of = [&](int group_at, int kt) { return tile0 + group_at * WARPS * KT + kt; };
+    auto first_of = [&](int nth) { return (nth < kept_tiles ? nth : nth - kept_tiles + (lo_first >> 4)) << 4; };
+
+    // the next 32 tiles' pages and scales, one tile a lane, for all lanes to read
+    auto look_up = [&](int group_at) {
+        __syncwarp();
+        const int nth = nth_of(group_at + lane / KT, lane % KT), key0 = first_of(nth);
+        const unsigned tile_flags = (key0 + 15 <= pos_first && key0 >= lo_last && plain ? SEEN_BY_ALL : 0) |
+                                    (key0 + 15 <= pos_last && key0 >= lo_first ? SEEN_BY_ONE : 0);
 #pragma unroll
-        for (int kt = 0; kt < KT; kt++) {
-            const int nth = it + kt;
-            key0[kt] = (nth < kept_tiles ? nth : nth - kept_tiles + (lo_first >> 4)) << 4;
-            const bool in = nth < tile_end;
-            auto seen = [&](int j) { return in && j <= pos_last && (j >= lo_first || j < a.keep_first); };
-            int tile_page = -1, slot0 = 0;
-            if (whole_pages && in) {
-                const int b = key0[kt] / ps;
-                slot0 = key0[kt] - b * ps;
-                tile_page = b < a.max_blocks ? table[b] : -1;
+        for (int r = 0; r < HALVES; r++) {
+            Run run = {0, 0.0f, 0.0f, 0.0f, 0.0f, tile_flags, 0};
+            const int j = key0 + 8 * r;
+            if (nth < tile_end && j <= pos_last && (j + RUN - 1 >= lo_first || j < a.keep_first)) {
+                const int b = j / ps;
+                const int page = b < a.max_blocks ? table[b] : -1;
+                if (page >= 0 && page < a.num_pages) {
+                    run.off = page * a.page_stride + (long long)(head_at + (size_t)(j - b * ps) * D);
+                    run.ks = a.k_scale[page * a.scale_stride + kvh];
+                    run.vs = a.v_scale[page * a.scale_stride + kvh];
+                    run.flags |= HAS_PAGE | power_of(run.vs, run.ev, run.inv);
+                } else if (a.status) {
+                    atomicOr(a.status, 16);
+                }
             }
-            auto row_of = [&](int j, size_t& off, int& page) {       // false: no such row
-                int slot = slot0 + (j - key0[kt]);
-                page = tile_page;
-                if (!seen(j)) return false;
-                if (!whole_pages) {
-                    const int b = j / ps;
-                    slot = j - b * ps;
-                    page = b < a.max_blocks ? table[b] : -1;
-                }
-                if (page < 0 || page >= a.num_pages) {
-                    if (a.status) atomicOr(a.status, 16);
-                    return false;
-                }
-                off = (size_t)page * a.page_stride + head_at + (size_t)slot * D;
-                return true;
-            };
+            known[warp][HALVES * lane + r] = run;
+        }
+        __syncwarp();
+    };
+    // RUN 0: the row of key j, if a query sees it and it has a page
+    auto row_of = [&](int nth, int j, size_t& off, int& page) {
+        if (nth >= tile_end || !seen(j)) return false;
+        const int b = j / ps;
+        page = b < a.max_blocks ? table[b] : -1;
+        if (page < 0 || page >= a.num_pages) {
+            if (a.status) atomicOr(a.status, 16);
+            return false;
+        }
+        off = (size_t)page * a.page_stride + head_at + (size_t)(j - b * ps) * D;
+        return true;
+    };
+
+    uint4 kw[KT][2][CH];                                  // keys g, g + 8: dims 64 c + 16 t ..
+    uint2 vw[KT][4][CH];                                  // keys 2t, 2t + 1, 2t + 8, 2t + 9: dims 64 c + 8 g ..
+    // of keys g and g + 8 (RUN 16: of both) of a group's tiles: scales and what is made of them, flags
+    constexpr int R = RUN == 16 ? 1 : 2;
+    auto load_keys = [&](int group_at, float (&ks)[KT][R], float (&ev)[KT][R], unsigned (&flags)[KT][R], float (&inv)[KT][R], float (&vs)[KT][R]) {
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                size_t off = 0;
-                int page = 0;
-                const bool ok = row_of(key0[kt] + g + 8 * r, off, page);
-                if (ok) there |= 1u << (2 * kt + r);
-                ks[kt][r] = ok ? a.k_scale[(size_t)page * a.scale_stride + kvh] : 0.0f;
-                vs[kt][r] = ok ? a.v_scale[(size_t)page * a.scale_stride + kvh] : 0.0f;
+                if constexpr (RUN != 0) {
+                    const Run& run = known[warp][((group_at * KT + kt) & 31) * HALVES + (RUN == 16 ? 0 : r)];
+                    if (RUN != 16 || r == 0) {
+                        ks[kt][r] = run.ks;
+                        ev[kt][r] = run.ev;
+                        inv[kt][r] = run.inv;
+                        vs[kt][r] = run.vs;
+                        flags[kt][r] = run.flags;
+                    }
+                    // rows that no query sees are read too: their scores are left out
+                    const uint8_t* p = a.k + run.off + (g + (RUN == 16 ? 8 * r : 0)) * D + 16 * t;
 #pragma unroll
-                for (int c = 0; c < CH; c++)
-                    kw[kt][r][c] = ok && 64 * c + 16 * t < D ? __ldg(reinterpret_cast<const uint4*>(a.k + off + 64 * c + 16 * t))
-                                                            : make_uint4(0u, 0u, 0u, 0u);
+                    for (int c = 0; c < CH; c++)
+                        kw[kt][r][c] = DK || 64 * c + 16 * t < D ? __ldg(reinterpret_cast<const uint4*>(p + 64 * c)) : make_uint4(0u, 0u, 0u, 0u);
+                } else {
+                    const int nth = nth_of(group_at, kt);
+                    size_t off = 0;
+                    int page = 0;
+                    const bool ok = row_of(nth, first_of(nth) + g + 8 * r, off, page);
+                    ks[kt][r % R] = ok ? a.k_scale[(size_t)page * a.scale_stride + kvh] : 0.0f;
+                    vs[kt][r % R] = ok ? a.v_scale[(size_t)page * a.scale_stride + kvh] : 0.0f;
+                    flags[kt][r % R] = power_of(vs[kt][r % R], ev[kt][r % R], inv[kt][r % R]) | (ok ? HAS_PAGE : 0u);
+#pragma unroll
+                    for (int c = 0; c < CH; c++)
+                        kw[kt][r][c] = ok && 64 * c + 16 * t < D ? __ldg(reinterpret_cast<const uint4*>(a.k + off + 64 * c + 16 * t))
+                                                                : make_uint4(0u, 0u, 0u, 0u);
+                }
             }
+    };
+    auto load_values = [&](int group_at) {
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                size_t off = 0;
-                int page = 0;
-                const bool ok = row_of(key0[kt] + 2 * t + (r & 1) + 8 * (r >> 1), off, page);
+                if constexpr (RUN != 0) {
+                    const Run& run = known[warp][((group_at * KT + kt) & 31) * HALVES + (RUN == 16 ? 0 : r >> 1)];
+                    const uint8_t* p = a.v + run.off + (2 * t + (r & 1) + (RUN == 16 ? 8 * (r >> 1) : 0)) * D + 8 * g;
 #pragma unroll
-                for (int c = 0; c < CH; c++)
-                    vw[kt][r][c] = ok && 64 * c + 8 * g < D ? __ldg(reinterpret_cast<const uint2*>(a.v + off + 64 * c + 8 * g)) : make_uint2(0u, 0u);
+                    for (int c = 0; c < CH; c++)
+                        vw[kt][r][c] = DK || 64 * c + 8 * g < D ? __ldg(reinterpret_cast<const uint2*>(p + 64 * c)) : make_uint2(0u, 0u);
+                } else {
+                    const int nth = nth_of(group_at, kt);
+                    size_t off = 0;
+                    int page = 0;
+                    const bool ok = row_of(nth, first_of(nth) + 2 * t + (r & 1) + 8 * (r >> 1), off, page);
+#pragma unroll
+                    for (int c = 0; c < CH; c++)
+                        vw[kt][r][c] = ok && 64 * c + 8 * g < D ? __ldg(reinterpret_cast<const uint2*>(a.v + off + 64 * c + 8 * g)) : make_uint2(0u, 0u);
+                }
             }
+    };
+
+    float ks_next[KT][R], ev_next[KT][R], inv_next[KT][R], vs_next[KT][R];
+    unsigned flags_next[KT][R];
+    if (n_groups > 0) {
+        if constexpr (RUN != 0) look_up(0);
+        load_keys(0, ks_next, ev_next, flags_next, inv_next, vs_next);
+        load_values(0);
+    }
+    // ---- q: column g of every tile, as the second operand ------------------------------------------------------
+    unsigned qf[NT][CH * 4][2];
+    float my_factor[NT];                                 // of column g
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int i = (n * 8 + g) / P, qi = tile * QT + (i < n_queries ? i : 0);
+        const T* src = (const T*)a.q + (size_t)(at.row0 + token_of(qi)) * a.ld_q + (size_t)head_of(qi) * D;
+        float x[CH][16];                                 // dims 64 c + 16 t ..
+        unsigned amax = 0;
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            load16(src + 64 * c + 16 * t, i < n_queries && 64 * c + 16 * t < D, a.q_aligned, x[c]);
+#pragma unroll
+            for (int e = 0; e < 16; e++) amax = max(amax, __float_as_uint(x[c][e]) & 0x7fffffffu);
+        }
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const int e2 = max(-100, min(120, (int)(amax >> 23) - 127));
+        const float down = __uint_as_float((unsigned)(127 - e2) << 23);
+        my_factor[n] = __uint_as_float((unsigned)(127 + e2) << 23) * a.scale;
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+            for (int w = 0; w < 8; w++) {                // word w: dims 64 c + 16 t + 2 w, + 1; k-step w / 2
+                float x0 = x[c][2 * w] * down, x1 = x[c][2 * w + 1] * down;
+                if (P == 2 && (g & 1)) {                 // the second piece: what the first one leaves
+                    x0 -= __half2float(__float2half_rn(x0));
+                    x1 -= __half2float(__float2half_rn(x1));
+                }
+                qf[n][c * 4 + (w >> 1)][w & 1] = pack_half(x0, x1);
+            }
+    }
+    // the lane's two columns 2t, 2t + 1 of every tile: one query each, or the two pieces of one
+    float factor[NT][Q2];                                // S times this and the key's scale: a score, in units of log 2 if `plain`
+    int pos[NT][Q2], lo[NT][Q2];
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < Q2; e++) {
+            const int i = (n * 8 + 2 * t) / P + e;
+            factor[n][e] = __shfl_sync(0xffffffffu, my_factor[n], (2 * t + e) * 4) * (plain ? LOG2E : 1.0f);
+            pos[n][e] = i < n_queries ? at.before + token_of(tile * QT + i) : -1;
+            lo[n][e] = first_key(a, max(pos[n][e], 0));
         }
 
-        // ---- S, and the scores in units of log 2 -----------------------------------------------------------------
+    for (int it = 0; it < n_groups; it++) {
+        float ks[KT][R], ev[KT][R], inv[KT][R], vs[KT][R];
+        unsigned flags[KT][R];
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                ks[kt][r] = ks_next[kt][r];
+                ev[kt][r] = ev_next[kt][r];
+                inv[kt][r] = inv_next[kt][r];
+                vs[kt][r] = vs_next[kt][r];
+                flags[kt][r] = flags_next[kt][r];
+            }
+
+    // ---- S; the keys' registers are free after it, and the next group's keys are asked for -------------------
         float sc[KT][NT][4];
 #pragma unroll
         for (int kt = 0; kt < KT; kt++) {
@@ -299,74 +424,109 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                 }
             }
         }
-        float x[KT][NT][2][Q2], top[NT][Q2];              // [tile][column tile][key g, g + 8][query]
+        if (it + 1 < n_groups) {
+            if constexpr (RUN != 0)
+                if ((((it + 1) * KT) & 31) == 0) look_up(it + 1);
+            load_keys(it + 1, ks_next, ev_next, flags_next, inv_next, vs_next);
+        }
+
+        // ---- x = score + log2 of the value's scale, -inf where the key is not seen ------------------------------------
+        float top[NT][Q2];
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < Q2; e++) top[n][e] = M[n][e];
+            for (int e = 0; e < Q2; e++) top[n][e] = -INFINITY;
 #pragma unroll
-        for (int kt = 0; kt < KT; kt++)
+        for (int kt = 0; kt < KT; kt++) {
+            const bool all = RUN && (flags[kt][0] & SEEN_BY_ALL) && (flags[kt][0] & flags[kt][R - 1] & HAS_PAGE);
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const int j = key0[kt] + g + 8 * r;
-                const bool ok = (there >> (2 * kt + r)) & 1;
-                // log2 of the value's scale; of one that is not finite 0, so that its weight is NaN and the others stay numbers
-                const int exponent = (int)(__float_as_uint(vs[kt][r]) >> 23) & 255;
-                const float ev = exponent == 255 ? 0.0f : (float)(exponent - 127);
+            for (int r = 0; r < 2; r++)
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int e = 0; e < Q2; e++) {
-                        float s = (P == 2 ? sc[kt][n][2 * r] + sc[kt][n][2 * r + 1] : sc[kt][n][2 * r + e]) * (ks[kt][r] * factor[n][e]);
-                        if (a.softcap > 0.0f) s = a.softcap * (P == 2 ? tanhf(s / a.softcap) : tanh_fast(s / a.softcap));
-                        const bool visible = ok && j <= pos[n][e] && (j >= lo[n][e] || j < a.keep_first);
-                        if (a.dist_bias && visible) {
-                            const int h = kvh * group + (tile * QT + (n * 8 + 2 * t) / P + e) % group;
-                            s += a.dist_bias[(size_t)h * a.n_dist + min(pos[n][e] - j, a.n_dist - 1)];
+                        float x = P == 2 ? sc[kt][n][2 * r] + sc[kt][n][2 * r + 1] : sc[kt][n][2 * r + e];
+                        if (all) {
+                            x = fmaf(x, ks[kt][r % R] * factor[n][e], ev[kt][r % R]);
+                        } else {
+                            const int j = first_of(nth_of(it, kt)) + g + 8 * r;
+                            const bool visible = (flags[kt][r % R] & HAS_PAGE) && j <= pos[n][e] && (j >= lo[n][e] || j < a.keep_first);
+                            x *= ks[kt][r % R] * factor[n][e];
+                            if (!plain) {
+                                if (a.softcap > 0.0f) x = a.softcap * (P == 2 ? tanhf(x / a.softcap) : tanh_fast(x / a.softcap));
+                                if (a.dist_bias && visible)
+                                    x += a.dist_bias[(size_t)head_of(tile * QT + (n * 8 + 2 * t) / P + e) * a.n_dist + min(pos[n][e] - j, a.n_dist - 1)];
+                                x *= LOG2E;
+                            }
+                            x = visible ? x + ev[kt][r % R] : -INFINITY;
                         }
-                        s = visible ? s * LOG2E : -INFINITY;
-                        x[kt][n][r][e] = s;
-                        top[n][e] = fmaxf(top[n][e], s + ev);
+                        sc[kt][n][P == 2 ? 2 * r : 2 * r + e] = x;
+                        top[n][e] = fmaxf(top[n][e], x);
                     }
-            }
-        // ---- the running maximum; weights; P as the second operand ---------------------------------------------
+        }
+        // The column's reference moves when a score has run far ahead of it (always on the first keys), for the whole warp together.
+        bool move = false;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < Q2; e++) {
-                const float m = max_over_groups(top[n][e]);
-                const float shrink = m == -INFINITY ? 1.0f : ex2(M[n][e] - m);
-                M[n][e] = m;
-                l[n][e] *= shrink;
+            for (int e = 0; e < Q2; e++) move |= top[n][e] > M[n][e] + RESCALE;
+        if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-                for (int j = 0; j < CH * 4; j++) {
-                    o[j][n][e] *= shrink;
-                    o[j][n][e + 2] *= shrink;
-                    if (P == 2) {
-                        o[j][n][1] *= shrink;
-                        o[j][n][3] *= shrink;
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < Q2; e++) {
+                    const float m = fmaxf(M[n][e], max_over_groups(top[n][e]));
+                    const float shrink = m == -INFINITY ? 1.0f : ex2(M[n][e] - m);
+                    M[n][e] = m;
+                    l[n][e] *= shrink;
+#pragma unroll
+                    for (int j = 0; j < CH * 4; j++) {
+                        o[j][n][e] *= shrink;
+                        o[j][n][e + 2] *= shrink;
+                        if (P == 2) {
+                            o[j][n][1] *= shrink;
+                            o[j][n][3] *= shrink;
+                        }
                     }
                 }
-            }
+        }
+        float m_use[NT][Q2];                              // a column that has seen no key yet: its weights are 2^-inf
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < Q2; e++) m_use[n][e] = M[n][e] == -INFINITY ? 0.0f : M[n][e];
+        // ---- weights, as the second operand; O ---------------------------------------------------------------------
 #pragma unroll
         for (int kt = 0; kt < KT; kt++) {
             unsigned pf[NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int r = 0; r < 2; r++)
 #pragma unroll
-                for (int r = 0; r < 2; r++) {
+                for (int n = 0; n < NT; n++) {
+                    // 2^(x - M) is the weight times the value's scale, where that is a power of two: what appending gives
                     float w[2];
 #pragma unroll
                     for (int e = 0; e < Q2; e++) {
-                        const float s = x[kt][n][r][e];
-                        const bool none = s == -INFINITY;                        // not visible, or a score that weighs nothing
-                        const float p = none ? 0.0f : ex2(s - M[n][e]);
-                        l[n][e] += p;
-                        w[e] = none ? 0.0f : p * vs[kt][r];
+                        const float x = sc[kt][n][P == 2 ? 2 * r : 2 * r + e];
+                        w[e] = ex2(x - m_use[n][e]);
+                        l[n][e] = fmaf(w[e], inv[kt][r % R], l[n][e]);
+                        if (flags[kt][r % R] & NO_POWER) w[e] = x == -INFINITY ? 0.0f : w[e] * inv[kt][r % R] * vs[kt][r % R];
                     }
                     if (P == 2) w[1] = w[0] - __half2float(__float2half_rn(w[0]));
                     pf[n][r] = turn(pack_half(w[0], w[1]));
                 }
+            if constexpr (RUN != 0) {
+                // Values of rows that no query sees become zeros: a weight of 0 times what such a row may hold would be NaN.
+                if (!(flags[kt][0] & SEEN_BY_ONE) || !(flags[kt][0] & flags[kt][R - 1] & HAS_PAGE)) {
+                    const int key0 = first_of(nth_of(it, kt));
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (!(flags[kt][(r >> 1) % R] & HAS_PAGE) || !seen(key0 + 2 * t + (r & 1) + 8 * (r >> 1))) {
+#pragma unroll
+                            for (int c = 0; c < CH; c++) vw[kt][r][c] = make_uint2(0u, 0u);
+                        }
+                }
+            }
 #pragma unroll
             for (int c = 0; c < CH; c++)
 #pragma unroll
@@ -388,6 +548,7 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                     for (int n = 0; n < NT; n++) mma_f16(o[c * 4 + half * 2 + 1][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
                 }
         }
+        if (it + 1 < n_groups) load_values(it + 1);
     }
 
     // ---- the warps' states in shared memory, joined in their order ------------------------------------------------
@@ -397,19 +558,21 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
         for (int e = 0; e < Q2; e++) {
             const int i = (n * 8 + 2 * t) / P + e;
             const float sum = sum_over_groups(l[n][e]);
-            if (g == 0) {
-                sm_m[warp][i] = M[n][e];
-                sm_l[warp][i] = sum;
+            if (i < n_queries) {
+                if (g == 0) {
+                    sm_m[warp][i] = M[n][e];
+                    sm_l[warp][i] = sum;
+                }
+#pragma unroll
+                for (int j = 0; j < CH * 4; j++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++)          // product j of a run of 64: dims 8 g + 2 j, + 1
+                        sm_o[warp][i][(j >> 2) * 64 + 8 * g + 2 * (j & 3) + r] = P == 2 ? o[j][n][2 * r] + o[j][n][2 * r + 1] : o[j][n][2 * r + e];
             }
-#pragma unroll
-            for (int j = 0; j < CH * 4; j++)
-#pragma unroll
-                for (int r = 0; r < 2; r++)              // product j of a run of 64: dims 8 g + 2 j, + 1
-                    sm_o[warp][i][(j >> 2) * 64 + 8 * g + 2 * (j & 3) + r] = P == 2 ? o[j][n][2 * r] + o[j][n][2 * r + 1] : o[j][n][2 * r + e];
         }
     __syncthreads();
     for (int idx = tid; idx < n_queries * D; idx += WARPS * 32) {
-        const int i = idx / D, d = idx % D, qi = tile * QT + i;
+        const int i = idx / D, d = idx - i * D, qi = tile * QT + i;
         float m = -INFINITY, L = 0.0f, O = 0.0f;
 #pragma unroll
         for (int w = 0; w < WARPS; w++) m = fmaxf(m, sm_m[w][i]);
@@ -420,11 +583,11 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
             L = fmaf(sm_l[w][i], f, L);
             O = fmaf(sm_o[w][i][d], f, O);
         }
+        const int row = at.row0 + token_of(qi), h = head_of(qi);
         if (a.num_splits == 1) {
-            finish<T>(a, O, L, m, at.row0 + qi / group, kvh * group + qi % group, d);
+            finish<T>(a, O, L, m, row, h, d);
         } else {
-            const size_t row = ((size_t)(at.row0 + qi / group) * a.n_heads + kvh * group + qi % group) * a.num_splits + split;
-            float* part = a.scratch + row * (D + 2);
+            float* part = a.scratch + (((size_t)row * a.n_heads + h) * a.num_splits + split) * (D + 2);
             part[d] = O;
             if (d == 0) {
                 part[D] = m;
@@ -434,29 +597,46 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
     }
 }
 
-// The splits' partial results of a (row, head), joined in their order: one warp each.
+// The splits' partial results of a (row, head), joined in a fixed order: one block each.  The splits' factors meet in shared memory;
+// then every thread sums its dims (at heads of 64 two threads share one, every other split each), eight splits at a time on their way.
+constexpr int MAX_SPLITS = 256;
+
 template <typename T>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args a, int n_z) {
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args a) {
+    __shared__ float factor[MAX_SPLITS];
+    __shared__ float scratch[32];
+    __shared__ float other[128];
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x & 31;
+    const int tid = threadIdx.x, D = a.head_dim, h = blockIdx.x % a.n_heads, nth = blockIdx.x / a.n_heads;
     const Portion at = portion_of(a, blockIdx.y);
-    const int unit = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (unit >= at.n * a.n_heads) return;
-    const int row = at.row0 + unit / a.n_heads, h = unit % a.n_heads, D = a.head_dim;
+    if (nth >= at.n) return;
+    const int row = at.row0 + nth;
     const float* part = a.scratch + ((size_t)row * a.n_heads + h) * a.num_splits * (D + 2);
-    float m = -INFINITY;
-    for (int s = lane; s < a.num_splits; s += 32) m = fmaxf(m, part[(size_t)s * (D + 2) + D]);
-    m = warp_max(m);
-    for (int d = lane; d < D; d += 32) {
-        float L = 0.0f, O = 0.0f;
-        for (int s = 0; s < a.num_splits; s++) {
-            const float* p = part + (size_t)s * (D + 2);
-            const float f = p[D] == -INFINITY ? 1.0f : ex2(p[D] - m);
-            L = fmaf(p[D + 1], f, L);
-            O = fmaf(p[d], f, O);
+    float m = -INFINITY, L = 0.0f;
+    for (int s = tid; s < a.num_splits; s += 128) m = fmaxf(m, part[(size_t)s * (D + 2) + D]);
+    m = block_max(m, scratch);
+    for (int s = tid; s < a.num_splits; s += 128) {
+        const float ms = part[(size_t)s * (D + 2) + D];
+        const float f = ms == -INFINITY ? 1.0f : ex2(ms - m);       // no key: zeros; NaN: no maximum, and it counts
+        factor[s] = f;
+        L = fmaf(part[(size_t)s * (D + 2) + D + 1], f, L);
+    }
+    L = block_sum(L, scratch);                                       // factor is there for all after it
+    const int shares = D <= 64 ? 2 : 1, width = 128 / shares, share = tid / width;
+    for (int d0 = 0; d0 < D; d0 += width) {
+        const int d = d0 + tid % width;
+        float O = 0.0f;
+        if (d < D) {
+#pragma unroll 8
+            for (int s = share; s < a.num_splits; s += shares) O = fmaf(part[(size_t)s * (D + 2) + d], factor[s], O);
         }
-        finish<T>(a, O, L, m, row, h, d);
+        if (shares == 2) {
+            other[tid] = O;
+            __syncthreads();
+            if (share == 0) O += other[tid + width];
+        }
+        if (d < D && share == 0) finish<T>(a, O, L, m, row, h, d);
     }
 }
 
@@ -465,51 +645,65 @@ int launch(const Args& a, int n_z, int max_queries, int max_n, cudaStream_t stre
     constexpr int P = sizeof(T) == 4 ? 2 : 1;
     const bool wide = max_queries * P > 8;               // more columns than one tile has
     int e;
-#define RUN(DMAX, NT, KT)                                                                                                        \
-    e = sandy_launch(attention_8bit_kernel<T, CODE, DMAX, NT, KT>,                                                               \
+#define LAUNCH(WARPS, DMAX, DK, NT, KT, RUN)                                                                                            \
+    e = sandy_launch(attention_8bit_kernel<T, CODE, WARPS, DMAX, DK, NT, KT, RUN>,                                                      \
                      dim3((unsigned)((max_queries + 8 * NT / P - 1) / (8 * NT / P) * a.num_splits), a.n_kv_heads, n_z), dim3(WARPS * 32), 0, \
                      stream, a)
-    if (a.head_dim <= 64) {
-        if (wide) RUN(64, 4, 2);
-        else RUN(64, 1, 4);
+    if (a.page_size % 8 != 0) {                          // rows one by one
+        if (a.head_dim <= 64) LAUNCH(1, 64, 0, 1, 1, 0);
+        else if (a.head_dim <= 128) LAUNCH(1, 128, 0, 1, 1, 0);
+        else LAUNCH(1, 256, 0, 1, 1, 0);
+    } else if (a.page_size % 16 == 0 && a.head_dim == 64) {
+        if (wide) LAUNCH(4, 64, 64, 4, 1, 16);
+        else LAUNCH(1, 64, 64, 1, 2, 16);
+    } else if (a.page_size % 16 == 0 && a.head_dim == 128) {
+        if (wide) LAUNCH(4, 128, 128, 2, 1, 16);
+        else LAUNCH(1, 128, 128, 1, 1, 16);
+    } else if (a.head_dim <= 64) {
+        if (wide) LAUNCH(4, 64, 0, 4, 1, 8);
+        else LAUNCH(1, 64, 0, 1, 2, 8);
     } else if (a.head_dim <= 128) {
-        if (wide) RUN(128, 2, 1);
-        else RUN(128, 1, 2);
+        if (wide) LAUNCH(4, 128, 0, 2, 1, 8);
+        else LAUNCH(1, 128, 0, 1, 1, 8);
     } else {
-        RUN(256, 1, 1);
+        LAUNCH(1, 256, 0, 1, 1, 8);
     }
-#undef RUN
+#undef LAUNCH
     if (e != SANDY_OK || a.num_splits == 1) return e;
-    return sandy_launch(join_kernel<T>, dim3((unsigned)(((long long)max_n * a.n_heads + 3) / 4), n_z), dim3(128), 0, stream, a, n_z);
+    return sandy_launch(join_kernel<T>, dim3((unsigned)((long long)max_n * a.n_heads), n_z), dim3(128), 0, stream, a);
 }
 
 }  // namespace
 
-// How many blocks share a request's keys: as many as give every SM some four blocks, none with fewer than 16 keys x 16.
+// How many blocks share a request's keys (max_keys: the most that one of its queries may see).  Single tokens' blocks are one warp,
+// of which an SM holds sixteen: as many as fill the SMs once, none with fewer than 128 keys.  A portion's blocks are four warps.
 SANDY_API int sandy_attention_8bit_splits(int n_z, int max_n, int n_heads, int n_kv_heads, int head_dim, int max_keys, int dtype) {
     if (n_z < 1 || max_n < 1 || n_kv_heads < 1 || n_heads < n_kv_heads || max_keys < 1) return 1;
     const long long queries = (long long)max_n * (n_heads / n_kv_heads), columns = queries * (dtype == SANDY_F32 ? 2 : 1);
-    const long long tile = columns <= 8 || head_dim > 128 ? 8 : head_dim <= 64 ? 32 : 16;
-    const long long blocks = (columns + tile - 1) / tile * n_kv_heads * n_z;
-    const long long wanted = ((long long)sandy_sm_count() * 4 + blocks - 1) / blocks, most = (max_keys + 255) / 256;
+    const bool narrow = columns <= 8 || head_dim > 128;
+    const long long tile = narrow ? 8 : head_dim <= 64 ? 32 : 16;
+    const long long blocks = (columns + tile - 1) / tile * n_kv_heads * n_z, room = (long long)sandy_sm_count() * (narrow ? 16 : 2);
+    const long long wanted = room / blocks, most = (max_keys + 127) / 128;
     long long splits = wanted < most ? wanted : most;
-    return (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
+    return (int)(splits < 1 ? 1 : splits > MAX_SPLITS ? MAX_SPLITS : splits);
 }
 
 // Attention of prompt portions (q_start [n_z + 1], positions = kv_before [n_z], token_seq null, request z = row z of the block
 // table; max_n: the most tokens of one) or of single tokens (q_start null: token z of request token_seq[z] at positions[z]; max_n 1).
 // q: [n_rows, H * D], out likewise, row pitches ld_q and ld_out (elements); k, v, scales and table as sandy_kv_append_8bit has them,
-// n_seqs rows in the table.  num_splits > 1 needs `scratch`: n_rows * H * num_splits * (D + 2) floats.  A row without a visible key
+// n_seqs rows in the table.  max_keys: the most keys that
+// one of a request's blocks of queries sees, by which the splits are cut; num_splits > 1 needs `scratch`: n_rows * H * num_splits * (D + 2) floats.  A row without a visible key
 // becomes zeros.  Bit 4 of *status: a visible key without a page, a token of no request, or rows past n_rows.
 SANDY_API int sandy_attention_8bit(const void* q, long long ld_q, const void* k, const void* v, const float* k_scale,
                                    const float* v_scale, long long page_stride, long long scale_stride, const int* block_table,
                                    int max_blocks, int n_seqs, const int* token_seq, const int* positions, const int* q_start, void* out,
                                    long long ld_out, int n_rows, int n_z, int max_n, int n_heads, int n_kv_heads, int head_dim,
-                                   int page_size, int num_pages, float scale, const SandyAttentionRules* rules, int num_splits, float* scratch,
+                                   int page_size, int num_pages, float scale, const SandyAttentionRules* rules, int max_keys,
+                                   int num_splits, float* scratch,
                                    int dtype, int code, int* status, cudaStream_t stream) {
     if (n_z == 0 || max_n == 0) return SANDY_OK;
     if (!rules || !q || !k || !v || !k_scale || !v_scale || !block_table || !positions || !out || !(token_seq || q_start) || n_z < 0 ||
-        max_n < 0 || n_seqs < 1 || max_blocks < 1 || page_size < 1 || num_splits < 1 || (num_splits > 1 && !scratch))
+        max_n < 0 || n_seqs < 1 || max_blocks < 1 || page_size < 1 || max_keys < 1 || num_splits < 1 || (num_splits > 1 && !scratch))
         return SANDY_ERR_ARGUMENT;
     if (rules->dist_bias && rules->n_dist < 1) return SANDY_ERR_ARGUMENT;
     if (rules->window < 0 || rules->keep_first < 0 || rules->chunk < 0 || !(rules->softcap >= 0.0f) ||
@@ -518,11 +712,15 @@ SANDY_API int sandy_attention_8bit(const void* q, long long ld_q, const void* k,
     if (head_dim < 16 || head_dim % 16 || head_dim > 256 || n_kv_heads < 1 || n_heads % n_kv_heads) return SANDY_ERR_UNSUPPORTED;
     if (page_stride % 16 || (((uintptr_t)k | (uintptr_t)v) & 15) || n_z > 65535 || n_kv_heads > 65535) return SANDY_ERR_UNSUPPORTED;
     const long long queries = (long long)max_n * (n_heads / n_kv_heads);
-    if (queries > (1 << 28) || queries * num_splits > 0x7fffffffll) return SANDY_ERR_UNSUPPORTED;
+    if (queries > (1 << 28) || queries * num_splits > 0x7fffffffll || (long long)max_n * n_heads > 0x7fffffffll || num_splits > MAX_SPLITS)
+        return SANDY_ERR_UNSUPPORTED;
+    // a split's tiles of 16 keys, an even number; two more for the ends of a window and of the kept keys
+    const int split_tiles = (((max_keys - 1) / 16 + 3 + num_splits - 1) / num_splits + 1) / 2 * 2;
     const Args a = {q, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, block_table, token_seq, positions, q_start, out, scratch,
                     status, rules->sink, rules->out_gate, rules->dist_bias, rules->elem_gate, ld_q, ld_out, page_stride, scale_stride,
-                    max_blocks, n_rows, n_seqs, n_heads, n_kv_heads, head_dim, page_size, num_pages, num_splits, rules->window,
-                    rules->keep_first, rules->chunk, rules->n_dist, rules->ld_elem_gate, rules->gate_dim, scale, rules->softcap};
+                    max_blocks, n_rows, n_seqs, n_heads, n_kv_heads, head_dim, page_size, num_pages, num_splits, split_tiles, rules->window,
+                    rules->keep_first, rules->chunk, rules->n_dist, rules->ld_elem_gate, rules->gate_dim, scale, rules->softcap,
+                    (((uintptr_t)q | (uintptr_t)(ld_q * (dtype == SANDY_F32 ? 4 : 2))) & 15) == 0};
     if (dtype == SANDY_F32 && code == SANDY_E4M3) return launch<float, SANDY_E4M3>(a, n_z, (int)queries, max_n, stream);
     if (dtype == SANDY_F32 && code == SANDY_INT8) return launch<float, SANDY_INT8>(a, n_z, (int)queries, max_n, stream);
     if (dtype == SANDY_BF16 && code == SANDY_E4M3) return launch<bf16, SANDY_E4M3>(a, n_z, (int)queries, max_n, stream);

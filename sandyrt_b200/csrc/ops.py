@@ -612,7 +612,7 @@ def _rows_of(what: str, hkv: int, d: int, *tensors) -> None:
 
 _APPEND8 = (_V, _V, _L, _L, _V, _V, _V, _V, _L, _L, _V, _I, _V, _V, _I, _I, _I, _I, _I, _I, _I, _I, _I, _V, _V)
 _READ8 = (_V, _V, _V, _V, _L, _L, _V, _I, _V, _V, _V, _V, _L, _L, _I, _I, _I, _I, _I, _I, _I, _I, _I, _V, _V)
-_ATTEND8 = (_V, _L, _V, _V, _V, _V, _L, _L, _V, _I, _I, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _I, _I, _I, _F, _V, _I, _V, _I, _I, _V, _V)
+_ATTEND8 = (_V, _L, _V, _V, _V, _V, _L, _L, _V, _I, _I, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _I, _I, _I, _F, _V, _I, _I, _V, _I, _I, _V, _V)
 
 
 def kv_append_8bit(k_src, v_src, cache: Cache8, block_table, q_start, kv_before, *, max_q_len: int) -> None:
@@ -686,8 +686,8 @@ def _attention_8bit(what, q, cache, block_table, token_seq, positions, q_start, 
         return
     if block_table.shape[0] == 0 or block_table.shape[1] == 0 or pages == 0:
         raise KernelError(f"{what}: an empty block table or cache")
-    splits = num_splits or _entry("attention_8bit", "sandy_attention_8bit_splits", (_I,) * 7)(
-        n_z, max_n, n_heads, hkv, d, min(block_table.shape[1] * ps, window + keep_first + max_n if window else 1 << 30), dtype)
+    max_keys = min(block_table.shape[1] * ps, window + keep_first + max_n if window else 1 << 30)
+    splits = num_splits or _entry("attention_8bit", "sandy_attention_8bit_splits", (_I,) * 7)(n_z, max_n, n_heads, hkv, d, max_keys, dtype)
     # partial results of the splits: memory of the stream the call is on, given back to the allocator when it returns
     scratch = torch.empty(T * n_heads * splits * (d + 2), dtype=torch.float32, device=device) if splits > 1 else None
     args = _AttentionRules(window, keep_first, softcap, chunk, _at(sink), _at(out_gate), _at(dist_bias),
@@ -696,7 +696,7 @@ def _attention_8bit(what, q, cache, block_table, token_seq, positions, q_start, 
     _run_on(device, _entry("attention_8bit", "sandy_attention_8bit", _ATTEND8),
             (q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), page_stride,
              scale_stride, block_table.data_ptr(), block_table.shape[1], block_table.shape[0], _at(token_seq), positions.data_ptr(), _at(q_start),
-             out.data_ptr(), out.stride(0), T, n_z, max_n, n_heads, hkv, d, ps, pages, scale, ctypes.addressof(args), splits, _at(scratch),
+             out.data_ptr(), out.stride(0), T, n_z, max_n, n_heads, hkv, d, ps, pages, scale, ctypes.addressof(args), max_keys, splits, _at(scratch),
              dtype, code, _status_word(device)), f"{what}(H={n_heads},Hkv={hkv},D={d},page={ps},splits={splits})")
     if splits > 1:
         global LAUNCHES

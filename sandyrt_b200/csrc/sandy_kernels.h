@@ -482,7 +482,7 @@ int sandy_attention_8bit(const void* q, long long ld_q, const void* k, const voi
                          long long page_stride, long long scale_stride, const int* block_table, int max_blocks, int n_seqs,
                          const int* token_seq, const int* positions, const int* q_start, void* out, long long ld_out, int n_rows, int n_z,
                          int max_n, int n_heads, int n_kv_heads, int head_dim, int page_size, int num_pages, float scale,
-                         const SandyAttentionRules* rules, int num_splits, float* scratch, int dtype, int code, int* status,
+                         const SandyAttentionRules* rules, int max_keys, int num_splits, float* scratch, int dtype, int code, int* status,
                          cudaStream_t stream);
 
 /* logprobs.cu */
