@@ -29,8 +29,15 @@
 // at heads of 64), so 16 warps an SM keep more than 100 KB on their way; a block's four warps take turns along the keys, and
 // `num_splits` blocks share a request's keys where there are few requests (partial results in scratch, joined by a second
 // kernel in a fixed order).  Prompt portions: the tensor cores' warp-level instructions.
+#include <algorithm>
+#include <atomic>
+
+#include <cooperative_groups.h>
+
 #include "attention_rules.h"
 #include "kv_8bit.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -47,9 +54,10 @@ struct Args {
     const float *sink, *out_gate, *dist_bias;
     const void* elem_gate;
     long long ld_q, ld_out, page_stride, scale_stride;
-    int max_blocks, n_rows, n_seqs, n_heads, n_kv_heads, head_dim, page_size, num_pages, num_splits, split_tiles;
+    int max_blocks, n_rows, n_seqs, n_heads, n_kv_heads, head_dim, page_size, num_pages, num_splits, split_tiles, group, page_shift;    // heads of a key/value head; -1: no power of two
     int window, keep_first, chunk, n_dist, ld_elem_gate, gate_dim;
     float scale, softcap;
+    bool in_cluster;                                                 // the splits of a block of queries are a cluster
     bool q_aligned;                                                  // q's rows start on 16 bytes
 };
 
@@ -163,6 +171,31 @@ constexpr unsigned NO_POWER = 2;         // vs is not 2^ev: the weights are mult
 constexpr unsigned SEEN_BY_ALL = 4;      // every query of the block sees all keys of the tile, and scores are as they are
 constexpr unsigned SEEN_BY_ONE = 8;      // every key of the tile is seen by one query or more
 
+// Stages of KT tiles of 16 keys that a warp has on their way: 12 KB (heads of 256: 24).
+__host__ __device__ constexpr int stages_of(int dmax, int kt) { return 3; }
+
+// Where piece p (16 bytes) of row r lies in its row: what a quarter warp reads at a time of the keys (two rows' 64 bytes) and half
+// a warp of the values (four rows' 32 bytes) then comes from different banks.
+template <int DMAX>
+__device__ __forceinline__ int swizzled(int r, int p) {
+    return DMAX == 64 ? p ^ (r & 2) : p ^ (2 * (r & 3));
+}
+// Which key of a tile's first eight is row g of the first product, for the same reason: 0, 7, 1, 6, 2, 5, 3, 4.
+__device__ __forceinline__ int row_key(int g) { return g & 1 ? 7 - (g >> 1) : g >> 1; }
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void lds128(unsigned (&w)[4], uint32_t at) {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void lds64(unsigned (&w)[2], uint32_t at) {
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+}
+
 // ev and inv of a value's scale.  Of one that is not finite ev = 0, so that its weights are NaN and the others stay numbers.
 __device__ __forceinline__ unsigned power_of(float vs, float& ev, float& inv) {
     const unsigned bits = __float_as_uint(vs);
@@ -176,23 +209,27 @@ __device__ __forceinline__ unsigned power_of(float vs, float& ev, float& inv) {
 // 8; KT: key tiles of 16 that a warp takes at a time; RUN: 16 or 8, pages are a multiple of it, so that a tile or half a tile lies in
 // one page; 0: every row is looked up by itself.
 template <typename T, int CODE, int WARPS, int DMAX, int DK, int NT, int KT, int RUN>
-__global__ void __launch_bounds__(WARPS * 32, NT == 1 && RUN && DMAX < 256 ? DK ? 16 : 12 : 1)
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 && DMAX < 256 ? 4 : 1)
 attention_8bit_kernel(const __grid_constant__ Args a) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1;            // pieces a number is split into
     constexpr int QT = 8 * NT / P;                       // queries of a block
     constexpr int CH = DMAX / 64;                        // runs of 64 dims
     constexpr int Q2 = 2 / P;                            // queries in a lane's two columns of a tile
-    __shared__ float sm_o[WARPS][QT][DMAX + 1];
+    constexpr int STAGES = stages_of(DMAX, KT), STAGE = 2 * KT * 16 * DMAX;
+    // a warp's stages [STAGES][keys | values][KT * 16 rows of DMAX bytes]; at the end the warps' sums in the same place
+    extern __shared__ __align__(128) uint8_t smem[];
+    float (*sm_o)[QT][DMAX + 1] = reinterpret_cast<float (*)[QT][DMAX + 1]>(smem);
     __shared__ float sm_m[WARPS][QT], sm_l[WARPS][QT];
     constexpr int HALVES = RUN == 16 ? 1 : 2;            // runs of a tile
-    __shared__ Run known[RUN ? WARPS : 1][RUN ? 32 * HALVES : 1];
+    constexpr int BATCH = 16 / HALVES;                   // tiles a warp looks up at a time; it keeps two batches
+    __shared__ Run known[RUN ? WARPS : 1][RUN ? 32 : 1];
 
     pdl_launch_dependents();
     pdl_wait();
     const int z = blockIdx.z, kvh = blockIdx.y;
     const int tile = a.num_splits == 1 ? blockIdx.x : blockIdx.x / a.num_splits, split = blockIdx.x - tile * a.num_splits;
     const Portion at = portion_of(a, z);
-    const int group = a.n_heads / a.n_kv_heads;
+    const int group = a.group;
     const int n_queries = min(QT, at.n * group - tile * QT);         // of this block
     if (n_queries <= 0) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -236,30 +273,27 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
     auto nth_of = [&](int group_at, int kt) { return tile0 + group_at * WARPS * KT + kt; };
     auto first_of = [&](int nth) { return (nth < kept_tiles ? nth : nth - kept_tiles + (lo_first >> 4)) << 4; };
 
-    // the next 32 tiles' pages and scales, one tile a lane, for all lanes to read
+    // pages and scales of the next BATCH tiles, a run a lane, for all lanes to read; the batch before stays
     auto look_up = [&](int group_at) {
         __syncwarp();
-        const int nth = nth_of(group_at + lane / KT, lane % KT), key0 = first_of(nth);
-        const unsigned tile_flags = (key0 + 15 <= pos_first && key0 >= lo_last && plain ? SEEN_BY_ALL : 0) |
-                                    (key0 + 15 <= pos_last && key0 >= lo_first ? SEEN_BY_ONE : 0);
-#pragma unroll
-        for (int r = 0; r < HALVES; r++) {
-            Run run = {0, 0.0f, 0.0f, 0.0f, 0.0f, tile_flags, 0};
-            const int j = key0 + 8 * r;
-            if (nth < tile_end && j <= pos_last && (j + RUN - 1 >= lo_first || j < a.keep_first)) {
-                const int b = j / ps;
-                const int page = b < a.max_blocks ? table[b] : -1;
-                if (page >= 0 && page < a.num_pages) {
-                    run.off = page * a.page_stride + (long long)(head_at + (size_t)(j - b * ps) * D);
-                    run.ks = a.k_scale[page * a.scale_stride + kvh];
-                    run.vs = a.v_scale[page * a.scale_stride + kvh];
-                    run.flags |= HAS_PAGE | power_of(run.vs, run.ev, run.inv);
-                } else if (a.status) {
-                    atomicOr(a.status, 16);
-                }
+        const int in = group_at * KT + lane / HALVES, half = lane % HALVES;
+        const int nth = nth_of(in / KT, in % KT), key0 = first_of(nth), j = key0 + 8 * half;
+        Run run = {0, 0.0f, 0.0f, 0.0f, 0.0f, 0, 0};
+        run.flags = (key0 + 15 <= pos_first && key0 >= lo_last && plain ? SEEN_BY_ALL : 0) |
+                    (key0 + 15 <= pos_last && key0 >= lo_first ? SEEN_BY_ONE : 0);
+        if (lane < 16 && nth < tile_end && j <= pos_last && (j + RUN - 1 >= lo_first || j < a.keep_first)) {
+            const int b = a.page_shift >= 0 ? j >> a.page_shift : j / ps;
+            const int page = b < a.max_blocks ? table[b] : -1;
+            if (page >= 0 && page < a.num_pages) {
+                run.off = page * a.page_stride + (long long)(head_at + (size_t)(j - b * ps) * D);
+                run.ks = a.k_scale[page * a.scale_stride + kvh];
+                run.vs = a.v_scale[page * a.scale_stride + kvh];
+                run.flags |= HAS_PAGE | power_of(run.vs, run.ev, run.inv);
+            } else if (a.status) {
+                atomicOr(a.status, 16);
             }
-            known[warp][HALVES * lane + r] = run;
         }
+        if (lane < 16) known[warp][(HALVES * in + half) % 32] = run;
         __syncwarp();
     };
     // RUN 0: the row of key j, if a query sees it and it has a page
@@ -275,74 +309,57 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
         return true;
     };
 
-    uint4 kw[KT][2][CH];                                  // keys g, g + 8: dims 64 c + 16 t ..
-    uint2 vw[KT][4][CH];                                  // keys 2t, 2t + 1, 2t + 8, 2t + 9: dims 64 c + 8 g ..
-    // of keys g and g + 8 (RUN 16: of both) of a group's tiles: scales and what is made of them, flags
-    constexpr int R = RUN == 16 ? 1 : 2;
-    auto load_keys = [&](int group_at, float (&ks)[KT][R], float (&ev)[KT][R], unsigned (&flags)[KT][R], float (&inv)[KT][R], float (&vs)[KT][R]) {
+    // Copies a group's rows, 16 bytes a lane, into its stage; rows that no query sees, and those without a page, become zeros (a
+    // weight of 0 times what such a row may hold would be NaN).  Piece p of row r lies at piece swizzled(r, p).
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * STAGE;
+    constexpr int PIECES = DMAX / 16, STEP = 32 / PIECES;            // of a row; rows that a warp copies at a time
+    const int my_piece = lane % PIECES, my_row = lane / PIECES;
+    const uint32_t my_place = my_row * DMAX + swizzled<DMAX>(my_row, my_piece) * 16;      // of rows my_row + a multiple of 4
+    auto copy = [&](int group_at, int stage) {
 #pragma unroll
-        for (int kt = 0; kt < KT; kt++)
+        for (int kt = 0; kt < KT; kt++) {
+            const uint32_t to = ring + stage * STAGE + kt * 16 * DMAX;
+            if constexpr (RUN == 16) {
+                const Run& run = known[warp][(group_at * KT + kt) % 32];
+                if ((run.flags & (HAS_PAGE | SEEN_BY_ONE)) == (HAS_PAGE | SEEN_BY_ONE)) {      // all of the tile, as it lies
+                    const uint8_t *k = a.k + (run.off + my_row * D + my_piece * 16), *v = a.v + (run.off + my_row * D + my_piece * 16);
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                if constexpr (RUN != 0) {
-                    const Run& run = known[warp][((group_at * KT + kt) & 31) * HALVES + (RUN == 16 ? 0 : r)];
-                    if (RUN != 16 || r == 0) {
-                        ks[kt][r] = run.ks;
-                        ev[kt][r] = run.ev;
-                        inv[kt][r] = run.inv;
-                        vs[kt][r] = run.vs;
-                        flags[kt][r] = run.flags;
+                    for (int i = 0; i < 16 / STEP; i++) {
+                        copy16(to + my_place + i * STEP * DMAX, k + i * STEP * D);
+                        copy16(to + my_place + i * STEP * DMAX + KT * 16 * DMAX, v + i * STEP * D);
                     }
-                    // rows that no query sees are read too: their scores are left out
-                    const uint8_t* p = a.k + run.off + (g + (RUN == 16 ? 8 * r : 0)) * D + 16 * t;
-#pragma unroll
-                    for (int c = 0; c < CH; c++)
-                        kw[kt][r][c] = DK || 64 * c + 16 * t < D ? __ldg(reinterpret_cast<const uint4*>(p + 64 * c)) : make_uint4(0u, 0u, 0u, 0u);
-                } else {
-                    const int nth = nth_of(group_at, kt);
-                    size_t off = 0;
-                    int page = 0;
-                    const bool ok = row_of(nth, first_of(nth) + g + 8 * r, off, page);
-                    ks[kt][r % R] = ok ? a.k_scale[(size_t)page * a.scale_stride + kvh] : 0.0f;
-                    vs[kt][r % R] = ok ? a.v_scale[(size_t)page * a.scale_stride + kvh] : 0.0f;
-                    flags[kt][r % R] = power_of(vs[kt][r % R], ev[kt][r % R], inv[kt][r % R]) | (ok ? HAS_PAGE : 0u);
-#pragma unroll
-                    for (int c = 0; c < CH; c++)
-                        kw[kt][r][c] = ok && 64 * c + 16 * t < D ? __ldg(reinterpret_cast<const uint4*>(a.k + off + 64 * c + 16 * t))
-                                                                : make_uint4(0u, 0u, 0u, 0u);
+                    continue;
                 }
             }
-    };
-    auto load_values = [&](int group_at) {
+            const int nth = nth_of(group_at, kt), key0 = first_of(nth);
 #pragma unroll
-        for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
+            for (int i = 0; i < 16 / STEP; i++) {
+                const int row = i * STEP + my_row;
+                size_t off = 0;
+                bool ok;
                 if constexpr (RUN != 0) {
-                    const Run& run = known[warp][((group_at * KT + kt) & 31) * HALVES + (RUN == 16 ? 0 : r >> 1)];
-                    const uint8_t* p = a.v + run.off + (2 * t + (r & 1) + (RUN == 16 ? 8 * (r >> 1) : 0)) * D + 8 * g;
-#pragma unroll
-                    for (int c = 0; c < CH; c++)
-                        vw[kt][r][c] = DK || 64 * c + 8 * g < D ? __ldg(reinterpret_cast<const uint2*>(p + 64 * c)) : make_uint2(0u, 0u);
+                    const Run& run = known[warp][(HALVES * (group_at * KT + kt) + (RUN == 16 ? 0 : row >> 3)) % 32];
+                    off = run.off + (size_t)(RUN == 16 ? row : row & 7) * D;
+                    ok = (run.flags & HAS_PAGE) && ((run.flags & SEEN_BY_ONE) || seen(key0 + row));
                 } else {
-                    const int nth = nth_of(group_at, kt);
-                    size_t off = 0;
                     int page = 0;
-                    const bool ok = row_of(nth, first_of(nth) + 2 * t + (r & 1) + 8 * (r >> 1), off, page);
-#pragma unroll
-                    for (int c = 0; c < CH; c++)
-                        vw[kt][r][c] = ok && 64 * c + 8 * g < D ? __ldg(reinterpret_cast<const uint2*>(a.v + off + 64 * c + 8 * g)) : make_uint2(0u, 0u);
+                    ok = row_of(nth, key0 + row, off, page);
                 }
+                if (!DK) ok = ok && my_piece * 16 < D;               // dims there are not: zeros too
+                const uint32_t dst = to + row * DMAX + swizzled<DMAX>(row, my_piece) * 16;
+                copy16(dst, a.k + off + my_piece * 16, ok);
+                copy16(dst + KT * 16 * DMAX, a.v + off + my_piece * 16, ok);
             }
+        }
     };
 
-    float ks_next[KT][R], ev_next[KT][R], inv_next[KT][R], vs_next[KT][R];
-    unsigned flags_next[KT][R];
-    if (n_groups > 0) {
-        if constexpr (RUN != 0) look_up(0);
-        load_keys(0, ks_next, ev_next, flags_next, inv_next, vs_next);
-        load_values(0);
+    if (RUN != 0 && n_groups > 0) look_up(0);
+#pragma unroll
+    for (int st = 0; st < STAGES; st++) {
+        if (st < n_groups) copy(st, st);
+        asm volatile("cp.async.commit_group;" ::: "memory");
     }
+
     // ---- q: column g of every tile, as the second operand ------------------------------------------------------
     unsigned qf[NT][CH * 4][2];
     float my_factor[NT];                                 // of column g
@@ -388,21 +405,49 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
             lo[n][e] = first_key(a, max(pos[n][e], 0));
         }
 
+    // rows of the first product and columns of the second: key `my_key` (+ 8) of a tile for lane group g, see row_key()
+    const int my_key = row_key(g);
+    int stage = 0;
     for (int it = 0; it < n_groups; it++) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");      // group `it` has landed (a lane's own copies),
+        __syncwarp();                                                                  // and every lane's
+        const uint32_t k_at = ring + stage * STAGE, v_at = k_at + KT * 16 * DMAX;
+        // of keys my_key and my_key + 8 (RUN 16: of both) of the group's tiles: scales and what is made of them, flags
+        constexpr int R = RUN == 16 ? 1 : 2;
         float ks[KT][R], ev[KT][R], inv[KT][R], vs[KT][R];
         unsigned flags[KT][R];
 #pragma unroll
         for (int kt = 0; kt < KT; kt++)
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                ks[kt][r] = ks_next[kt][r];
-                ev[kt][r] = ev_next[kt][r];
-                inv[kt][r] = inv_next[kt][r];
-                vs[kt][r] = vs_next[kt][r];
-                flags[kt][r] = flags_next[kt][r];
+                if constexpr (RUN != 0) {
+                    const Run& run = known[warp][(HALVES * (it * KT + kt) + r) % 32];
+                    ks[kt][r] = run.ks;
+                    ev[kt][r] = run.ev;
+                    inv[kt][r] = run.inv;
+                    vs[kt][r] = run.vs;
+                    flags[kt][r] = run.flags;
+                } else {
+                    size_t off = 0;
+                    int page = 0;
+                    const bool ok = row_of(nth_of(it, kt), first_of(nth_of(it, kt)) + my_key + 8 * r, off, page);
+                    ks[kt][r] = ok ? a.k_scale[(size_t)page * a.scale_stride + kvh] : 0.0f;
+                    vs[kt][r] = ok ? a.v_scale[(size_t)page * a.scale_stride + kvh] : 0.0f;
+                    flags[kt][r] = power_of(vs[kt][r], ev[kt][r], inv[kt][r]) | (ok ? HAS_PAGE : 0u);
+                }
             }
 
-    // ---- S; the keys' registers are free after it, and the next group's keys are asked for -------------------
+        unsigned every = HAS_PAGE | SEEN_BY_ALL, some = 0;          // flags that all of the group's keys have, that one has
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                every &= flags[kt][r];
+                some |= flags[kt][r];
+            }
+        const bool plainly = RUN && every == (HAS_PAGE | SEEN_BY_ALL);       // no mask, no rule
+
+        // ---- S ----------------------------------------------------------------------------------------------------
         float sc[KT][NT][4];
 #pragma unroll
         for (int kt = 0; kt < KT; kt++) {
@@ -412,8 +457,9 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                 for (int e = 0; e < 4; e++) sc[kt][n][e] = 0.0f;
 #pragma unroll
             for (int c = 0; c < CH; c++) {
-                const unsigned w0[4] = {kw[kt][0][c].x, kw[kt][0][c].y, kw[kt][0][c].z, kw[kt][0][c].w};
-                const unsigned w1[4] = {kw[kt][1][c].x, kw[kt][1][c].y, kw[kt][1][c].z, kw[kt][1][c].w};
+                unsigned w0[4], w1[4];                    // 16 dims of keys my_key, my_key + 8
+                lds128(w0, k_at + (kt * 16 + my_key) * DMAX + swizzled<DMAX>(my_key, 4 * c + t) * 16);
+                lds128(w1, k_at + (kt * 16 + my_key + 8) * DMAX + swizzled<DMAX>(my_key, 4 * c + t) * 16);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     unsigned a0, a1, a2, a3;
@@ -424,11 +470,6 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                 }
             }
         }
-        if (it + 1 < n_groups) {
-            if constexpr (RUN != 0)
-                if ((((it + 1) * KT) & 31) == 0) look_up(it + 1);
-            load_keys(it + 1, ks_next, ev_next, flags_next, inv_next, vs_next);
-        }
 
         // ---- x = score + log2 of the value's scale, -inf where the key is not seen ------------------------------------
         float top[NT][Q2];
@@ -438,7 +479,6 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
             for (int e = 0; e < Q2; e++) top[n][e] = -INFINITY;
 #pragma unroll
         for (int kt = 0; kt < KT; kt++) {
-            const bool all = RUN && (flags[kt][0] & SEEN_BY_ALL) && (flags[kt][0] & flags[kt][R - 1] & HAS_PAGE);
 #pragma unroll
             for (int r = 0; r < 2; r++)
 #pragma unroll
@@ -446,10 +486,10 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
 #pragma unroll
                     for (int e = 0; e < Q2; e++) {
                         float x = P == 2 ? sc[kt][n][2 * r] + sc[kt][n][2 * r + 1] : sc[kt][n][2 * r + e];
-                        if (all) {
+                        if (plainly) {
                             x = fmaf(x, ks[kt][r % R] * factor[n][e], ev[kt][r % R]);
                         } else {
-                            const int j = first_of(nth_of(it, kt)) + g + 8 * r;
+                            const int j = first_of(nth_of(it, kt)) + my_key + 8 * r;
                             const bool visible = (flags[kt][r % R] & HAS_PAGE) && j <= pos[n][e] && (j >= lo[n][e] || j < a.keep_first);
                             x *= ks[kt][r % R] * factor[n][e];
                             if (!plain) {
@@ -510,30 +550,24 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                         const float x = sc[kt][n][P == 2 ? 2 * r : 2 * r + e];
                         w[e] = ex2(x - m_use[n][e]);
                         l[n][e] = fmaf(w[e], inv[kt][r % R], l[n][e]);
-                        if (flags[kt][r % R] & NO_POWER) w[e] = x == -INFINITY ? 0.0f : w[e] * inv[kt][r % R] * vs[kt][r % R];
+                        if (some & NO_POWER) w[e] = x == -INFINITY ? 0.0f : w[e] * inv[kt][r % R] * vs[kt][r % R];
                     }
                     if (P == 2) w[1] = w[0] - __half2float(__float2half_rn(w[0]));
                     pf[n][r] = turn(pack_half(w[0], w[1]));
                 }
-            if constexpr (RUN != 0) {
-                // Values of rows that no query sees become zeros: a weight of 0 times what such a row may hold would be NaN.
-                if (!(flags[kt][0] & SEEN_BY_ONE) || !(flags[kt][0] & flags[kt][R - 1] & HAS_PAGE)) {
-                    const int key0 = first_of(nth_of(it, kt));
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (!(flags[kt][(r >> 1) % R] & HAS_PAGE) || !seen(key0 + 2 * t + (r & 1) + 8 * (r >> 1))) {
+            for (int c = 0; c < CH; c++) {
+                unsigned vw[4][2];                        // dims 64 c + 8 g .. of the keys of the second product's columns 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-                            for (int c = 0; c < CH; c++) vw[kt][r][c] = make_uint2(0u, 0u);
-                        }
+                for (int r = 0; r < 4; r++) {
+                    const int low = r & 1 ? 7 - t : t, row = low + 8 * (r >> 1);
+                    lds64(vw[r], v_at + (kt * 16 + row) * DMAX + swizzled<DMAX>(low, 4 * c + (g >> 1)) * 16 + (g & 1) * 8);
                 }
-            }
-#pragma unroll
-            for (int c = 0; c < CH; c++)
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     unsigned w[4];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) w[r] = half ? vw[kt][r][c].y : vw[kt][r][c].x;
+                    for (int r = 0; r < 4; r++) w[r] = vw[r][half];
                     // bytes of two keys side by side: dims d, d + 1 and d + 2, d + 3 of the piece's four
                     const unsigned e0 = __byte_perm(w[0], w[1], 0x5140), e1 = __byte_perm(w[0], w[1], 0x7362);
                     const unsigned f0 = __byte_perm(w[2], w[3], 0x5140), f1 = __byte_perm(w[2], w[3], 0x7362);
@@ -547,9 +581,19 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
 #pragma unroll
                     for (int n = 0; n < NT; n++) mma_f16(o[c * 4 + half * 2 + 1][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
                 }
+            }
         }
-        if (it + 1 < n_groups) load_values(it + 1);
+        __syncwarp();                                     // the stage may be written again
+        if (it + STAGES < n_groups) {
+            if constexpr (RUN != 0)
+                if ((it + STAGES) * KT % BATCH == 0) look_up(it + STAGES);
+            copy(it + STAGES, stage);
+        }
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
+        asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    __syncthreads();                                      // no stage is in use any more
+    if (a.in_cluster) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
     // ---- the warps' states in shared memory, joined in their order ------------------------------------------------
 #pragma unroll
@@ -571,6 +615,13 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
             }
         }
     __syncthreads();
+    // splits as a cluster: their results meet in the shared memory of its first block, behind that block's own warps' sums
+    const size_t behind = sizeof(float) * WARPS * QT * (DMAX + 1);
+    float* met = reinterpret_cast<float*>(smem + behind);             // [split][query][D + 2]
+    if (a.in_cluster) {
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // the first block has left its stages
+        met = cg::this_cluster().map_shared_rank(met, 0);
+    }
     for (int idx = tid; idx < n_queries * D; idx += WARPS * 32) {
         const int i = idx / D, d = idx - i * D, qi = tile * QT + i;
         float m = -INFINITY, L = 0.0f, O = 0.0f;
@@ -587,12 +638,29 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
         if (a.num_splits == 1) {
             finish<T>(a, O, L, m, row, h, d);
         } else {
-            float* part = a.scratch + (((size_t)row * a.n_heads + h) * a.num_splits + split) * (D + 2);
+            float* part = a.in_cluster ? met + (split * QT + i) * (D + 2)
+                                       : a.scratch + (((size_t)row * a.n_heads + h) * a.num_splits + split) * (D + 2);
             part[d] = O;
             if (d == 0) {
                 part[D] = m;
                 part[D + 1] = L;
             }
+        }
+    }
+    if (a.in_cluster) {
+        cg::this_cluster().sync();
+        if (split != 0) return;
+        for (int idx = tid; idx < n_queries * D; idx += WARPS * 32) {
+            const int i = idx / D, d = idx - i * D, qi = tile * QT + i;
+            float m = -INFINITY, L = 0.0f, O = 0.0f;
+            for (int k = 0; k < a.num_splits; k++) m = fmaxf(m, met[(k * QT + i) * (D + 2) + D]);
+            for (int k = 0; k < a.num_splits; k++) {
+                const float* part = met + (k * QT + i) * (D + 2);
+                const float f = part[D] == -INFINITY ? 1.0f : ex2(part[D] - m);
+                L = fmaf(part[D + 1], f, L);
+                O = fmaf(part[d], f, O);
+            }
+            finish<T>(a, O, L, m, at.row0 + token_of(qi), head_of(qi), d);
         }
     }
 }
@@ -640,59 +708,113 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args 
     }
 }
 
+constexpr int MAX_CLUSTER = 8;           // splits up to here join in a cluster, if the blocks are of single tokens' size
+
+// A kernel of four warps with more shared memory than a launch has by itself; the kernel is told so once on each device.
+template <auto KERNEL>
+int start(const Args& a, dim3 grid, int smem, int most_smem, cudaStream_t stream) {
+    static std::atomic<unsigned long long> told{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return (int)e;
+    const unsigned long long bit = 1ull << (device & 63);
+    if (!(told.load() & bit) || device > 63) {
+        e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);
+        if (e != cudaSuccess) return (int)e;
+        told.fetch_or(bit);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int na = 0;
+    if (a.in_cluster) {
+        attr[na].id = cudaLaunchAttributeClusterDimension;
+        attr[na].val.clusterDim.x = a.num_splits;
+        attr[na].val.clusterDim.y = 1;
+        attr[na].val.clusterDim.z = 1;
+        na++;
+    }
+    if (sandy_pdl_enabled()) {
+        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[na].val.programmaticStreamSerializationAllowed = 1;
+        na++;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = na;
+    e = cudaLaunchKernelEx(&cfg, KERNEL, a);
+    return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+// Whether the queries of a (request, key/value head) are more columns than one tile has.
+inline bool is_wide(long long queries, int head_dim, int dtype) { return queries * (dtype == SANDY_F32 ? 2 : 1) > 8 && head_dim <= 128; }
+
 template <typename T, int CODE>
 int launch(const Args& a, int n_z, int max_queries, int max_n, cudaStream_t stream) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1;
-    const bool wide = max_queries * P > 8;               // more columns than one tile has
+    const bool wide = is_wide(max_queries, a.head_dim, sizeof(T) == 4 ? SANDY_F32 : SANDY_BF16);
     int e;
-#define LAUNCH(WARPS, DMAX, DK, NT, KT, RUN)                                                                                            \
-    e = sandy_launch(attention_8bit_kernel<T, CODE, WARPS, DMAX, DK, NT, KT, RUN>,                                                      \
-                     dim3((unsigned)((max_queries + 8 * NT / P - 1) / (8 * NT / P) * a.num_splits), a.n_kv_heads, n_z), dim3(WARPS * 32), 0, \
-                     stream, a)
+#define LAUNCH(DMAX, DK, NT, KT, RUN)                                                                                            \
+    do {                                                                                                                         \
+        constexpr int QT = 8 * NT / P, ring = 4 * stages_of(DMAX, KT) * 2 * KT * 16 * DMAX, sums = 4 * QT * (DMAX + 1) * 4;       \
+        constexpr int alone = std::max(ring, sums), together = std::max(ring, sums + MAX_CLUSTER * QT * (DMAX + 2) * 4);          \
+        e = start<attention_8bit_kernel<T, CODE, 4, DMAX, DK, NT, KT, RUN>>(                                                     \
+            a, dim3((unsigned)((max_queries + QT - 1) / QT * a.num_splits), a.n_kv_heads, n_z), a.in_cluster ? together : alone,  \
+            NT == 1 ? together : alone, stream);                                                                                 \
+    } while (0)
     if (a.page_size % 8 != 0) {                          // rows one by one
-        if (a.head_dim <= 64) LAUNCH(1, 64, 0, 1, 1, 0);
-        else if (a.head_dim <= 128) LAUNCH(1, 128, 0, 1, 1, 0);
-        else LAUNCH(1, 256, 0, 1, 1, 0);
+        if (a.head_dim <= 64) LAUNCH(64, 0, 1, 1, 0);
+        else if (a.head_dim <= 128) LAUNCH(128, 0, 1, 1, 0);
+        else LAUNCH(256, 0, 1, 1, 0);
     } else if (a.page_size % 16 == 0 && a.head_dim == 64) {
-        if (wide) LAUNCH(4, 64, 64, 4, 1, 16);
-        else LAUNCH(1, 64, 64, 1, 2, 16);
+        if (wide) LAUNCH(64, 64, 4, 1, 16);
+        else LAUNCH(64, 64, 1, 2, 16);
     } else if (a.page_size % 16 == 0 && a.head_dim == 128) {
-        if (wide) LAUNCH(4, 128, 128, 2, 1, 16);
-        else LAUNCH(1, 128, 128, 1, 1, 16);
+        if (wide) LAUNCH(128, 128, 2, 1, 16);
+        else LAUNCH(128, 128, 1, 1, 16);
     } else if (a.head_dim <= 64) {
-        if (wide) LAUNCH(4, 64, 0, 4, 1, 8);
-        else LAUNCH(1, 64, 0, 1, 2, 8);
+        if (wide) LAUNCH(64, 0, 4, 1, 8);
+        else LAUNCH(64, 0, 1, 2, 8);
     } else if (a.head_dim <= 128) {
-        if (wide) LAUNCH(4, 128, 0, 2, 1, 8);
-        else LAUNCH(1, 128, 0, 1, 1, 8);
+        if (wide) LAUNCH(128, 0, 2, 1, 8);
+        else LAUNCH(128, 0, 1, 1, 8);
     } else {
-        LAUNCH(1, 256, 0, 1, 1, 8);
+        LAUNCH(256, 0, 1, 1, 8);
     }
 #undef LAUNCH
-    if (e != SANDY_OK || a.num_splits == 1) return e;
+    if (e != SANDY_OK || a.num_splits == 1 || a.in_cluster) return e;
     return sandy_launch(join_kernel<T>, dim3((unsigned)((long long)max_n * a.n_heads), n_z), dim3(128), 0, stream, a);
 }
 
 }  // namespace
 
-// How many blocks share a request's keys (max_keys: the most that one of its queries may see).  Single tokens' blocks are one warp,
-// of which an SM holds sixteen: as many as fill the SMs once, none with fewer than 128 keys.  A portion's blocks are four warps.
-SANDY_API int sandy_attention_8bit_splits(int n_z, int max_n, int n_heads, int n_kv_heads, int head_dim, int max_keys, int dtype) {
-    if (n_z < 1 || max_n < 1 || n_kv_heads < 1 || n_heads < n_kv_heads || max_keys < 1) return 1;
-    const long long queries = (long long)max_n * (n_heads / n_kv_heads), columns = queries * (dtype == SANDY_F32 ? 2 : 1);
-    const bool narrow = columns <= 8 || head_dim > 128;
-    const long long tile = narrow ? 8 : head_dim <= 64 ? 32 : 16;
-    const long long blocks = (columns + tile - 1) / tile * n_kv_heads * n_z, room = (long long)sandy_sm_count() * (narrow ? 16 : 2);
-    const long long wanted = room / blocks, most = (max_keys + 127) / 128;
-    long long splits = wanted < most ? wanted : most;
-    return (int)(splits < 1 ? 1 : splits > MAX_SPLITS ? MAX_SPLITS : splits);
+// How many blocks share a request's keys (max_keys: the most that one of its queries may see): as many as fill the SMs once (four
+// blocks of single tokens an SM, two of a portion's), none with fewer than 128 keys, and no cluster of 6 or 7 (they fit an SM group
+// badly); *scratch_floats: what their partial results take.
+SANDY_API int sandy_attention_8bit_splits(int n_rows, int n_z, int max_n, int n_heads, int n_kv_heads, int head_dim, int max_keys,
+                                          int dtype, int asked, long long* scratch_floats) {
+    if (n_z < 1 || max_n < 1 || n_kv_heads < 1 || n_heads < n_kv_heads || max_keys < 1 || asked < 0) return 1;
+    const long long queries = (long long)max_n * (n_heads / n_kv_heads);
+    const bool wide = is_wide(queries, head_dim, dtype);
+    long long splits = asked;
+    if (!asked) {
+        const long long columns = queries * (dtype == SANDY_F32 ? 2 : 1), tile = !wide ? 8 : head_dim <= 64 ? 32 : 16;
+        const long long blocks = (columns + tile - 1) / tile * n_kv_heads * n_z, room = (long long)sandy_sm_count() * (wide ? 2 : 4);
+        splits = std::min(room / blocks, (long long)(max_keys + 127) / 128);
+        if (!wide && (splits == 6 || splits == 7)) splits = 5;
+        splits = std::max(1ll, std::min(splits, (long long)MAX_SPLITS));
+    }
+    if (scratch_floats) *scratch_floats = splits > (wide ? 1 : MAX_CLUSTER) ? (long long)n_rows * n_heads * splits * (head_dim + 2) : 0;
+    return (int)splits;
 }
 
 // Attention of prompt portions (q_start [n_z + 1], positions = kv_before [n_z], token_seq null, request z = row z of the block
 // table; max_n: the most tokens of one) or of single tokens (q_start null: token z of request token_seq[z] at positions[z]; max_n 1).
 // q: [n_rows, H * D], out likewise, row pitches ld_q and ld_out (elements); k, v, scales and table as sandy_kv_append_8bit has them,
 // n_seqs rows in the table.  max_keys: the most keys that
-// one of a request's blocks of queries sees, by which the splits are cut; num_splits > 1 needs `scratch`: n_rows * H * num_splits * (D + 2) floats.  A row without a visible key
+// one of a request's blocks of queries sees, by which the splits are cut; `scratch` as sandy_attention_8bit_splits says.  A row without a visible key
 // becomes zeros.  Bit 4 of *status: a visible key without a page, a token of no request, or rows past n_rows.
 SANDY_API int sandy_attention_8bit(const void* q, long long ld_q, const void* k, const void* v, const float* k_scale,
                                    const float* v_scale, long long page_stride, long long scale_stride, const int* block_table,
@@ -703,7 +825,7 @@ SANDY_API int sandy_attention_8bit(const void* q, long long ld_q, const void* k,
                                    int dtype, int code, int* status, cudaStream_t stream) {
     if (n_z == 0 || max_n == 0) return SANDY_OK;
     if (!rules || !q || !k || !v || !k_scale || !v_scale || !block_table || !positions || !out || !(token_seq || q_start) || n_z < 0 ||
-        max_n < 0 || n_seqs < 1 || max_blocks < 1 || page_size < 1 || max_keys < 1 || num_splits < 1 || (num_splits > 1 && !scratch))
+        max_n < 0 || n_seqs < 1 || max_blocks < 1 || page_size < 1 || max_keys < 1 || num_splits < 1)
         return SANDY_ERR_ARGUMENT;
     if (rules->dist_bias && rules->n_dist < 1) return SANDY_ERR_ARGUMENT;
     if (rules->window < 0 || rules->keep_first < 0 || rules->chunk < 0 || !(rules->softcap >= 0.0f) ||
@@ -714,12 +836,15 @@ SANDY_API int sandy_attention_8bit(const void* q, long long ld_q, const void* k,
     const long long queries = (long long)max_n * (n_heads / n_kv_heads);
     if (queries > (1 << 28) || queries * num_splits > 0x7fffffffll || (long long)max_n * n_heads > 0x7fffffffll || num_splits > MAX_SPLITS)
         return SANDY_ERR_UNSUPPORTED;
+    const bool in_cluster = num_splits > 1 && num_splits <= MAX_CLUSTER && !is_wide(queries, head_dim, dtype);
+    if (num_splits > 1 && !in_cluster && !scratch) return SANDY_ERR_ARGUMENT;
     // a split's tiles of 16 keys, an even number; two more for the ends of a window and of the kept keys
     const int split_tiles = (((max_keys - 1) / 16 + 3 + num_splits - 1) / num_splits + 1) / 2 * 2;
     const Args a = {q, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, block_table, token_seq, positions, q_start, out, scratch,
                     status, rules->sink, rules->out_gate, rules->dist_bias, rules->elem_gate, ld_q, ld_out, page_stride, scale_stride,
-                    max_blocks, n_rows, n_seqs, n_heads, n_kv_heads, head_dim, page_size, num_pages, num_splits, split_tiles, rules->window,
-                    rules->keep_first, rules->chunk, rules->n_dist, rules->ld_elem_gate, rules->gate_dim, scale, rules->softcap,
+                    max_blocks, n_rows, n_seqs, n_heads, n_kv_heads, head_dim, page_size, num_pages, num_splits, split_tiles, n_heads / n_kv_heads,
+                    (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1, rules->window,
+                    rules->keep_first, rules->chunk, rules->n_dist, rules->ld_elem_gate, rules->gate_dim, scale, rules->softcap, in_cluster,
                     (((uintptr_t)q | (uintptr_t)(ld_q * (dtype == SANDY_F32 ? 4 : 2))) & 15) == 0};
     if (dtype == SANDY_F32 && code == SANDY_E4M3) return launch<float, SANDY_E4M3>(a, n_z, (int)queries, max_n, stream);
     if (dtype == SANDY_F32 && code == SANDY_INT8) return launch<float, SANDY_INT8>(a, n_z, (int)queries, max_n, stream);

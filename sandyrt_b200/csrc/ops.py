@@ -687,9 +687,11 @@ def _attention_8bit(what, q, cache, block_table, token_seq, positions, q_start, 
     if block_table.shape[0] == 0 or block_table.shape[1] == 0 or pages == 0:
         raise KernelError(f"{what}: an empty block table or cache")
     max_keys = min(block_table.shape[1] * ps, window + keep_first + max_n if window else 1 << 30)
-    splits = num_splits or _entry("attention_8bit", "sandy_attention_8bit_splits", (_I,) * 7)(n_z, max_n, n_heads, hkv, d, max_keys, dtype)
-    # partial results of the splits: memory of the stream the call is on, given back to the allocator when it returns
-    scratch = torch.empty(T * n_heads * splits * (d + 2), dtype=torch.float32, device=device) if splits > 1 else None
+    # partial results of many splits: memory of the stream the call is on, given back to the allocator when it returns
+    floats = ctypes.c_longlong(0)
+    splits = _entry("attention_8bit", "sandy_attention_8bit_splits", (_I,) * 9 + (_V,))(T, n_z, max_n, n_heads, hkv, d, max_keys, dtype, num_splits,
+                                                                                        ctypes.addressof(floats))
+    scratch = torch.empty(floats.value, dtype=torch.float32, device=device) if floats.value else None
     args = _AttentionRules(window, keep_first, softcap, chunk, _at(sink), _at(out_gate), _at(dist_bias),
                            0 if dist_bias is None else dist_bias.shape[1], _at(elem_gate), 0 if elem_gate is None else elem_gate.stride(0),
                            0 if elem_gate is None else elem_gate.shape[1] // n_heads)
@@ -698,7 +700,7 @@ def _attention_8bit(what, q, cache, block_table, token_seq, positions, q_start, 
              scale_stride, block_table.data_ptr(), block_table.shape[1], block_table.shape[0], _at(token_seq), positions.data_ptr(), _at(q_start),
              out.data_ptr(), out.stride(0), T, n_z, max_n, n_heads, hkv, d, ps, pages, scale, ctypes.addressof(args), max_keys, splits, _at(scratch),
              dtype, code, _status_word(device)), f"{what}(H={n_heads},Hkv={hkv},D={d},page={ps},splits={splits})")
-    if splits > 1:
+    if scratch is not None:
         global LAUNCHES
         LAUNCHES += 1
 

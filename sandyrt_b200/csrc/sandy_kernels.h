@@ -477,7 +477,8 @@ int sandy_kv_read_8bit(const void* k, const void* v, const float* k_scale, const
                        int head_dim, int page_size, int num_pages, int dtype, int code, int* status, cudaStream_t stream);
 
 /* attention_8bit.cu */
-int sandy_attention_8bit_splits(int n_z, int max_n, int n_heads, int n_kv_heads, int head_dim, int max_keys, int dtype);
+int sandy_attention_8bit_splits(int n_rows, int n_z, int max_n, int n_heads, int n_kv_heads, int head_dim, int max_keys, int dtype, int asked,
+                                long long* scratch_floats);
 int sandy_attention_8bit(const void* q, long long ld_q, const void* k, const void* v, const float* k_scale, const float* v_scale,
                          long long page_stride, long long scale_stride, const int* block_table, int max_blocks, int n_seqs,
                          const int* token_seq, const int* positions, const int* q_start, void* out, long long ld_out, int n_rows, int n_z,
