@@ -1,0 +1,556 @@
+// Causal attention of prompt portions over the paged cache in 8 bits (kv_8bit.cuh) on the tcgen05 tensor cores: bfloat16 queries,
+// heads of 64 and 128, pages of a multiple of 16 keys.
+//
+// Formula and scales as in attention_8bit.cu; the products are half-precision ones here too: codes are half-precision numbers without
+// rounding, a query row is scaled by a power of two so that its largest element lies in [1, 2), and the scales of keys and values, which
+// are the same for 16 keys of a tile at least, never touch an operand:
+//   x_j = S_j * (sk * 2^eq * scale * log2 e) + log2 sv        p_j sv = 2^(x_j - M)       l += (sum over the run of 2^(x_j - M)) / sv
+// With the maximum of a run taken over S, a score costs what it costs without scales: a maximum, an fma, an exponential, an addition.
+//
+// A block owns 256 query rows -- the heads of a group for consecutive tokens, row = token * group + head -- of one request's key/value
+// head, as two tiles of 128 (tensor-memory lanes), and walks the keys in tiles of 128 which both share:
+//   warps 0-3, 4-7   softmax of the two tiles, a thread a row: it reads its 128 scores with tcgen05.ld, and writes its weights as
+//                    half-precision pairs over the first half of them with tcgen05.st;
+//   warps 8-11       bring the codes (16 bytes a thread at a time, the next tile's while this one's are being written), turn
+//                    them into half-precision numbers, and write them into shared memory as the operands lie there: K rows of 128
+//                    bytes in the 128-byte swizzle, V likewise (an MN-major operand); rows past the portion's last key are zeros;
+//   warp 12          issues the products: S of one tile while the other's softmax runs.  P lies where S lay, so that S of the next
+//                    key tile follows P V of this one; both tiles' S and O fill the 512 columns of tensor memory at heads of 128.
+// The accumulators stay in tensor memory over all tiles and are rescaled there only when a row's maximum has run ahead of its reference
+// by more than 2^8 (P stays below 256).  When S of a tile is there, the products before it are complete: O is at rest then.
+//
+// What bounds it: 32,768 exponentials a pair of tiles are 2,048 cycles of the special-function units, the products at heads of 128
+// as much of the tensor cores; converting 32,768 codes is some 700 (int8) issue slots of each SM quarter.  256 rows a block halve the
+// conversion's share and the reads of the cache.  One block an SM (213 KB of shared memory at heads of 128).
+//
+// Every wait on an mbarrier is bounded; one that runs out raises bit 8 of the status word and the block ends without waiting again.
+#include <atomic>
+
+#include "attention_rules.h"
+#include "kv_8bit.cuh"
+#include "tcgen05.cuh"
+
+namespace {
+
+constexpr int BN = 128;                  // keys of a tile
+constexpr int THREADS = 416;
+constexpr int FIRST_PRODUCER = 256, ISSUE_WARP = 12;
+constexpr int STAGES = 2;
+constexpr int CONSTS = 8;                // key tiles whose scales and pages are kept
+constexpr float RESCALE = 8.0f;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr uint32_t HALF_TILE = 128 * 128;            // 128 rows of 64 half-precision numbers
+
+constexpr uint32_t idesc_f16(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24); }
+
+struct Args {
+    const bf16* q;
+    const uint8_t *k, *v;
+    const float *k_scale, *v_scale;
+    const int *block_table, *q_start, *kv_before;
+    bf16* out;
+    int* status;
+    const float *sink, *out_gate;
+    const bf16* elem_gate;
+    long long ld_q, ld_out, page_stride, scale_stride;
+    int max_blocks, n_rows, n_heads, n_kv_heads, group, page_size, page_shift, num_pages;
+    int window, keep_first, chunk, ld_elem_gate, gate_dim;
+    float scale, softcap;
+};
+
+// What a run of 16 keys gives to its scores: the key's scale, log2 of the value's, one over it.
+struct __align__(16) RunConsts {
+    float ks, ev, inv, unused;
+};
+
+__device__ __forceinline__ void umma_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "}" ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+template <int CODE, int HD>
+__global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_constant__ Args a) {
+    constexpr int SUBS = HD / 64;                        // runs of 64 dims: 128-byte rows
+    constexpr uint32_t Q_BYTES = SUBS * HALF_TILE, KV_BYTES = SUBS * HALF_TILE;
+    constexpr uint32_t OFF_K = 2 * Q_BYTES, OFF_V = OFF_K + STAGES * KV_BYTES;
+    auto s_col = [](int g) { return (uint32_t)(128 * g); };           // columns of tensor memory: scores, later weights; results
+    auto o_col = [](int g) { return (uint32_t)(256 + HD * g); };
+    constexpr uint32_t IDESC_S = idesc_f16(BN), IDESC_PV = idesc_f16(HD) | (1u << 16);        // V: MN-major
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ RunConsts s_consts[CONSTS][BN / 16];
+    __shared__ long long s_off[CONSTS][BN / 16];         // where a run's rows lie in keys and values, -1: nowhere
+    __shared__ uint64_t q_ready[2], k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_ready[2], o_full[2], c_full[CONSTS];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int s_failed;
+
+    pdl_launch_dependents();
+    pdl_wait();
+    const int z = blockIdx.z, kvh = blockIdx.y;
+    const int row0 = a.q_start[z], n = a.q_start[z + 1] - row0, before = a.kv_before[z];
+    const bool there = row0 >= 0 && n <= a.n_rows - row0;            // the portion's rows
+    if (!there && n > 0 && threadIdx.x == 0 && a.status) atomicOr(a.status, 16);
+    const int tiles = there && n > 0 ? (int)(((long long)n * a.group + 255) / 256) : 0;
+    if ((int)blockIdx.x >= tiles) return;
+    const int first = (tiles - 1 - blockIdx.x) * 256;                // the rows with the most keys start first
+    const int n_valid = min(256, n * a.group - first);
+    const int groups = n_valid > 128 ? 2 : 1;
+    const int pos_first = before + first / a.group, pos_last = before + (first + n_valid - 1) / a.group;
+    auto first_key = [&](int pos) {
+        int lo = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+        if (a.chunk > 0) lo = max(lo, pos - pos % a.chunk);
+        return lo;
+    };
+    const int lo_first = first_key(max(pos_first, 0)), lo_last = first_key(max(pos_last, 0));
+    const int kt_window = lo_first / BN;
+    const int kept_tiles = lo_first > 0 ? min((a.keep_first + BN - 1) / BN, kt_window) : 0;
+    const int n_it = pos_last >= 0 ? kept_tiles + pos_last / BN - kt_window + 1 : 0;
+    auto first_of = [&](int t) { return (t < kept_tiles ? t : t - kept_tiles + kt_window) * BN; };
+    const int tid = threadIdx.x, warp = tid >> 5;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+
+    if (tid == 0) {
+        for (int g = 0; g < 2; g++) {
+            mbar_init(&q_ready[g], 128);
+            mbar_init(&s_full[g], 1);
+            mbar_init(&p_ready[g], 128);
+            mbar_init(&o_full[g], 1);
+        }
+        for (int i = 0; i < STAGES; i++) {
+            mbar_init(&k_full[i], 128);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 128);
+            mbar_init(&v_empty[i], 1);
+        }
+        for (int i = 0; i < CONSTS; i++) mbar_init(&c_full[i], BN / 16);
+        s_failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == ISSUE_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    auto wait_for = [&](uint64_t* bar, uint32_t parity) {
+        if (s_failed) return;
+        if (!mbar_wait(bar, parity)) {
+            if (a.status) atomicOr(a.status, 256);
+            s_failed = 1;
+        }
+    };
+
+    if (warp < 8) {
+        // ---- softmax ------------------------------------------------------------------------------------------------
+        const int g = warp >> 2, r = tid & 127;          // which tile; which row of it, the tensor-memory lane
+        const int at = first + g * 128 + r;              // of the (request, key/value head)'s rows
+        const bool mine = g * 128 + r < n_valid;
+        const int token = mine ? at / a.group : 0, h = kvh * a.group + (mine ? at - token * a.group : 0);
+        const int pos = mine ? before + token : -1;
+        const int lo = first_key(max(pos, 0));
+        float factor = 0.0f;
+        if (g < groups) {
+            // the row of q, scaled, as the first operand: 16-byte piece c of its 128-byte rows at piece c ^ (r & 7)
+            const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(row0 + token) * a.ld_q + (size_t)h * HD);
+            uint32_t amax = 0;
+#pragma unroll 4
+            for (int c = 0; c < HD / 8; c++) {
+                const uint4 w = mine ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+                amax = max(amax, max(m & 0xffffu, m >> 16));
+            }
+            const int e2 = max(-100, min(120, (int)(amax >> 7) - 127));
+            const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+            factor = __uint_as_float((uint32_t)(127 + e2) << 23) * a.scale * (a.softcap > 0.0f ? 1.0f : LOG2E);
+            const uint32_t to = base + g * Q_BYTES + r * 128;
+#pragma unroll 4
+            for (int c = 0; c < HD / 8; c++) {
+                const uint4 w = mine ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+                auto two = [&](uint32_t x) { return pack_half(__uint_as_float(x << 16) * down, __uint_as_float(x & 0xffff0000u) * down); };
+                sts128(to + (c >> 3) * HALF_TILE + (((c & 7) ^ (r & 7)) << 4), two(w.x), two(w.y), two(w.z), two(w.w));
+            }
+            fence_async_proxy();
+            mbar_arrive(&q_ready[g]);
+        }
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        float M = -INFINITY, l = 0.0f;
+        for (int it = 0; it < n_it && g < groups; it++) {
+            const int j0 = first_of(it);
+            wait_for(&c_full[it % CONSTS], (it / CONSTS) & 1);       // long there
+            wait_for(&s_full[g], it & 1);
+            tc_fence_after();
+            uint32_t s[64];                              // half of the tile's scores at a time; later its weights, as pairs
+            const RunConsts* consts = s_consts[it % CONSTS];
+            auto read = [&](int half) {
+                tmem_ld_32x32(lanes + s_col(g) + 64 * half, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+                tmem_ld_32x32(lanes + s_col(g) + 64 * half + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+                tmem_wait_ld();
+            };
+            // A tile that every row of the block sees whole needs no mask.  In any other the scores become x where they lie.
+            const bool whole = j0 + BN - 1 <= pos_first && j0 >= lo_last && a.softcap == 0.0f;
+            if (!whole) {
+                const bool ranged = a.window > 0 || a.chunk > 0;
+#pragma unroll 1
+                for (int half = 0; half < 2; half++) {
+                    const int j = j0 + 64 * half;
+                    const int last = pos - j, from = lo - j, kept = a.keep_first - j;      // this row sees e <= last, e >= from or e < kept
+                    read(half);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const float f = consts[4 * half + u].ks * factor, ev = consts[4 * half + u].ev;
+                        if (a.softcap > 0.0f) {
+#pragma unroll
+                            for (int e = 16 * u; e < 16 * u + 16; e++)
+                                s[e] = __float_as_uint(
+                                    fmaf(a.softcap * LOG2E, tanh_fast(__fdividef(__uint_as_float(s[e]) * f, a.softcap)), ev));
+                        } else {
+#pragma unroll
+                            for (int e = 16 * u; e < 16 * u + 16; e++) s[e] = __float_as_uint(fmaf(__uint_as_float(s[e]), f, ev));
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 64; e++)
+                        if (e > last) s[e] = 0xff800000u;
+                    if (ranged) {
+#pragma unroll
+                        for (int e = 0; e < 64; e++)
+                            if (e < from && e >= kept) s[e] = 0xff800000u;
+                    }
+                    tmem_st_32x32(lanes + s_col(g) + 64 * half, s);
+                    tmem_st_32x32(lanes + s_col(g) + 64 * half + 32, s + 32);
+                }
+                tmem_wait_st();
+            }
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int half = 0; half < 2; half++) {
+                read(half);
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    float m0 = __uint_as_float(s[16 * u]), m1 = __uint_as_float(s[16 * u + 1]);
+#pragma unroll
+                    for (int e = 2; e < 16; e += 2) {
+                        m0 = fmaxf(m0, __uint_as_float(s[16 * u + e]));
+                        m1 = fmaxf(m1, __uint_as_float(s[16 * u + e + 1]));
+                    }
+                    m0 = fmaxf(m0, m1);
+                    top = fmaxf(top, whole ? fmaf(m0, consts[4 * half + u].ks * factor, consts[4 * half + u].ev) : m0);
+                }
+            }
+            const bool move = top > M + RESCALE;
+            if (__any_sync(0xffffffffu, move)) {
+                const float alpha = move ? ex2(M - top) : 1.0f;      // 0 on the row's first keys
+                if (it > 0) {
+#pragma unroll 1
+                    for (int c = 0; c < HD / 16; c++) {
+                        uint32_t o[16];
+                        tmem_ld_32x16(lanes + o_col(g) + 16 * c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        asm volatile(
+                            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+                            "%15, %16};" ::"r"(lanes + o_col(g) + 16 * c),
+                            "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]), "r"(o[8]), "r"(o[9]),
+                            "r"(o[10]), "r"(o[11]), "r"(o[12]), "r"(o[13]), "r"(o[14]), "r"(o[15])
+                            : "memory");
+                    }
+                    tmem_wait_st();
+                }
+                l *= alpha;
+                if (move) M = top;
+            }
+            const float m_use = M == -INFINITY ? 0.0f : M;           // no key yet: weights are 2^-inf
+#pragma unroll 1
+            for (int half = 0; half < 2; half++) {
+                read(half);
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const RunConsts c = consts[4 * half + u];
+                    const float f = whole ? c.ks * factor : 1.0f, off = (whole ? c.ev : 0.0f) - m_use;
+                    float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float p0 = ex2(fmaf(__uint_as_float(s[16 * u + e]), f, off)), p1 = ex2(fmaf(__uint_as_float(s[16 * u + e + 1]), f, off));
+                        sum0 += p0;
+                        sum1 += p1;
+                        s[8 * u + e / 2] = pack_half(p0, p1);
+                    }
+                    l = fmaf(sum0 + sum1, c.inv, l);
+                }
+                // over columns whose scores have been read: 0..31 of the tile's 128, then 32..63
+                tmem_st_32x32(lanes + s_col(g) + 32 * half, s);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&p_ready[g]);
+        }
+        if (g < groups) {
+            if (n_it > 0) {
+                wait_for(&o_full[g], 0);
+                tc_fence_after();
+            }
+            if (a.sink && M > -INFINITY) l += ex2(fmaf(a.sink[h], LOG2E, -M));
+            float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;        // no visible key: zeros
+            if (a.out_gate && mine) inv *= a.out_gate[(size_t)(row0 + token) * a.n_heads + h];
+            bf16* dst = a.out + (size_t)(row0 + token) * a.ld_out + (size_t)h * HD;
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; c++) {
+                uint32_t o[32];
+                if (n_it > 0) {
+                    tmem_ld_32x32(lanes + o_col(g) + 32 * c, o);
+                    tmem_wait_ld();
+                }
+                if (mine) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        float y[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            y[i] = M == -INFINITY && l == 0.0f ? 0.0f : __uint_as_float(o[e + i]) * inv;
+                            if (a.elem_gate)
+                                y[i] *= elem_gate_of(a.elem_gate, a.ld_elem_gate, a.gate_dim, row0 + token, h, 32 * c + e + i);
+                        }
+                        *reinterpret_cast<uint4*>(dst + 32 * c + e) =
+                            make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+                    }
+                }
+            }
+        }
+    } else if (warp < ISSUE_WARP) {
+        // ---- codes into operands ----------------------------------------------------------------------------------------
+        constexpr int PIECES = HD / 16, STEP = 128 / PIECES, EACH = 128 / STEP;      // 16-byte pieces of a row; rows at a time; a thread's
+        const int p = tid - FIRST_PRODUCER, piece = p % PIECES, my_row = p / PIECES;
+        const int* table = a.block_table + (size_t)z * a.max_blocks;
+        auto seen = [&](int j) { return j <= pos_last && (j >= lo_first || j < a.keep_first); };
+        // Threads 0..7: page and scales of a run of tile `it`, two tiles before the tile is brought, so that no one waits for the
+        // chain from the table to the scales.  A run whose values' scale is not finite takes a key scale of NaN: rows that see it
+        // become NaN.  The tile's slot is free: whoever is two tiles behind has stored a tile whose stage the products had left.
+        auto look_up = [&](int it) {
+            if (p >= BN / 16 || it >= n_it) return;
+            const int j = first_of(it) + 16 * p;
+            RunConsts c = {0.0f, -INFINITY, 0.0f, 0.0f};             // keys of no page weigh nothing
+            long long off = -1;
+            if (j <= pos_last && (j + 15 >= lo_first || j < a.keep_first)) {
+                const int b = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
+                const int page = b < a.max_blocks ? table[b] : -1;
+                if (page >= 0 && page < a.num_pages) {
+                    off = page * a.page_stride + ((long long)kvh * a.page_size + (j - b * a.page_size)) * HD;
+                    const float vs = a.v_scale[(size_t)page * a.scale_stride + kvh];
+                    c.ks = a.k_scale[(size_t)page * a.scale_stride + kvh];
+                    const int e = (int)(__float_as_uint(vs) >> 23) & 255;
+                    c.ev = (float)(e - 127);
+                    c.inv = __uint_as_float((unsigned)max(254 - e, 0) << 23);
+                    if (e == 255) {
+                        c.ks = __uint_as_float(0x7fffffffu);
+                        c.ev = 0.0f;
+                        c.inv = 1.0f;
+                    }
+                } else if (a.status) {
+                    atomicOr(a.status, 16);
+                }
+            }
+            s_consts[it % CONSTS][p] = c;
+            s_off[it % CONSTS][p] = off;
+            mbar_arrive(&c_full[it % CONSTS]);
+        };
+        // A thread's pieces of a tile; bit i of the result: piece i is one that counts.  The others are read from where something is, so
+        // that no load hangs on a condition, and become zeros when stored.
+        auto load = [&](const uint8_t* from, int it, uint4 (&w)[EACH]) {
+            const int j0 = it < n_it ? first_of(it) : 0;
+            const bool every = it < n_it && j0 + BN - 1 <= pos_last && j0 >= lo_first;      // a query sees each of the tile's keys
+            unsigned counts = 0;
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                const int row = i * STEP + my_row;
+                const long long off = s_off[it % CONSTS][row >> 4];
+                const bool ok = it < n_it && off >= 0 && (every || seen(j0 + row));
+                if (ok) counts |= 1u << i;
+                w[i] = __ldg(reinterpret_cast<const uint4*>(from + (ok ? off + (row & 15) * HD : 0) + piece * 16));
+            }
+            return counts;
+        };
+        // 16 codes of row i * STEP + my_row: two pieces of eight half-precision numbers
+        auto store = [&](uint32_t to, uint4 (&w)[EACH], unsigned counts) {
+            if (counts != (1u << EACH) - 1) {
+#pragma unroll
+                for (int i = 0; i < EACH; i++)
+                    if (!((counts >> i) & 1)) w[i] = make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                const int row = i * STEP + my_row, c = 2 * piece;
+                const uint32_t at = to + (c >> 3) * HALF_TILE + row * 128;
+                uint32_t x[8];
+                decode4<CODE>(w[i].x, x[0], x[1]);
+                decode4<CODE>(w[i].y, x[2], x[3]);
+                decode4<CODE>(w[i].z, x[4], x[5]);
+                decode4<CODE>(w[i].w, x[6], x[7]);
+                sts128(at + (((c & 7) ^ (row & 7)) << 4), x[0], x[1], x[2], x[3]);
+                sts128(at + ((((c & 7) + 1) ^ (row & 7)) << 4), x[4], x[5], x[6], x[7]);
+            }
+        };
+        uint4 kw[EACH], vw[EACH];
+        look_up(0);
+        look_up(1);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        unsigned k_counts = load(a.k, 0, kw), v_counts = load(a.v, 0, vw);
+        for (int it = 0; it < n_it; it++) {
+            const int stage = it % STAGES;
+            look_up(it + 2);
+            asm volatile("bar.sync 1, 128;" ::: "memory");           // the producers: tile it + 1 has been looked up
+            if (it >= STAGES) wait_for(&k_empty[stage], (it / STAGES - 1) & 1);
+            store(base + OFF_K + stage * KV_BYTES, kw, k_counts);
+            fence_async_proxy();
+            mbar_arrive(&k_full[stage]);
+            k_counts = load(a.k, it + 1, kw);
+            if (it >= STAGES) wait_for(&v_empty[stage], (it / STAGES - 1) & 1);
+            store(base + OFF_V + stage * KV_BYTES, vw, v_counts);
+            fence_async_proxy();
+            mbar_arrive(&v_full[stage]);
+            v_counts = load(a.v, it + 1, vw);
+        }
+    } else {
+        if (tid == ISSUE_WARP * 32 && n_it > 0) {
+            // ---- products ------------------------------------------------------------------------------------------------------
+            auto issue_s = [&](int g, int stage) {
+                const uint32_t q = base + g * Q_BYTES, k = base + OFF_K + stage * KV_BYTES;
+#pragma unroll
+                for (int ks = 0; ks < HD / UMMA_K; ks++) {
+                    const uint32_t off = (ks >> 2) * HALF_TILE + (ks & 3) * 32;
+                    umma_bf16(tmem + s_col(g), make_smem_desc(q + off), make_smem_desc(k + off), IDESC_S, ks > 0);
+                }
+            };
+            auto issue_pv = [&](int g, int stage, bool first_tile) {
+                const uint32_t v = base + OFF_V + stage * KV_BYTES;
+#pragma unroll
+                for (int ks = 0; ks < BN / UMMA_K; ks++) {
+                    // 16 keys are 2,048 bytes further; the second run of 64 dims is HALF_TILE behind the first (the leading byte offset)
+                    uint64_t desc = make_smem_desc(v + ks * (UMMA_K * 128));
+                    if (SUBS == 2) desc = (desc & ~((uint64_t)0x3fff << 16)) | ((uint64_t)(HALF_TILE >> 4) << 16);
+                    umma_ta(tmem + o_col(g), tmem + s_col(g) + ks * (UMMA_K / 2), desc, IDESC_PV, !first_tile || ks > 0);
+                }
+            };
+            wait_for(&k_full[0], 0);
+            for (int g = 0; g < groups; g++) {
+                wait_for(&q_ready[g], 0);
+                tc_fence_after();
+                issue_s(g, 0);
+                umma_commit(&s_full[g]);
+            }
+            umma_commit(&k_empty[0]);
+            for (int it = 0; it < n_it; it++) {
+                const bool more = it + 1 < n_it;
+                for (int g = 0; g < groups; g++) {
+                    wait_for(&p_ready[g], it & 1);
+                    if (g == 0) wait_for(&v_full[it % STAGES], (it / STAGES) & 1);
+                    tc_fence_after();
+                    issue_pv(g, it % STAGES, it == 0);
+                    if (g == groups - 1) umma_commit(&v_empty[it % STAGES]);
+                    if (more) {
+                        if (g == 0) {
+                            wait_for(&k_full[(it + 1) % STAGES], ((it + 1) / STAGES) & 1);
+                            tc_fence_after();
+                        }
+                        issue_s(g, (it + 1) % STAGES);
+                        umma_commit(&s_full[g]);
+                    } else {
+                        umma_commit(&o_full[g]);
+                    }
+                }
+                if (more) umma_commit(&k_empty[(it + 1) % STAGES]);
+            }
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == ISSUE_WARP) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <int CODE, int HD>
+int launch(const Args& a, int n_seqs, int max_q_len, cudaStream_t stream) {
+    constexpr int SMEM = (2 + 2 * STAGES) * (HD / 64) * (int)HALF_TILE + 1024;
+    static std::atomic<unsigned long long> told{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return (int)e;
+    const unsigned long long bit = 1ull << (device & 63);
+    if (!(told.load() & bit) || device > 63) {
+        e = cudaFuncSetAttribute(prefill_8bit_kernel<CODE, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        if (e != cudaSuccess) return (int)e;
+        told.fetch_or(bit);
+    }
+    const dim3 grid((unsigned)(((long long)max_q_len * a.group + 255) / 256), a.n_kv_heads, n_seqs);
+    return sandy_launch(prefill_8bit_kernel<CODE, HD>, grid, dim3(THREADS), SMEM, stream, a);
+}
+
+}  // namespace
+
+// Arguments as sandy_attention_8bit (attention_8bit.cu) of prompt portions.  bfloat16, heads of 64 and 128, pages of a multiple of 16 keys,
+// rows of q and out on 16 bytes, a positive scale, no bias by distance; SANDY_ERR_UNSUPPORTED for everything else, which the other kernel
+// takes.  The scales of values are powers of two here (what appending gives), or not finite.
+SANDY_API int sandy_prefill_attention_8bit_tc(const void* q, long long ld_q, const void* k, const void* v, const float* k_scale,
+                                              const float* v_scale, long long page_stride, long long scale_stride, const int* block_table,
+                                              int max_blocks, const int* kv_before, const int* q_start, void* out, long long ld_out,
+                                              int n_rows, int n_seqs, int max_q_len, int n_heads, int n_kv_heads, int head_dim,
+                                              int page_size, int num_pages, float scale, const SandyAttentionRules* rules, int code,
+                                              int* status, cudaStream_t stream) {
+    if (n_seqs == 0 || max_q_len == 0) return SANDY_OK;
+    if (!rules || !q || !k || !v || !k_scale || !v_scale || !block_table || !kv_before || !q_start || !out || n_seqs < 0 || max_q_len < 0 ||
+        max_blocks < 1 || page_size < 1)
+        return SANDY_ERR_ARGUMENT;
+    if (rules->dist_bias || rules->window < 0 || rules->keep_first < 0 || rules->chunk < 0 || !(rules->softcap >= 0.0f) ||
+        (rules->keep_first > 0 && rules->chunk > 0) || (rules->elem_gate && rules->gate_dim < 1) || !(scale > 0.0f))
+        return SANDY_ERR_UNSUPPORTED;
+    if ((head_dim != 64 && head_dim != 128) || page_size % 16 || n_kv_heads < 1 || n_heads % n_kv_heads) return SANDY_ERR_UNSUPPORTED;
+    if (page_stride % 16 || (((uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)out) & 15) || ld_q % 8 || ld_out % 8 ||
+        n_seqs > 65535 || n_kv_heads > 65535 || (long long)max_q_len * (n_heads / n_kv_heads) > (1 << 28))
+        return SANDY_ERR_UNSUPPORTED;
+    const Args a = {(const bf16*)q, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, block_table, q_start, kv_before, (bf16*)out, status,
+                    rules->sink, rules->out_gate, (const bf16*)rules->elem_gate, ld_q, ld_out, page_stride, scale_stride, max_blocks, n_rows,
+                    n_heads, n_kv_heads, n_heads / n_kv_heads, page_size, (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1,
+                    num_pages, rules->window, rules->keep_first, rules->chunk, rules->ld_elem_gate, rules->gate_dim, scale, rules->softcap};
+    if (code == SANDY_E4M3 && head_dim == 64) return launch<SANDY_E4M3, 64>(a, n_seqs, max_q_len, stream);
+    if (code == SANDY_E4M3 && head_dim == 128) return launch<SANDY_E4M3, 128>(a, n_seqs, max_q_len, stream);
+    if (code == SANDY_INT8 && head_dim == 64) return launch<SANDY_INT8, 64>(a, n_seqs, max_q_len, stream);
+    if (code == SANDY_INT8 && head_dim == 128) return launch<SANDY_INT8, 128>(a, n_seqs, max_q_len, stream);
+    return SANDY_ERR_UNSUPPORTED;
+}

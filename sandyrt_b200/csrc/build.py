@@ -53,6 +53,7 @@ LIBRARIES: Dict[str, List[str]] = {
     "attention_prefill_f32_tc": [],
     "kv_8bit": [],
     "attention_8bit": [],
+    "attention_8bit_tc": [],
     "sampling": [],
     "logprobs": [],
     "rmsnorm": [],

@@ -614,6 +614,8 @@ _APPEND8 = (_V, _V, _L, _L, _V, _V, _V, _V, _L, _L, _V, _I, _V, _V, _I, _I, _I, 
 _READ8 = (_V, _V, _V, _V, _L, _L, _V, _I, _V, _V, _V, _V, _L, _L, _I, _I, _I, _I, _I, _I, _I, _I, _I, _V, _V)
 _ATTEND8 = (_V, _L, _V, _V, _V, _V, _L, _L, _V, _I, _I, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _I, _I, _I, _F, _V, _I, _I, _V, _I, _I, _V, _V)
 
+_PREFILL8_TC = (_V, _L, _V, _V, _V, _V, _L, _L, _V, _I, _V, _V, _V, _L, _I, _I, _I, _I, _I, _I, _I, _I, _F, _V, _I, _V, _V)
+
 
 def kv_append_8bit(k_src, v_src, cache: Cache8, block_table, q_start, kv_before, *, max_q_len: int) -> None:
     """Quantise the step's keys and values ([T, Hkv * D] views, float32 or bfloat16, a row pitch each) into their pages.
@@ -655,7 +657,7 @@ def kv_read_8bit(cache: Cache8, block_table, first, out_start, k_out, v_out, *, 
              k_out.stride(0), v_out.stride(0), S, k_out.shape[0], max_len, hkv, d, ps, pages, dtype, code, _status_word(device)), "kv_read_8bit")
 
 
-def _attention_8bit(what, q, cache, block_table, token_seq, positions, q_start, out, n_z, max_n, n_heads, scale, num_splits, rules) -> None:
+def _attention_8bit(what, q, cache, block_table, token_seq, positions, q_start, out, n_z, max_n, n_heads, scale, num_splits, rules, tc=False) -> None:
     hkv, ps, d, page_stride, scale_stride, pages, code = cache.check(what)
     if n_heads < 1 or n_heads % hkv:
         raise UnsupportedShape(f"{what}: {n_heads} heads do not divide into {hkv} key/value heads")
@@ -687,18 +689,27 @@ def _attention_8bit(what, q, cache, block_table, token_seq, positions, q_start, 
     if block_table.shape[0] == 0 or block_table.shape[1] == 0 or pages == 0:
         raise KernelError(f"{what}: an empty block table or cache")
     max_keys = min(block_table.shape[1] * ps, window + keep_first + max_n if window else 1 << 30)
+    args = _AttentionRules(window, keep_first, softcap, chunk, _at(sink), _at(out_gate), _at(dist_bias),
+                           0 if dist_bias is None else dist_bias.shape[1], _at(elem_gate), 0 if elem_gate is None else elem_gate.stride(0),
+                           0 if elem_gate is None else elem_gate.shape[1] // n_heads)
+    at = ctypes.addressof(args)
+    if tc:
+        if dtype != BF16:
+            raise UnsupportedShape(f"{what}: the tcgen05 kernel takes bfloat16")
+        _run_on(device, _entry("attention_8bit_tc", "sandy_prefill_attention_8bit_tc", _PREFILL8_TC),
+                (q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), page_stride,
+                 scale_stride, block_table.data_ptr(), block_table.shape[1], positions.data_ptr(), q_start.data_ptr(), out.data_ptr(), out.stride(0),
+                 T, n_z, max_n, n_heads, hkv, d, ps, pages, scale, at, code, _status_word(device)), f"{what}(tc,H={n_heads},Hkv={hkv},D={d},page={ps})")
+        return
     # partial results of many splits: memory of the stream the call is on, given back to the allocator when it returns
     floats = ctypes.c_longlong(0)
     splits = _entry("attention_8bit", "sandy_attention_8bit_splits", (_I,) * 9 + (_V,))(T, n_z, max_n, n_heads, hkv, d, max_keys, dtype, num_splits,
                                                                                         ctypes.addressof(floats))
     scratch = torch.empty(floats.value, dtype=torch.float32, device=device) if floats.value else None
-    args = _AttentionRules(window, keep_first, softcap, chunk, _at(sink), _at(out_gate), _at(dist_bias),
-                           0 if dist_bias is None else dist_bias.shape[1], _at(elem_gate), 0 if elem_gate is None else elem_gate.stride(0),
-                           0 if elem_gate is None else elem_gate.shape[1] // n_heads)
     _run_on(device, _entry("attention_8bit", "sandy_attention_8bit", _ATTEND8),
             (q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), page_stride,
              scale_stride, block_table.data_ptr(), block_table.shape[1], block_table.shape[0], _at(token_seq), positions.data_ptr(), _at(q_start),
-             out.data_ptr(), out.stride(0), T, n_z, max_n, n_heads, hkv, d, ps, pages, scale, ctypes.addressof(args), max_keys, splits, _at(scratch),
+             out.data_ptr(), out.stride(0), T, n_z, max_n, n_heads, hkv, d, ps, pages, scale, at, max_keys, splits, _at(scratch),
              dtype, code, _status_word(device)), f"{what}(H={n_heads},Hkv={hkv},D={d},page={ps},splits={splits})")
     if scratch is not None:
         global LAUNCHES
@@ -722,18 +733,34 @@ def decode_attention_8bit(q, cache: Cache8, block_table, token_seq, positions, o
     _attention_8bit("decode_attention_8bit", q, cache, block_table, token_seq, positions, None, out, T, 1, n_heads, scale, num_splits, rules)
 
 
+# From so many rows (tokens x heads of a group) of the longest portion on, 8-bit prompt attention goes to the tcgen05 kernel.
+TC_ROWS_8BIT = 64
+
+
+def prefill_8bit_on_tcgen05(q, cache: Cache8, out, n_heads: int, scale: float, dist_bias=None) -> bool:
+    """Whether the tcgen05 kernel of 8-bit prompt attention takes a call: bfloat16, heads of 64 or 128, pages of a multiple of 16 keys, rows
+    on 16-byte boundaries, a positive scale, no bias by distance."""
+    _, _, ps, d = cache.k.shape
+    return (q.dtype == torch.bfloat16 and d in (64, 128) and ps % 16 == 0 and scale > 0 and dist_bias is None
+            and not (q.data_ptr() | out.data_ptr()) % 16 and not (q.stride(0) | out.stride(0)) % 8)
+
+
 def prefill_attention_8bit(q, cache: Cache8, block_table, q_start, kv_before, out, *, n_heads: int, max_q_len: int, scale: float,
-                           num_splits: int = 0, **rules) -> None:
+                           num_splits: int = 0, tc: Optional[bool] = None, **rules) -> None:
     """Attention of prompt portions over a cache in 8 bits: request s of the block table's rows brings rows q_start[s] ..
     q_start[s + 1] - 1 (int32 [S + 1]) at its positions kv_before[s] on (int32 [S]), whose keys and values kv_append_8bit has
     written; max_q_len: the most that one request brings.  Types, sizes and rules as in decode_attention_8bit; portions of one
-    token are allowed.  Rows of no request are left as they were."""
+    token are allowed.  Rows of no request are left as they were.  tc: True asks for the tcgen05 kernel (prefill_8bit_on_tcgen05),
+    False for the mma.sync one, None picks; num_splits is the latter's."""
     _known_rules("prefill_attention_8bit", rules)
     S = _portions("prefill_attention_8bit", block_table, q_start, kv_before)
     if max_q_len < 0:
         raise KernelError("prefill_attention_8bit: max_q_len is negative")
+    if tc is None:
+        tc = not num_splits and max_q_len * n_heads >= TC_ROWS_8BIT * cache.k.shape[1] and prefill_8bit_on_tcgen05(
+            q, cache, out, n_heads, scale, rules.get("dist_bias"))
     _attention_8bit("prefill_attention_8bit", q, cache, block_table, None, kv_before, q_start, out, S, max_q_len, n_heads, scale, num_splits,
-                    rules)
+                    rules, tc)
 
 
 def _known_rules(what: str, rules: dict) -> None:

@@ -486,6 +486,13 @@ int sandy_attention_8bit(const void* q, long long ld_q, const void* k, const voi
                          const SandyAttentionRules* rules, int max_keys, int num_splits, float* scratch, int dtype, int code, int* status,
                          cudaStream_t stream);
 
+/* attention_8bit_tc.cu */
+int sandy_prefill_attention_8bit_tc(const void* q, long long ld_q, const void* k, const void* v, const float* k_scale,
+                                    const float* v_scale, long long page_stride, long long scale_stride, const int* block_table,
+                                    int max_blocks, const int* kv_before, const int* q_start, void* out, long long ld_out, int n_rows,
+                                    int n_seqs, int max_q_len, int n_heads, int n_kv_heads, int head_dim, int page_size, int num_pages,
+                                    float scale, const SandyAttentionRules* rules, int code, int* status, cudaStream_t stream);
+
 /* logprobs.cu */
 int sandy_token_logprobs(const void* logits, long long ld, int n_rows, int vocab, const int* ids, int top, float* logprob,
                          float* entropy, int* top_ids, float* top_logprobs, int dtype, int* status, cudaStream_t stream);

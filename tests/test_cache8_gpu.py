@@ -255,7 +255,7 @@ def _rules_on_host(rules):
     return {k: v.double().cpu() if isinstance(v, torch.Tensor) else v for k, v in rules.items()}
 
 
-def _check_attention(code, dtype, H, hkv, d, ps, seqs, decode, seed=0, splits=0, q_scale=1.0, more=0.0, **rules):
+def _check_attention(code, dtype, H, hkv, d, ps, seqs, decode, seed=0, splits=0, q_scale=1.0, more=0.0, tc=None, **rules):
     """seqs: (positions in the cache before, new tokens) of each request; single tokens go to requests in another order."""
     from sandyrt_b200.csrc import ops
 
@@ -281,7 +281,7 @@ def _check_attention(code, dtype, H, hkv, d, ps, seqs, decode, seed=0, splits=0,
         rows = [(s, [t], [seqs[s][0]]) for t, s in enumerate(order)]
     else:
         ops.prefill_attention_8bit(q, dev, table, _i32(starts), _i32([b for b, _ in seqs]), out[:, :H * d], n_heads=H, max_q_len=max(lens),
-                                   scale=scale, num_splits=splits, **rules)
+                                   scale=scale, num_splits=splits, tc=tc, **rules)
         rows = [(s, list(range(starts[s], starts[s + 1])), list(range(b, b + m))) for s, (b, m) in enumerate(seqs)]
     ops.check_kernel_status(DEV)
     got = out.cpu().double()
@@ -331,6 +331,29 @@ def test_rules(code, dtype, H, hkv, d, ps, decode, rules):
 def test_prompt_portions(code, dtype, H, hkv, d, ps):
     _check_attention(code, dtype, H, hkv, d, ps, [(0, 1), (0, 130), (100, 33), (3, 0), (127, 2), (250, 17)], False)
     _check_attention(code, dtype, H, hkv, d, ps, [(300, 140)], False, seed=1)
+
+
+@pytest.mark.parametrize("code", list(CODES))
+@pytest.mark.parametrize("H,hkv,d,ps", [(2, 2, 64, 16), (2, 2, 128, 32), (12, 3, 64, 48), (8, 1, 128, 16), (3, 1, 64, 256)])
+@pytest.mark.parametrize("seqs", [[(0, 1)], [(0, 128)], [(0, 129), (5, 0), (511, 2)], [(0, 300), (130, 40)], [(400, 257)], [(1000, 8), (0, 8)]])
+def test_prompt_portions_on_tcgen05(code, H, hkv, d, ps, seqs):
+    _check_attention(code, "bf16", H, hkv, d, ps, seqs, False, tc=True)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rules", [r for r in RULES if "dist_bias" not in r], ids=lambda r: "-".join(r))
+def test_rules_on_tcgen05(d, rules):
+    _check_attention("e4m3", "bf16", 4, 2, d, 16, [(0, 150), (290, 1), (0, 0), (333, 170)], False, tc=True, **dict(rules))
+
+
+def test_calls_the_tcgen05_kernel_does_not_take():
+    from sandyrt_b200.errors import UnsupportedShape
+
+    for H, hkv, d, ps, dtype, rules in ((2, 2, 64, 8, "bf16", {}), (2, 2, 96, 16, "bf16", {}), (2, 2, 64, 16, "bf16", dict(dist_bias=True))):
+        with pytest.raises(UnsupportedShape):
+            _check_attention("int8", dtype, H, hkv, d, ps, [(0, 70)], False, tc=True, **rules)
+    with pytest.raises(UnsupportedShape):
+        _check_attention("int8", "f32", 2, 2, 64, 16, [(0, 70)], False, tc=True)
 
 
 @pytest.mark.parametrize("splits", [1, 2, 5])
