@@ -97,6 +97,27 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+// One arrival for a warp whose lanes have all fenced what they wrote.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+// two 32-bit operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -111,7 +132,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
     constexpr uint32_t IDESC_S = idesc_f16(BN), IDESC_PV = idesc_f16(HD) | (1u << 16);        // V: MN-major
     extern __shared__ uint8_t smem_raw[];
     __shared__ RunConsts s_consts[CONSTS][BN / 16];
-    __shared__ long long s_off[CONSTS][BN / 16];         // where a run's rows lie in keys and values, -1: nowhere
+    __shared__ long long s_off[CONSTS][BN / 16];         // where a run's rows lie in keys and values (page 0's, if nowhere)
+    __shared__ unsigned s_good[CONSTS];                  // the tile's runs that have a page, a bit each
     __shared__ uint64_t q_ready[2], k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_ready[2], o_full[2], c_full[CONSTS];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int s_failed;
@@ -143,15 +165,15 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
 
     if (tid == 0) {
         for (int g = 0; g < 2; g++) {
-            mbar_init(&q_ready[g], 128);
+            mbar_init(&q_ready[g], 4);
             mbar_init(&s_full[g], 1);
-            mbar_init(&p_ready[g], 128);
+            mbar_init(&p_ready[g], 4);
             mbar_init(&o_full[g], 1);
         }
         for (int i = 0; i < STAGES; i++) {
-            mbar_init(&k_full[i], 128);
+            mbar_init(&k_full[i], 4);
             mbar_init(&k_empty[i], 1);
-            mbar_init(&v_full[i], 128);
+            mbar_init(&v_full[i], 4);
             mbar_init(&v_empty[i], 1);
         }
         for (int i = 0; i < CONSTS; i++) mbar_init(&c_full[i], BN / 16);
@@ -204,7 +226,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                 sts128(to + (c >> 3) * HALF_TILE + (((c & 7) ^ (r & 7)) << 4), two(w.x), two(w.y), two(w.z), two(w.w));
             }
             fence_async_proxy();
-            mbar_arrive(&q_ready[g]);
+            warp_arrive(&q_ready[g]);
         }
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         float M = -INFINITY, l = 0.0f;
@@ -302,22 +324,23 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                 for (int u = 0; u < 4; u++) {
                     const RunConsts c = consts[4 * half + u];
                     const float f = whole ? c.ks * factor : 1.0f, off = (whole ? c.ev : 0.0f) - m_use;
-                    float sum0 = 0.0f, sum1 = 0.0f;
+                    float2 sum = {0.0f, 0.0f};
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        const float p0 = ex2(fmaf(__uint_as_float(s[16 * u + e]), f, off)), p1 = ex2(fmaf(__uint_as_float(s[16 * u + e + 1]), f, off));
-                        sum0 += p0;
-                        sum1 += p1;
-                        s[8 * u + e / 2] = pack_half(p0, p1);
+                        float2 x = fma2(make_float2(__uint_as_float(s[16 * u + e]), __uint_as_float(s[16 * u + e + 1])), make_float2(f, f), make_float2(off, off));
+                        x.x = ex2(x.x);
+                        x.y = ex2(x.y);
+                        sum = add2(sum, x);
+                        s[8 * u + e / 2] = pack_half(x.x, x.y);
                     }
-                    l = fmaf(sum0 + sum1, c.inv, l);
+                    l = fmaf(sum.x + sum.y, c.inv, l);
                 }
                 // over columns whose scores have been read: 0..31 of the tile's 128, then 32..63
                 tmem_st_32x32(lanes + s_col(g) + 32 * half, s);
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&p_ready[g]);
+            warp_arrive(&p_ready[g]);
         }
         if (g < groups) {
             if (n_it > 0) {
@@ -363,12 +386,14 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
         auto look_up = [&](int it) {
             if (p >= BN / 16 || it >= n_it) return;
             const int j = first_of(it) + 16 * p;
+            bool good = false;
             RunConsts c = {0.0f, -INFINITY, 0.0f, 0.0f};             // keys of no page weigh nothing
-            long long off = -1;
+            long long off = 0;
             if (j <= pos_last && (j + 15 >= lo_first || j < a.keep_first)) {
                 const int b = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
                 const int page = b < a.max_blocks ? table[b] : -1;
                 if (page >= 0 && page < a.num_pages) {
+                    good = true;
                     off = page * a.page_stride + ((long long)kvh * a.page_size + (j - b * a.page_size)) * HD;
                     const float vs = a.v_scale[(size_t)page * a.scale_stride + kvh];
                     c.ks = a.k_scale[(size_t)page * a.scale_stride + kvh];
@@ -386,21 +411,28 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             }
             s_consts[it % CONSTS][p] = c;
             s_off[it % CONSTS][p] = off;
+            const unsigned all = __ballot_sync(0xffu, good);
+            if (p == 0) s_good[it % CONSTS] = all;
             mbar_arrive(&c_full[it % CONSTS]);
         };
         // A thread's pieces of a tile; bit i of the result: piece i is one that counts.  The others are read from where something is, so
         // that no load hangs on a condition, and become zeros when stored.
         auto load = [&](const uint8_t* from, int it, uint4 (&w)[EACH]) {
-            const int j0 = it < n_it ? first_of(it) : 0;
-            const bool every = it < n_it && j0 + BN - 1 <= pos_last && j0 >= lo_first;      // a query sees each of the tile's keys
-            unsigned counts = 0;
+            if (it >= n_it) return 0u;
+            const int j0 = first_of(it), at = it % CONSTS;
+            const unsigned good = s_good[at];
+            unsigned counts = (1u << EACH) - 1;
+            if (good != 0xff || j0 + BN - 1 > pos_last || j0 < lo_first) {       // not every key has a page and is seen by a query
+#pragma unroll
+                for (int i = 0; i < EACH; i++) {
+                    const int row = i * STEP + my_row;
+                    if (!((good >> (row >> 4)) & 1) || !seen(j0 + row)) counts &= ~(1u << i);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < EACH; i++) {
                 const int row = i * STEP + my_row;
-                const long long off = s_off[it % CONSTS][row >> 4];
-                const bool ok = it < n_it && off >= 0 && (every || seen(j0 + row));
-                if (ok) counts |= 1u << i;
-                w[i] = __ldg(reinterpret_cast<const uint4*>(from + (ok ? off + (row & 15) * HD : 0) + piece * 16));
+                w[i] = __ldg(reinterpret_cast<const uint4*>(from + s_off[at][row >> 4] + ((row & 15) * HD + piece * 16)));
             }
             return counts;
         };
@@ -436,12 +468,12 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             if (it >= STAGES) wait_for(&k_empty[stage], (it / STAGES - 1) & 1);
             store(base + OFF_K + stage * KV_BYTES, kw, k_counts);
             fence_async_proxy();
-            mbar_arrive(&k_full[stage]);
+            warp_arrive(&k_full[stage]);
             k_counts = load(a.k, it + 1, kw);
             if (it >= STAGES) wait_for(&v_empty[stage], (it / STAGES - 1) & 1);
             store(base + OFF_V + stage * KV_BYTES, vw, v_counts);
             fence_async_proxy();
-            mbar_arrive(&v_full[stage]);
+            warp_arrive(&v_full[stage]);
             v_counts = load(a.v, it + 1, vw);
         }
     } else {
@@ -475,17 +507,15 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             umma_commit(&k_empty[0]);
             for (int it = 0; it < n_it; it++) {
                 const bool more = it + 1 < n_it;
+                // what the products need beside the weights, long there: a wait costs some 300 cycles even so, and none may follow the weights
+                wait_for(&v_full[it % STAGES], (it / STAGES) & 1);
+                if (more) wait_for(&k_full[(it + 1) % STAGES], ((it + 1) / STAGES) & 1);
                 for (int g = 0; g < groups; g++) {
                     wait_for(&p_ready[g], it & 1);
-                    if (g == 0) wait_for(&v_full[it % STAGES], (it / STAGES) & 1);
                     tc_fence_after();
                     issue_pv(g, it % STAGES, it == 0);
                     if (g == groups - 1) umma_commit(&v_empty[it % STAGES]);
                     if (more) {
-                        if (g == 0) {
-                            wait_for(&k_full[(it + 1) % STAGES], ((it + 1) / STAGES) & 1);
-                            tc_fence_after();
-                        }
                         issue_s(g, (it + 1) % STAGES);
                         umma_commit(&s_full[g]);
                     } else {
