@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
     __shared__ RunConsts s_consts[CONSTS][BN / 16];
     __shared__ long long s_off[CONSTS][BN / 16];         // where a run's rows lie in keys and values (page 0's, if nowhere)
     __shared__ unsigned s_good[CONSTS];                  // the tile's runs that have a page, a bit each
-    __shared__ uint64_t q_ready[2], k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_ready[2], o_full[2], c_full[CONSTS];
+    __shared__ uint64_t q_ready[2], first_k, k_empty[STAGES], v_empty[STAGES], s_full[2], go[2][2], o_full[2], c_full[CONSTS];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int s_failed;
 
@@ -167,13 +167,14 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
         for (int g = 0; g < 2; g++) {
             mbar_init(&q_ready[g], 4);
             mbar_init(&s_full[g], 1);
-            mbar_init(&p_ready[g], 4);
+            // per tile of rows and parity of the key tile: its weights, V of the key tile and K of the next are there
+            mbar_init(&go[g][0], 12);
+            mbar_init(&go[g][1], 12);
             mbar_init(&o_full[g], 1);
         }
+        mbar_init(&first_k, 4);
         for (int i = 0; i < STAGES; i++) {
-            mbar_init(&k_full[i], 4);
             mbar_init(&k_empty[i], 1);
-            mbar_init(&v_full[i], 4);
             mbar_init(&v_empty[i], 1);
         }
         for (int i = 0; i < CONSTS; i++) mbar_init(&c_full[i], BN / 16);
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     auto wait_for = [&](uint64_t* bar, uint32_t parity) {
-        if (s_failed) return;
+        if (mbar_try_wait(bar, parity) || s_failed) return;
         if (!mbar_wait(bar, parity)) {
             if (a.status) atomicOr(a.status, 256);
             s_failed = 1;
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             }
             tmem_wait_st();
             tc_fence_before();
-            warp_arrive(&p_ready[g]);
+            warp_arrive(&go[g][it & 1]);
         }
         if (g < groups) {
             if (n_it > 0) {
@@ -468,12 +469,21 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             if (it >= STAGES) wait_for(&k_empty[stage], (it / STAGES - 1) & 1);
             store(base + OFF_K + stage * KV_BYTES, kw, k_counts);
             fence_async_proxy();
-            warp_arrive(&k_full[stage]);
+            // K of tile it is what the products after tile it - 1's weights wait for, V what those after its own do
+            if (it == 0) {
+                warp_arrive(&first_k);
+            } else {
+                warp_arrive(&go[0][(it - 1) & 1]);
+                if (groups == 2) warp_arrive(&go[1][(it - 1) & 1]);
+            }
             k_counts = load(a.k, it + 1, kw);
             if (it >= STAGES) wait_for(&v_empty[stage], (it / STAGES - 1) & 1);
             store(base + OFF_V + stage * KV_BYTES, vw, v_counts);
             fence_async_proxy();
-            warp_arrive(&v_full[stage]);
+            for (int g = 0; g < groups; g++) {
+                warp_arrive(&go[g][it & 1]);
+                if (it == n_it - 1) warp_arrive(&go[g][it & 1]);     // there is no next K
+            }
             v_counts = load(a.v, it + 1, vw);
         }
     } else {
@@ -497,7 +507,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                     umma_ta(tmem + o_col(g), tmem + s_col(g) + ks * (UMMA_K / 2), desc, IDESC_PV, !first_tile || ks > 0);
                 }
             };
-            wait_for(&k_full[0], 0);
+            wait_for(&first_k, 0);
             for (int g = 0; g < groups; g++) {
                 wait_for(&q_ready[g], 0);
                 tc_fence_after();
@@ -507,11 +517,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             umma_commit(&k_empty[0]);
             for (int it = 0; it < n_it; it++) {
                 const bool more = it + 1 < n_it;
-                // what the products need beside the weights, long there: a wait costs some 300 cycles even so, and none may follow the weights
-                wait_for(&v_full[it % STAGES], (it / STAGES) & 1);
-                if (more) wait_for(&k_full[(it + 1) % STAGES], ((it + 1) / STAGES) & 1);
                 for (int g = 0; g < groups; g++) {
-                    wait_for(&p_ready[g], it & 1);
+                    // one wait for all that the products need: each costs some 300 cycles, even when it is over
+                    wait_for(&go[g][it & 1], (it >> 1) & 1);
                     tc_fence_after();
                     issue_pv(g, it % STAGES, it == 0);
                     if (g == groups - 1) umma_commit(&v_empty[it % STAGES]);
