@@ -34,8 +34,10 @@
 
 #include <cooperative_groups.h>
 
-#include "attention_rules.h"
+#include "cache8.h"
 #include "kv_8bit.cuh"
+
+static_assert(sizeof(SandyAttend8) == 256, "the layout callers lay down");
 
 namespace cg = cooperative_groups;
 
@@ -810,45 +812,76 @@ SANDY_API int sandy_attention_8bit_splits(int n_rows, int n_z, int max_n, int n_
     return (int)splits;
 }
 
-// Attention of prompt portions (q_start [n_z + 1], positions = kv_before [n_z], token_seq null, request z = row z of the block
-// table; max_n: the most tokens of one) or of single tokens (q_start null: token z of request token_seq[z] at positions[z]; max_n 1).
-// q: [n_rows, H * D], out likewise, row pitches ld_q and ld_out (elements); k, v, scales and table as sandy_kv_append_8bit has them,
-// n_seqs rows in the table.  max_keys: the most keys that
-// one of a request's blocks of queries sees, by which the splits are cut; `scratch` as sandy_attention_8bit_splits says.  A row without a visible key
-// becomes zeros.  Bit 4 of *status: a visible key without a page, a token of no request, or rows past n_rows.
-SANDY_API int sandy_attention_8bit(const void* q, long long ld_q, const void* k, const void* v, const float* k_scale,
-                                   const float* v_scale, long long page_stride, long long scale_stride, const int* block_table,
-                                   int max_blocks, int n_seqs, const int* token_seq, const int* positions, const int* q_start, void* out,
-                                   long long ld_out, int n_rows, int n_z, int max_n, int n_heads, int n_kv_heads, int head_dim,
-                                   int page_size, int num_pages, float scale, const SandyAttentionRules* rules, int max_keys,
-                                   int num_splits, float* scratch,
-                                   int dtype, int code, int* status, cudaStream_t stream) {
-    if (n_z == 0 || max_n == 0) return SANDY_OK;
-    if (!rules || !q || !k || !v || !k_scale || !v_scale || !block_table || !positions || !out || !(token_seq || q_start) || n_z < 0 ||
-        max_n < 0 || n_seqs < 1 || max_blocks < 1 || page_size < 1 || max_keys < 1 || num_splits < 1)
+// Attention of prompt portions or of single tokens (cache8.h).  max_keys: the most keys that one of a request's blocks of queries sees, by
+// which the splits are cut; `scratch` as sandy_attention_8bit_splits says.  A row without a visible key becomes zeros.  Bit 4 of *status:
+// a visible key without a page, a token of no request, or rows past n_rows.
+SANDY_API int sandy_attention_8bit(const SandyAttend8* r, cudaStream_t stream) {
+    if (!r) return SANDY_ERR_ARGUMENT;
+    const SandyCache8& c = r->cache;
+    const SandyAttentionRules& rules = r->rules;
+    if (r->n_z == 0 || r->max_n == 0) return SANDY_OK;
+    if (!r->q || !r->out || !r->positions || !(r->token_seq || r->q_start) || !c.k || !c.v || !c.k_scale || !c.v_scale || !c.block_table ||
+        r->n_z < 0 || r->max_n < 0 || c.n_seqs < 1 || c.max_blocks < 1 || c.page_size < 1 || r->max_keys < 1 || r->num_splits < 1)
         return SANDY_ERR_ARGUMENT;
-    if (rules->dist_bias && rules->n_dist < 1) return SANDY_ERR_ARGUMENT;
-    if (rules->window < 0 || rules->keep_first < 0 || rules->chunk < 0 || !(rules->softcap >= 0.0f) ||
-        (rules->keep_first > 0 && rules->chunk > 0) || (rules->elem_gate && rules->gate_dim < 1))
+    if (rules.dist_bias && rules.n_dist < 1) return SANDY_ERR_ARGUMENT;
+    if (rules.window < 0 || rules.keep_first < 0 || rules.chunk < 0 || !(rules.softcap >= 0.0f) || (rules.keep_first > 0 && rules.chunk > 0) ||
+        (rules.elem_gate && rules.gate_dim < 1))
         return SANDY_ERR_UNSUPPORTED;
-    if (head_dim < 16 || head_dim % 16 || head_dim > 256 || n_kv_heads < 1 || n_heads % n_kv_heads) return SANDY_ERR_UNSUPPORTED;
-    if (page_stride % 16 || (((uintptr_t)k | (uintptr_t)v) & 15) || n_z > 65535 || n_kv_heads > 65535) return SANDY_ERR_UNSUPPORTED;
-    const long long queries = (long long)max_n * (n_heads / n_kv_heads);
-    if (queries > (1 << 28) || queries * num_splits > 0x7fffffffll || (long long)max_n * n_heads > 0x7fffffffll || num_splits > MAX_SPLITS)
+    if (c.head_dim < 16 || c.head_dim % 16 || c.head_dim > 256 || c.n_kv_heads < 1 || r->n_heads % c.n_kv_heads) return SANDY_ERR_UNSUPPORTED;
+    if (c.page_stride % 16 || (((uintptr_t)c.k | (uintptr_t)c.v) & 15) || r->n_z > 65535 || c.n_kv_heads > 65535) return SANDY_ERR_UNSUPPORTED;
+    const int group = r->n_heads / c.n_kv_heads, es = c.dtype == SANDY_F32 ? 4 : 2;
+    const long long queries = (long long)r->max_n * group;
+    if (queries > (1 << 28) || queries * r->num_splits > 0x7fffffffll || (long long)r->max_n * r->n_heads > 0x7fffffffll || r->num_splits > MAX_SPLITS)
         return SANDY_ERR_UNSUPPORTED;
-    const bool in_cluster = num_splits > 1 && num_splits <= MAX_CLUSTER && !is_wide(queries, head_dim, dtype);
-    if (num_splits > 1 && !in_cluster && !scratch) return SANDY_ERR_ARGUMENT;
+    const bool in_cluster = r->num_splits > 1 && r->num_splits <= MAX_CLUSTER && !is_wide(queries, c.head_dim, c.dtype);
+    if (r->num_splits > 1 && !in_cluster && !r->scratch) return SANDY_ERR_ARGUMENT;
+    Args a = {};
+    a.q = r->q;
+    a.k = (const uint8_t*)c.k;
+    a.v = (const uint8_t*)c.v;
+    a.k_scale = c.k_scale;
+    a.v_scale = c.v_scale;
+    a.block_table = c.block_table;
+    a.token_seq = r->token_seq;
+    a.positions = r->positions;
+    a.q_start = r->q_start;
+    a.out = r->out;
+    a.scratch = r->scratch;
+    a.status = c.status;
+    a.sink = rules.sink;
+    a.out_gate = rules.out_gate;
+    a.dist_bias = rules.dist_bias;
+    a.elem_gate = rules.elem_gate;
+    a.ld_q = r->ld_q;
+    a.ld_out = r->ld_out;
+    a.page_stride = c.page_stride;
+    a.scale_stride = c.scale_stride;
+    a.max_blocks = c.max_blocks;
+    a.n_rows = r->n_rows;
+    a.n_seqs = c.n_seqs;
+    a.n_heads = r->n_heads;
+    a.n_kv_heads = c.n_kv_heads;
+    a.head_dim = c.head_dim;
+    a.page_size = c.page_size;
+    a.num_pages = c.num_pages;
+    a.num_splits = r->num_splits;
     // a split's tiles of 16 keys, an even number; two more for the ends of a window and of the kept keys
-    const int split_tiles = (((max_keys - 1) / 16 + 3 + num_splits - 1) / num_splits + 1) / 2 * 2;
-    const Args a = {q, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, block_table, token_seq, positions, q_start, out, scratch,
-                    status, rules->sink, rules->out_gate, rules->dist_bias, rules->elem_gate, ld_q, ld_out, page_stride, scale_stride,
-                    max_blocks, n_rows, n_seqs, n_heads, n_kv_heads, head_dim, page_size, num_pages, num_splits, split_tiles, n_heads / n_kv_heads,
-                    (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1, rules->window,
-                    rules->keep_first, rules->chunk, rules->n_dist, rules->ld_elem_gate, rules->gate_dim, scale, rules->softcap, in_cluster,
-                    (((uintptr_t)q | (uintptr_t)(ld_q * (dtype == SANDY_F32 ? 4 : 2))) & 15) == 0};
-    if (dtype == SANDY_F32 && code == SANDY_E4M3) return launch<float, SANDY_E4M3>(a, n_z, (int)queries, max_n, stream);
-    if (dtype == SANDY_F32 && code == SANDY_INT8) return launch<float, SANDY_INT8>(a, n_z, (int)queries, max_n, stream);
-    if (dtype == SANDY_BF16 && code == SANDY_E4M3) return launch<bf16, SANDY_E4M3>(a, n_z, (int)queries, max_n, stream);
-    if (dtype == SANDY_BF16 && code == SANDY_INT8) return launch<bf16, SANDY_INT8>(a, n_z, (int)queries, max_n, stream);
+    a.split_tiles = (((r->max_keys - 1) / 16 + 3 + r->num_splits - 1) / r->num_splits + 1) / 2 * 2;
+    a.group = group;
+    a.page_shift = (c.page_size & (c.page_size - 1)) == 0 ? __builtin_ctz(c.page_size) : -1;
+    a.window = rules.window;
+    a.keep_first = rules.keep_first;
+    a.chunk = rules.chunk;
+    a.n_dist = rules.n_dist;
+    a.ld_elem_gate = rules.ld_elem_gate;
+    a.gate_dim = rules.gate_dim;
+    a.scale = r->scale;
+    a.softcap = rules.softcap;
+    a.in_cluster = in_cluster;
+    a.q_aligned = (((uintptr_t)r->q | (uintptr_t)(r->ld_q * es)) & 15) == 0;
+    if (c.dtype == SANDY_F32 && c.code == SANDY_E4M3) return launch<float, SANDY_E4M3>(a, r->n_z, (int)queries, r->max_n, stream);
+    if (c.dtype == SANDY_F32 && c.code == SANDY_INT8) return launch<float, SANDY_INT8>(a, r->n_z, (int)queries, r->max_n, stream);
+    if (c.dtype == SANDY_BF16 && c.code == SANDY_E4M3) return launch<bf16, SANDY_E4M3>(a, r->n_z, (int)queries, r->max_n, stream);
+    if (c.dtype == SANDY_BF16 && c.code == SANDY_INT8) return launch<bf16, SANDY_INT8>(a, r->n_z, (int)queries, r->max_n, stream);
     return SANDY_ERR_UNSUPPORTED;
 }

@@ -26,7 +26,7 @@
 // Every wait on an mbarrier is bounded; one that runs out raises bit 8 of the status word and the block ends without waiting again.
 #include <atomic>
 
-#include "attention_rules.h"
+#include "cache8.h"
 #include "kv_8bit.cuh"
 #include "tcgen05.cuh"
 
@@ -562,33 +562,60 @@ int launch(const Args& a, int n_seqs, int max_q_len, cudaStream_t stream) {
 
 }  // namespace
 
-// Arguments as sandy_attention_8bit (attention_8bit.cu) of prompt portions.  bfloat16, heads of 64 and 128, pages of a multiple of 16 keys,
-// rows of q and out on 16 bytes, a positive scale, no bias by distance; SANDY_ERR_UNSUPPORTED for everything else, which the other kernel
-// takes.  The scales of values are powers of two here (what appending gives), or not finite.
-SANDY_API int sandy_prefill_attention_8bit_tc(const void* q, long long ld_q, const void* k, const void* v, const float* k_scale,
-                                              const float* v_scale, long long page_stride, long long scale_stride, const int* block_table,
-                                              int max_blocks, const int* kv_before, const int* q_start, void* out, long long ld_out,
-                                              int n_rows, int n_seqs, int max_q_len, int n_heads, int n_kv_heads, int head_dim,
-                                              int page_size, int num_pages, float scale, const SandyAttentionRules* rules, int code,
-                                              int* status, cudaStream_t stream) {
-    if (n_seqs == 0 || max_q_len == 0) return SANDY_OK;
-    if (!rules || !q || !k || !v || !k_scale || !v_scale || !block_table || !kv_before || !q_start || !out || n_seqs < 0 || max_q_len < 0 ||
-        max_blocks < 1 || page_size < 1)
+// Prompt portions as sandy_attention_8bit (attention_8bit.cu) takes them, without splits.  bfloat16, heads of 64 and 128, pages of a multiple
+// of 16 keys, rows of q and out on 16 bytes, a positive scale, no bias by distance; SANDY_ERR_UNSUPPORTED for everything else, which the
+// other kernel takes.  The scales of values are powers of two here (what appending gives), or not finite.
+SANDY_API int sandy_prefill_attention_8bit_tc(const SandyAttend8* r, cudaStream_t stream) {
+    if (!r) return SANDY_ERR_ARGUMENT;
+    const SandyCache8& c = r->cache;
+    const SandyAttentionRules& rules = r->rules;
+    if (r->n_z == 0 || r->max_n == 0) return SANDY_OK;
+    if (!r->q || !r->out || !r->positions || !r->q_start || !c.k || !c.v || !c.k_scale || !c.v_scale || !c.block_table || r->n_z < 0 ||
+        r->max_n < 0 || c.max_blocks < 1 || c.page_size < 1)
         return SANDY_ERR_ARGUMENT;
-    if (rules->dist_bias || rules->window < 0 || rules->keep_first < 0 || rules->chunk < 0 || !(rules->softcap >= 0.0f) ||
-        (rules->keep_first > 0 && rules->chunk > 0) || (rules->elem_gate && rules->gate_dim < 1) || !(scale > 0.0f))
+    if (c.dtype != SANDY_BF16 || rules.dist_bias || rules.window < 0 || rules.keep_first < 0 || rules.chunk < 0 || !(rules.softcap >= 0.0f) ||
+        (rules.keep_first > 0 && rules.chunk > 0) || (rules.elem_gate && rules.gate_dim < 1) || !(r->scale > 0.0f))
         return SANDY_ERR_UNSUPPORTED;
-    if ((head_dim != 64 && head_dim != 128) || page_size % 16 || n_kv_heads < 1 || n_heads % n_kv_heads) return SANDY_ERR_UNSUPPORTED;
-    if (page_stride % 16 || (((uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)out) & 15) || ld_q % 8 || ld_out % 8 ||
-        n_seqs > 65535 || n_kv_heads > 65535 || (long long)max_q_len * (n_heads / n_kv_heads) > (1 << 28))
+    if ((c.head_dim != 64 && c.head_dim != 128) || c.page_size % 16 || c.n_kv_heads < 1 || r->n_heads % c.n_kv_heads) return SANDY_ERR_UNSUPPORTED;
+    if (c.page_stride % 16 || (((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)r->q | (uintptr_t)r->out) & 15) || r->ld_q % 8 || r->ld_out % 8 ||
+        r->n_z > 65535 || c.n_kv_heads > 65535 || (long long)r->max_n * (r->n_heads / c.n_kv_heads) > (1 << 28))
         return SANDY_ERR_UNSUPPORTED;
-    const Args a = {(const bf16*)q, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, block_table, q_start, kv_before, (bf16*)out, status,
-                    rules->sink, rules->out_gate, (const bf16*)rules->elem_gate, ld_q, ld_out, page_stride, scale_stride, max_blocks, n_rows,
-                    n_heads, n_kv_heads, n_heads / n_kv_heads, page_size, (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1,
-                    num_pages, rules->window, rules->keep_first, rules->chunk, rules->ld_elem_gate, rules->gate_dim, scale, rules->softcap};
-    if (code == SANDY_E4M3 && head_dim == 64) return launch<SANDY_E4M3, 64>(a, n_seqs, max_q_len, stream);
-    if (code == SANDY_E4M3 && head_dim == 128) return launch<SANDY_E4M3, 128>(a, n_seqs, max_q_len, stream);
-    if (code == SANDY_INT8 && head_dim == 64) return launch<SANDY_INT8, 64>(a, n_seqs, max_q_len, stream);
-    if (code == SANDY_INT8 && head_dim == 128) return launch<SANDY_INT8, 128>(a, n_seqs, max_q_len, stream);
+    Args a = {};
+    a.q = (const bf16*)r->q;
+    a.k = (const uint8_t*)c.k;
+    a.v = (const uint8_t*)c.v;
+    a.k_scale = c.k_scale;
+    a.v_scale = c.v_scale;
+    a.block_table = c.block_table;
+    a.q_start = r->q_start;
+    a.kv_before = r->positions;
+    a.out = (bf16*)r->out;
+    a.status = c.status;
+    a.sink = rules.sink;
+    a.out_gate = rules.out_gate;
+    a.elem_gate = (const bf16*)rules.elem_gate;
+    a.ld_q = r->ld_q;
+    a.ld_out = r->ld_out;
+    a.page_stride = c.page_stride;
+    a.scale_stride = c.scale_stride;
+    a.max_blocks = c.max_blocks;
+    a.n_rows = r->n_rows;
+    a.n_heads = r->n_heads;
+    a.n_kv_heads = c.n_kv_heads;
+    a.group = r->n_heads / c.n_kv_heads;
+    a.page_size = c.page_size;
+    a.page_shift = (c.page_size & (c.page_size - 1)) == 0 ? __builtin_ctz(c.page_size) : -1;
+    a.num_pages = c.num_pages;
+    a.window = rules.window;
+    a.keep_first = rules.keep_first;
+    a.chunk = rules.chunk;
+    a.ld_elem_gate = rules.ld_elem_gate;
+    a.gate_dim = rules.gate_dim;
+    a.scale = r->scale;
+    a.softcap = rules.softcap;
+    if (c.code == SANDY_E4M3 && c.head_dim == 64) return launch<SANDY_E4M3, 64>(a, r->n_z, r->max_n, stream);
+    if (c.code == SANDY_E4M3 && c.head_dim == 128) return launch<SANDY_E4M3, 128>(a, r->n_z, r->max_n, stream);
+    if (c.code == SANDY_INT8 && c.head_dim == 64) return launch<SANDY_INT8, 64>(a, r->n_z, r->max_n, stream);
+    if (c.code == SANDY_INT8 && c.head_dim == 128) return launch<SANDY_INT8, 128>(a, r->n_z, r->max_n, stream);
     return SANDY_ERR_UNSUPPORTED;
 }

@@ -12,7 +12,10 @@
 // What bounds it.  2 (keys, values) x 2 bytes in and 1 byte out a value: a copy's work.  One warp owns one block and holds the
 // block's new values in registers between the maximum and the rounding (up to 1,024 values; larger blocks are read twice,
 // the second time from the caches), so each value crosses the memory bus once.
+#include "cache8.h"
 #include "kv_8bit.cuh"
+
+static_assert(sizeof(SandyCache8) == 96 && sizeof(SandyRows8) == 152, "the layout callers lay down");
 
 namespace {
 
@@ -219,72 +222,63 @@ read_kernel(Planes cache, const int* __restrict__ block_table, int max_blocks, c
     }
 }
 
-bool bad_cache(const void* k, const void* v, const float* ks, const float* vs, long long page_stride, int n_kv_heads, int head_dim,
-               int page_size) {
-    return !k || !v || !ks || !vs || n_kv_heads < 1 || head_dim < 16 || page_size < 1 || page_stride < 1;
+// Sizes both entries refuse.
+int refused(const SandyRows8* r) {
+    const SandyCache8& c = r->cache;
+    if (!r->k_rows || !r->v_rows || !r->start || !r->first || !c.k || !c.v || !c.k_scale || !c.v_scale || !c.block_table || c.n_seqs < 0 ||
+        r->max_len < 0 || c.n_kv_heads < 1 || c.head_dim < 16 || c.page_size < 1 || c.page_stride < 1)
+        return SANDY_ERR_ARGUMENT;
+    if (c.head_dim % 16 || c.page_stride % 16 || (((uintptr_t)c.k | (uintptr_t)c.v) & 15) || c.n_seqs > 65535) return SANDY_ERR_UNSUPPORTED;
+    return SANDY_OK;
+}
+
+template <typename T>
+bool on_16_bytes(const SandyRows8& r) {
+    return (((uintptr_t)r.k_rows | (uintptr_t)r.v_rows | (size_t)(r.ld_k * (long long)sizeof(T)) | (size_t)(r.ld_v * (long long)sizeof(T))) & 15) == 0;
 }
 
 }  // namespace
 
-// k_src, v_src: [n_rows, Hkv * D] of dtype with row pitches ld_k, ld_v (elements).  Request s brings rows q_start[s] .. q_start[s + 1] - 1,
-// which go to positions kv_before[s] on; max_q_len: the most that one brings.  k, v: codes [num_pages][Hkv][page_size][D], page pitch
-// page_stride (bytes); k_scale, v_scale: [num_pages][Hkv], row pitch scale_stride.  Pages that two requests of one call both
-// write are not allowed.  Bit 3 of *status: a position without a page, or rows past n_rows.
-SANDY_API int sandy_kv_append_8bit(const void* k_src, const void* v_src, long long ld_k, long long ld_v, void* k, void* v,
-                                   float* k_scale, float* v_scale, long long page_stride, long long scale_stride,
-                                   const int* block_table, int max_blocks, const int* q_start, const int* kv_before, int n_seqs,
-                                   int n_rows, int max_q_len, int n_kv_heads, int head_dim, int page_size, int num_pages, int dtype, int code,
-                                   int* status, cudaStream_t stream) {
-    if (n_seqs == 0 || max_q_len == 0) return SANDY_OK;
-    if (!k_src || !v_src || !block_table || !q_start || !kv_before || n_seqs < 0 || max_q_len < 0 ||
-        bad_cache(k, v, k_scale, v_scale, page_stride, n_kv_heads, head_dim, page_size))
-        return SANDY_ERR_ARGUMENT;
-    if (head_dim % 16 || page_stride % 16 || (((uintptr_t)k | (uintptr_t)v) & 15) || n_seqs > 65535) return SANDY_ERR_UNSUPPORTED;
-    const int groups = (2 * n_kv_heads + WARPS - 1) / WARPS;
-    const long long touched = ((long long)max_q_len + page_size - 2) / page_size + 1;      // by one request, wherever it starts
+// Quantises rows (cache8.h) into their pages.  Pages that two requests of one call both write are not allowed.  Bit 3 of *status: a
+// position without a page, or rows past n_rows.
+SANDY_API int sandy_kv_append_8bit(const SandyRows8* r, cudaStream_t stream) {
+    if (!r) return SANDY_ERR_ARGUMENT;
+    const SandyCache8& c = r->cache;
+    if (c.n_seqs == 0 || r->max_len == 0) return SANDY_OK;
+    if (const int code = refused(r)) return code;
+    const int groups = (2 * c.n_kv_heads + WARPS - 1) / WARPS;
+    const long long touched = ((long long)r->max_len + c.page_size - 2) / c.page_size + 1;      // by one request, wherever it starts
     if (touched * groups > 0x7fffffffll) return SANDY_ERR_UNSUPPORTED;
-    const Planes cache = {(uint8_t*)k, (uint8_t*)v, k_scale, v_scale, page_stride, scale_stride};
-    const dim3 grid((unsigned)(touched * groups), n_seqs), block(WARPS * 32);
+    const Planes cache = {(uint8_t*)c.k, (uint8_t*)c.v, c.k_scale, c.v_scale, c.page_stride, c.scale_stride};
+    const dim3 grid((unsigned)(touched * groups), c.n_seqs), block(WARPS * 32);
 #define APPEND(T, CODE)                                                                                                         \
-    do {                                                                                                                        \
-        const size_t any = (uintptr_t)k_src | (uintptr_t)v_src | (size_t)(ld_k * (long long)sizeof(T)) | (size_t)(ld_v * (long long)sizeof(T)); \
-        return sandy_launch(any % 16 == 0 ? append_kernel<T, CODE, true> : append_kernel<T, CODE, false>, grid, block, 0, stream, \
-                            (const T*)k_src, (const T*)v_src, ld_k, ld_v, cache, block_table, max_blocks, q_start, kv_before,   \
-                            n_rows, n_kv_heads, head_dim, page_size, num_pages, groups, status);                                        \
-    } while (0)
-    if (dtype == SANDY_F32 && code == SANDY_E4M3) APPEND(float, SANDY_E4M3);
-    if (dtype == SANDY_F32 && code == SANDY_INT8) APPEND(float, SANDY_INT8);
-    if (dtype == SANDY_BF16 && code == SANDY_E4M3) APPEND(bf16, SANDY_E4M3);
-    if (dtype == SANDY_BF16 && code == SANDY_INT8) APPEND(bf16, SANDY_INT8);
+    return sandy_launch(on_16_bytes<T>(*r) ? append_kernel<T, CODE, true> : append_kernel<T, CODE, false>, grid, block, 0, stream, \
+                        (const T*)r->k_rows, (const T*)r->v_rows, r->ld_k, r->ld_v, cache, c.block_table, c.max_blocks, r->start, \
+                        r->first, r->n_rows, c.n_kv_heads, c.head_dim, c.page_size, c.num_pages, groups, c.status)
+    if (c.dtype == SANDY_F32 && c.code == SANDY_E4M3) APPEND(float, SANDY_E4M3);
+    if (c.dtype == SANDY_F32 && c.code == SANDY_INT8) APPEND(float, SANDY_INT8);
+    if (c.dtype == SANDY_BF16 && c.code == SANDY_E4M3) APPEND(bf16, SANDY_E4M3);
+    if (c.dtype == SANDY_BF16 && c.code == SANDY_INT8) APPEND(bf16, SANDY_INT8);
 #undef APPEND
     return SANDY_ERR_UNSUPPORTED;
 }
 
-// Rows out_start[s] .. out_start[s + 1] - 1 of k_out and v_out ([n_rows, Hkv * D] of dtype, row pitches ld_k, ld_v) become the cached
-// positions first[s] on of request s; max_len: the most rows of one request.  Bit 4 of *status: a position without a page, or rows past
-// n_rows.
-SANDY_API int sandy_kv_read_8bit(const void* k, const void* v, const float* k_scale, const float* v_scale, long long page_stride,
-                                 long long scale_stride, const int* block_table, int max_blocks, const int* first,
-                                 const int* out_start, void* k_out, void* v_out, long long ld_k, long long ld_v, int n_seqs,
-                                 int n_rows, int max_len, int n_kv_heads, int head_dim, int page_size, int num_pages, int dtype, int code,
-                                 int* status, cudaStream_t stream) {
-    if (n_seqs == 0 || max_len == 0) return SANDY_OK;
-    if (!k_out || !v_out || !block_table || !first || !out_start || n_seqs < 0 || max_len < 0 ||
-        bad_cache(k, v, k_scale, v_scale, page_stride, n_kv_heads, head_dim, page_size))
-        return SANDY_ERR_ARGUMENT;
-    if (head_dim % 16 || page_stride % 16 || (((uintptr_t)k | (uintptr_t)v) & 15) || n_seqs > 65535) return SANDY_ERR_UNSUPPORTED;
-    const Planes cache = {(uint8_t*)k, (uint8_t*)v, (float*)k_scale, (float*)v_scale, page_stride, scale_stride};
-    const dim3 grid((max_len - 1) / READ_ROWS + 1, n_seqs), block(READ_THREADS);
+// The rows become the cached numbers.  Bit 4 of *status: a position without a page, or rows past n_rows.
+SANDY_API int sandy_kv_read_8bit(const SandyRows8* r, cudaStream_t stream) {
+    if (!r) return SANDY_ERR_ARGUMENT;
+    const SandyCache8& c = r->cache;
+    if (c.n_seqs == 0 || r->max_len == 0) return SANDY_OK;
+    if (const int code = refused(r)) return code;
+    const Planes cache = {(uint8_t*)c.k, (uint8_t*)c.v, c.k_scale, c.v_scale, c.page_stride, c.scale_stride};
+    const dim3 grid((r->max_len - 1) / READ_ROWS + 1, c.n_seqs), block(READ_THREADS);
 #define READ(T, CODE)                                                                                                           \
-    do {                                                                                                                        \
-        const size_t any = (uintptr_t)k_out | (uintptr_t)v_out | (size_t)(ld_k * (long long)sizeof(T)) | (size_t)(ld_v * (long long)sizeof(T)); \
-        return sandy_launch(read_kernel<T, CODE>, grid, block, 0, stream, cache, block_table, max_blocks, first, out_start,     \
-                            (T*)k_out, (T*)v_out, ld_k, ld_v, n_rows, n_kv_heads, head_dim, page_size, num_pages, any % 16 == 0, status); \
-    } while (0)
-    if (dtype == SANDY_F32 && code == SANDY_E4M3) READ(float, SANDY_E4M3);
-    if (dtype == SANDY_F32 && code == SANDY_INT8) READ(float, SANDY_INT8);
-    if (dtype == SANDY_BF16 && code == SANDY_E4M3) READ(bf16, SANDY_E4M3);
-    if (dtype == SANDY_BF16 && code == SANDY_INT8) READ(bf16, SANDY_INT8);
+    return sandy_launch(read_kernel<T, CODE>, grid, block, 0, stream, cache, c.block_table, c.max_blocks, r->first, r->start,    \
+                        (T*)r->k_rows, (T*)r->v_rows, r->ld_k, r->ld_v, r->n_rows, c.n_kv_heads, c.head_dim, c.page_size,        \
+                        c.num_pages, on_16_bytes<T>(*r), c.status)
+    if (c.dtype == SANDY_F32 && c.code == SANDY_E4M3) READ(float, SANDY_E4M3);
+    if (c.dtype == SANDY_F32 && c.code == SANDY_INT8) READ(float, SANDY_INT8);
+    if (c.dtype == SANDY_BF16 && c.code == SANDY_E4M3) READ(bf16, SANDY_E4M3);
+    if (c.dtype == SANDY_BF16 && c.code == SANDY_INT8) READ(bf16, SANDY_INT8);
 #undef READ
     return SANDY_ERR_UNSUPPORTED;
 }

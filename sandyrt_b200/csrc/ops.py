@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 import dataclasses
 import functools
+import struct
 from typing import Optional
 
 import torch
@@ -499,53 +500,74 @@ def prefill_attention_f32(q, k_cache, v_cache, block_table, q_start, kv_before, 
         _check(code, f"decode_attention_single(H={n_heads},Hkv={hkv},D={d},splits={single_splits})")
 
 
-# ---- a cache in 8 bits (kv_8bit.cu, attention_8bit.cu) -----------------------------------------------------------------
+# ---- a cache in 8 bits (kv_8bit.cu, attention_8bit.cu, attention_8bit_tc.cu) -------------------------------------------
+# A call is one structure of cache8.h, packed in one go, and what its checks make of the tensors' types, shapes and strides is kept for
+# the next call of the same ones: a step of a few requests takes less time on the device (2 us) than a call with an argument
+# object each and every check anew (20 us).
 CODE_CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
 _V, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+_CACHE8 = "PPPPqqPP8i"                              # SandyCache8
+_ROWS8 = struct.Struct("@" + _CACHE8 + "PPqqPPii")  # SandyRows8
+_ATTEND8 = struct.Struct("@" + _CACHE8 + "PPqqPPPP" + "iifiPPPiPii" + "6ifi")       # SandyAttend8
+assert (_ROWS8.size, _ATTEND8.size) == (152, 256)
 
 
 @functools.lru_cache(maxsize=None)
-def _entry(library: str, name: str, argtypes: tuple, restype=ctypes.c_int):
-    """A typed entry point: it takes Python numbers and addresses as they are, without an object for each."""
+def _entry(library: str, name: str, *argtypes):
+    """A typed entry point: it takes Python numbers, bytes and addresses as they are, without an object for each."""
     f = getattr(load_library(library), name)
-    f.argtypes, f.restype = argtypes, restype
+    f.argtypes, f.restype = argtypes, ctypes.c_int
     return f
 
 
-def _at(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def _device_of(what: str, *tensors) -> torch.device:
-    """The one CUDA device all tensors are on."""
-    device = tensors[0].device
+def _layout(t: Optional[torch.Tensor]):
+    return None if t is None else (t.dtype, t.shape, t.stride())
+
+
+def _one_device(what: str, *tensors) -> int:
+    """The index of the one CUDA device all tensors are on."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != device:
-            raise KernelError(f"{what}: tensors on {device} and {t.device}")
-    if device.type != "cuda":
+        if t is not None and t.get_device() != index:
+            raise KernelError(f"{what}: tensors on {tensors[0].device} and {t.device}")
+    if index < 0:
         raise KernelError("kernel arguments must be CUDA tensors (there is no CPU path)")
-    return device
+    return index
 
 
-def _status_word(device: torch.device) -> int:
+def _status_word(index: int) -> int:
     """The address of the device's status word.  It is made by the first call on the device, which must not be a recorded one: a
     graph's memory would hold it."""
-    t = _kernel_status.get(device.index)
+    t = _kernel_status.get(index)
     if t is None:
         if torch.cuda.is_current_stream_capturing():
             raise KernelError("the device's status word is made by its first kernel call; call once before capturing a graph")
-        t = kernel_status(device)
+        t = kernel_status(torch.device("cuda", index))
     return t.data_ptr()
 
 
-def _run_on(device: torch.device, entry, args: tuple, what: str) -> None:
+def _run_on(index: int, entry, args: tuple, what: str) -> None:
     """One typed call on the device's current stream, whichever device is the current one."""
-    if device.index == torch.cuda.current_device():
-        code = entry(*args, torch.cuda.current_stream().cuda_stream)
+    if index == torch._C._cuda_getDevice():
+        code = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            code = entry(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            code = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     _check(code, what)
+
+
+def _dense(shape, stride) -> bool:
+    """Whether a tensor of this shape and these strides is contiguous."""
+    want = 1
+    for n, st in zip(reversed(shape), reversed(stride)):
+        if n != 1 and st != want:
+            return 0 in shape
+        want *= n
+    return True
 
 
 @dataclasses.dataclass
@@ -565,56 +587,73 @@ class Cache8:
         scales = lambda: torch.empty(num_pages, n_kv_heads, dtype=torch.float32, device=device)
         return cls(codes(), codes(), scales(), scales())
 
-    def check(self, what: str):
-        """(Hkv, page_size, D, page pitch, scale pitch, num_pages, code) or KernelError."""
-        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
-        if k.dtype not in CODE_CODES or v.dtype != k.dtype:
-            raise UnsupportedShape(f"{what}: codes are float8_e4m3fn or int8, got {k.dtype} and {v.dtype}")
-        if k.dim() != 4 or k.shape != v.shape:
-            raise KernelError(f"{what}: codes must be [num_pages, Hkv, page_size, D], keys and values alike")
-        n, hkv, ps, d = k.shape
-        stride = k.stride()
-        if stride != v.stride() or stride[1:] != (ps * d, d, 1):
-            raise KernelError(f"{what}: codes must be dense inside a page, keys and values with one page stride")
-        if d % 16 or not 16 <= d <= 256 or stride[0] % 16 or k.data_ptr() % 16 or v.data_ptr() % 16:
-            raise UnsupportedShape(f"{what}: head sizes 16..256 in steps of 16, pages on 16-byte boundaries")
-        for s in (ks, vs):
-            if s.dtype != torch.float32 or s.shape != (n, hkv) or s.stride(1) != 1 or s.stride(0) != ks.stride(0):
-                raise KernelError(f"{what}: scales must be float32 [num_pages, Hkv]")
-        if n > 1 and (stride[0] < hkv * ps * d or ks.stride(0) < hkv):
-            raise KernelError(f"{what}: pages overlap")
-        return hkv, ps, d, stride[0], ks.stride(0), n, CODE_CODES[k.dtype]
+
+@functools.lru_cache(maxsize=256)
+def _cache8_layout(what: str, k, v, ks, vs):
+    """(page pitch, scale pitch), Hkv, D, page size, num_pages, code of a cache with these layouts, or an error."""
+    (dtype, shape, stride), code = k, CODE_CODES.get(k[0])
+    if code is None or v[0] != dtype:
+        raise UnsupportedShape(f"{what}: codes are float8_e4m3fn or int8, got {dtype} and {v[0]}")
+    if len(shape) != 4 or shape != v[1]:
+        raise KernelError(f"{what}: codes must be [num_pages, Hkv, page_size, D], keys and values alike")
+    n, hkv, ps, d = shape
+    if stride != v[2] or stride[1:] != (ps * d, d, 1):
+        raise KernelError(f"{what}: codes must be dense inside a page, keys and values with one page stride")
+    if d % 16 or not 16 <= d <= 256 or stride[0] % 16:
+        raise UnsupportedShape(f"{what}: head sizes 16..256 in steps of 16, pages on 16-byte boundaries")
+    for s in (ks, vs):
+        if s[0] != torch.float32 or s[1] != (n, hkv) or (s[2][1] != 1 and hkv > 1) or s[2][0] != ks[2][0]:
+            raise KernelError(f"{what}: scales must be float32 [num_pages, Hkv], keys' and values' with one stride")
+    if n > 1 and (stride[0] < hkv * ps * d or ks[2][0] < hkv):
+        raise KernelError(f"{what}: pages overlap")
+    return (stride[0], ks[2][0]), hkv, d, ps, n, code
 
 
-def _indices(what: str, **arrays) -> None:
-    for name, t in arrays.items():
-        if t.dtype != torch.int32 or not t.is_contiguous():
+def _cache8(what: str, cache: Cache8):
+    k, v, ks, vs = cache.k, cache.v, cache.k_scale, cache.v_scale
+    layout = _cache8_layout(what, _layout(k), _layout(v), _layout(ks), _layout(vs))
+    at = (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr())
+    if (at[0] | at[1]) % 16:
+        raise UnsupportedShape(f"{what}: head sizes 16..256 in steps of 16, pages on 16-byte boundaries")
+    return at, layout
+
+
+@functools.lru_cache(maxsize=256)
+def _requests8(what: str, table, starts, firsts) -> tuple:
+    """(requests, entries a request) of a block table, row starts [S + 1] and first positions [S]."""
+    for name, (dtype, shape, stride) in (("block_table", table), ("the row starts", starts), ("the first positions", firsts)):
+        if dtype != torch.int32 or not _dense(shape, stride):
             raise KernelError(f"{what}: {name} must be a contiguous int32 tensor")
-
-
-def _portions(what: str, table, starts, befores) -> int:
-    """The number of requests of block table, row starts [S + 1] and first positions [S]."""
-    _indices(what, block_table=table, starts=starts, positions=befores)
-    S = befores.numel()
-    if table.dim() != 2 or table.shape[0] != S or starts.numel() != S + 1:
+    if len(firsts[1]) != 1 or len(starts[1]) != 1 or len(table[1]) != 2 or table[1][0] != firsts[1][0] or starts[1][0] != firsts[1][0] + 1:
         raise KernelError(f"{what}: the block table, the row starts and the first positions disagree on the requests")
-    if S > 65535:
+    if firsts[1][0] > 65535:
         raise UnsupportedShape(f"{what}: at most 65535 requests")
-    return S
+    return tuple(table[1])
 
 
-def _rows_of(what: str, hkv: int, d: int, *tensors) -> None:
-    first = tensors[0]
-    for t in tensors:
-        if t.dim() != 2 or t.shape != (first.shape[0], hkv * d) or t.dtype != first.dtype or (t.stride(1) != 1 and t.numel()):
+@functools.lru_cache(maxsize=4096)
+def _rows8(what: str, hkv: int, d: int, a, b) -> tuple:
+    """(row pitches), rows, type code of two tensors of rows."""
+    for dtype, shape, stride in (a, b):
+        if len(shape) != 2 or shape != (a[1][0], hkv * d) or dtype != a[0] or (stride[1] != 1 and shape[0]):
             raise KernelError(f"{what}: rows must be [T, Hkv * D] = [T, {hkv * d}] of one type, with an innermost stride of 1")
+    if a[0] not in (torch.float32, torch.bfloat16):
+        raise UnsupportedShape(f"{what}: kernels take float32 or bfloat16 tensors, got {a[0]}")
+    return (a[2][0], b[2][0]), a[1][0], F32 if a[0] == torch.float32 else BF16
 
 
-_APPEND8 = (_V, _V, _L, _L, _V, _V, _V, _V, _L, _L, _V, _I, _V, _V, _I, _I, _I, _I, _I, _I, _I, _I, _I, _V, _V)
-_READ8 = (_V, _V, _V, _V, _L, _L, _V, _I, _V, _V, _V, _V, _L, _L, _I, _I, _I, _I, _I, _I, _I, _I, _I, _V, _V)
-_ATTEND8 = (_V, _L, _V, _V, _V, _V, _L, _L, _V, _I, _I, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _I, _I, _I, _F, _V, _I, _I, _V, _I, _I, _V, _V)
-
-_PREFILL8_TC = (_V, _L, _V, _V, _V, _V, _L, _L, _V, _I, _V, _V, _V, _L, _I, _I, _I, _I, _I, _I, _I, _I, _F, _V, _I, _V, _V)
+def _rows_call8(what: str, name: str, cache: Cache8, k_rows, v_rows, block_table, starts, firsts, max_len: int, longest: str) -> None:
+    at, (pitch, hkv, d, ps, pages, code) = _cache8(what, cache)
+    ld, n_rows, dtype = _rows8(what, hkv, d, _layout(k_rows), _layout(v_rows))
+    S, width = _requests8(what, _layout(block_table), _layout(starts), _layout(firsts))
+    if max_len < 0:
+        raise KernelError(f"{what}: {longest} is negative")
+    index = _one_device(what, k_rows, v_rows, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, starts, firsts)
+    if S == 0 or max_len == 0 or n_rows == 0:
+        return
+    call = _ROWS8.pack(*at, *pitch, block_table.data_ptr(), _status_word(index), width, S, hkv, d, ps, pages, code, dtype,
+                       k_rows.data_ptr(), v_rows.data_ptr(), *ld, starts.data_ptr(), firsts.data_ptr(), n_rows, max_len)
+    _run_on(index, _entry("kv_8bit", name, ctypes.c_char_p, _V), (call,), what)
 
 
 def kv_append_8bit(k_src, v_src, cache: Cache8, block_table, q_start, kv_before, *, max_q_len: int) -> None:
@@ -624,50 +663,27 @@ def kv_append_8bit(k_src, v_src, cache: Cache8, block_table, q_start, kv_before,
     which its largest value fits the code; a block that held earlier positions keeps its scale or, where the new values need a
     larger one, has its earlier codes rounded again.  A block that is given a value that is not finite gets a scale of NaN.
     Requests must not share a page that they write.  Rows in front of the first request and behind the last one are not read."""
-    hkv, ps, d, page_stride, scale_stride, pages, code = cache.check("kv_append_8bit")
-    _rows_of("kv_append_8bit", hkv, d, k_src, v_src)
-    dtype, S = _dt(k_src), _portions("kv_append_8bit", block_table, q_start, kv_before)
-    if max_q_len < 0:
-        raise KernelError("kv_append_8bit: max_q_len is negative")
-    device = _device_of("kv_append_8bit", k_src, v_src, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, q_start, kv_before)
-    if S == 0 or max_q_len == 0 or k_src.shape[0] == 0:
-        return
-    _run_on(device, _entry("kv_8bit", "sandy_kv_append_8bit", _APPEND8),
-            (k_src.data_ptr(), v_src.data_ptr(), k_src.stride(0), v_src.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
-             cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), page_stride, scale_stride, block_table.data_ptr(), block_table.shape[1],
-             q_start.data_ptr(), kv_before.data_ptr(), S, k_src.shape[0], max_q_len, hkv, d, ps, pages, dtype, code, _status_word(device)),
-            "kv_append_8bit")
+    _rows_call8("kv_append_8bit", "sandy_kv_append_8bit", cache, k_src, v_src, block_table, q_start, kv_before, max_q_len, "max_q_len")
 
 
 def kv_read_8bit(cache: Cache8, block_table, first, out_start, k_out, v_out, *, max_len: int) -> None:
     """Cached rows back as numbers: rows out_start[s] .. out_start[s + 1] - 1 (int32 [S + 1]) of k_out and v_out ([N, Hkv * D], float32
     or bfloat16, a row pitch each) become positions first[s] on (int32 [S]) of the block table's request s; max_len: the
     most rows of one request.  Exact in both types.  Rows of no request, and of positions without a page, are left as they were."""
-    hkv, ps, d, page_stride, scale_stride, pages, code = cache.check("kv_read_8bit")
-    _rows_of("kv_read_8bit", hkv, d, k_out, v_out)
-    dtype, S = _dt(k_out), _portions("kv_read_8bit", block_table, out_start, first)
-    if max_len < 0:
-        raise KernelError("kv_read_8bit: max_len is negative")
-    device = _device_of("kv_read_8bit", k_out, v_out, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, out_start, first)
-    if S == 0 or max_len == 0 or k_out.shape[0] == 0:
-        return
-    _run_on(device, _entry("kv_8bit", "sandy_kv_read_8bit", _READ8),
-            (cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), page_stride, scale_stride,
-             block_table.data_ptr(), block_table.shape[1], first.data_ptr(), out_start.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
-             k_out.stride(0), v_out.stride(0), S, k_out.shape[0], max_len, hkv, d, ps, pages, dtype, code, _status_word(device)), "kv_read_8bit")
+    _rows_call8("kv_read_8bit", "sandy_kv_read_8bit", cache, k_out, v_out, block_table, out_start, first, max_len, "max_len")
 
 
-def _attention_8bit(what, q, cache, block_table, token_seq, positions, q_start, out, n_z, max_n, n_heads, scale, num_splits, rules, tc=False) -> None:
-    hkv, ps, d, page_stride, scale_stride, pages, code = cache.check(what)
-    if n_heads < 1 or n_heads % hkv:
-        raise UnsupportedShape(f"{what}: {n_heads} heads do not divide into {hkv} key/value heads")
-    if q.dim() != 2 or q.shape[1] != n_heads * d or out.shape != q.shape or out.dtype != q.dtype or \
-            (q.numel() and (q.stride(1) != 1 or out.stride(1) != 1)):
-        raise KernelError(f"{what}: q and out must be [T, H * D] = [T, {n_heads * d}] of one type, with an innermost stride of 1")
-    dtype, T = _dt(q), q.shape[0]
-    window, keep_first, softcap, chunk, sink, out_gate, dist_bias, elem_gate = (
-        rules.get(n, z) for n, z in (("window", 0), ("keep_first", 0), ("softcap", 0.0), ("chunk", 0), ("sink", None), ("out_gate", None),
-                                     ("dist_bias", None), ("elem_gate", None)))
+_RULES8 = {"window": 0, "keep_first": 0, "softcap": 0.0, "chunk": 0, "sink": None, "out_gate": None, "dist_bias": None, "elem_gate": None}
+_NO_RULES8 = (0, 0, 0.0, 0, 0, 0, 0, 0, 0, 0, 0)
+
+
+def _rules8(what: str, q, n_heads: int, rules: dict) -> tuple:
+    """The rules as SandyAttentionRules lays them out, and their tensors."""
+    for name in rules:
+        if name not in _RULES8:
+            raise TypeError(f"{what}() got an unexpected keyword argument {name!r}")
+    window, keep_first, softcap, chunk, sink, out_gate, dist_bias, elem_gate = (rules.get(n, z) for n, z in _RULES8.items())
+    T = q.shape[0]
     if min(window, keep_first, chunk) < 0 or not softcap >= 0 or (keep_first and chunk):
         raise UnsupportedShape(f"{what}: window, keep_first, softcap and chunk must not be negative, kept first keys and chunks not together")
     if sink is not None and (sink.dtype != torch.float32 or sink.shape != (n_heads,) or not sink.is_contiguous()):
@@ -680,40 +696,76 @@ def _attention_8bit(what, q, cache, block_table, token_seq, positions, q_start, 
     if elem_gate is not None and (elem_gate.dtype != q.dtype or elem_gate.dim() != 2 or elem_gate.shape[0] != T or elem_gate.shape[1] < n_heads
                                   or elem_gate.shape[1] % n_heads or elem_gate.shape[1] > q.shape[1] or (T and elem_gate.stride(1) != 1)):
         raise KernelError(f"{what}: a gate by element is [T, H * dim] of the queries' type, dim at most the head size")
+    laid = (window, keep_first, softcap, chunk, _at(sink), _at(out_gate), _at(dist_bias), 0 if dist_bias is None else dist_bias.shape[1],
+            _at(elem_gate), 0 if elem_gate is None else elem_gate.stride(0), 0 if elem_gate is None else elem_gate.shape[1] // n_heads)
+    return laid, (sink, out_gate, dist_bias, elem_gate)
+
+
+@functools.lru_cache(maxsize=4096)
+def _queries8(what: str, n_heads: int, hkv: int, d: int, q, out) -> tuple:
+    """(row pitches), rows, type code of queries and results."""
+    if n_heads < 1 or n_heads % hkv:
+        raise UnsupportedShape(f"{what}: {n_heads} heads do not divide into {hkv} key/value heads")
+    if len(q[1]) != 2 or q[1][1] != n_heads * d or out[1] != q[1] or out[0] != q[0] or (q[1][0] and (q[2][1] != 1 or out[2][1] != 1)):
+        raise KernelError(f"{what}: q and out must be [T, H * D] = [T, {n_heads * d}] of one type, with an innermost stride of 1")
+    if q[0] not in (torch.float32, torch.bfloat16):
+        raise UnsupportedShape(f"{what}: kernels take float32 or bfloat16 tensors, got {q[0]}")
+    return (q[2][0], out[2][0]), q[1][0], F32 if q[0] == torch.float32 else BF16
+
+
+@functools.lru_cache(maxsize=4096)
+def _splits8(*sizes) -> tuple:
+    """(splits, floats of scratch) by the library's rule (sandy_attention_8bit_splits)."""
+    floats = ctypes.c_longlong(0)
+    splits = _entry("attention_8bit", "sandy_attention_8bit_splits", *(_I,) * 9, _V)(*sizes, ctypes.addressof(floats))
+    return splits, floats.value
+
+
+# From so many rows (tokens x heads of a group) of the longest portion on, 8-bit prompt attention goes to the tcgen05 kernel.
+TC_ROWS_8BIT = 64
+
+
+def _attention_8bit(what, q, cache, block_table, width, token_seq, positions, q_start, out, n_z, max_n, n_heads, scale, num_splits, tc, rules) -> None:
+    at, (pitch, hkv, d, ps, pages, code) = _cache8(what, cache)
+    ld, T, dtype = _queries8(what, n_heads, hkv, d, _layout(q), _layout(out))
+    laid, extra = _rules8(what, q, n_heads, rules) if rules else (_NO_RULES8, ())
     if num_splits < 0 or num_splits > 256:
         raise KernelError(f"{what}: num_splits must lie in 0 .. 256 (0: the kernel's choice)")
-    device = _device_of(what, q, out, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, token_seq, positions, q_start, sink,
-                        out_gate, dist_bias, elem_gate)
+    index = _one_device(what, q, out, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, token_seq, positions, q_start, *extra)
     if n_z == 0 or max_n == 0 or T == 0:
         return
-    if block_table.shape[0] == 0 or block_table.shape[1] == 0 or pages == 0:
+    if block_table.shape[0] == 0 or width == 0 or pages == 0:
         raise KernelError(f"{what}: an empty block table or cache")
-    max_keys = min(block_table.shape[1] * ps, window + keep_first + max_n if window else 1 << 30)
-    args = _AttentionRules(window, keep_first, softcap, chunk, _at(sink), _at(out_gate), _at(dist_bias),
-                           0 if dist_bias is None else dist_bias.shape[1], _at(elem_gate), 0 if elem_gate is None else elem_gate.stride(0),
-                           0 if elem_gate is None else elem_gate.shape[1] // n_heads)
-    at = ctypes.addressof(args)
-    if tc:
-        if dtype != BF16:
-            raise UnsupportedShape(f"{what}: the tcgen05 kernel takes bfloat16")
-        _run_on(device, _entry("attention_8bit_tc", "sandy_prefill_attention_8bit_tc", _PREFILL8_TC),
-                (q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), page_stride,
-                 scale_stride, block_table.data_ptr(), block_table.shape[1], positions.data_ptr(), q_start.data_ptr(), out.data_ptr(), out.stride(0),
-                 T, n_z, max_n, n_heads, hkv, d, ps, pages, scale, at, code, _status_word(device)), f"{what}(tc,H={n_heads},Hkv={hkv},D={d},page={ps})")
-        return
+    q_at, out_at, window = q.data_ptr(), out.data_ptr(), laid[0]
+    if q_start is None:
+        tc = False
+    elif tc is None:
+        tc = not num_splits and max_n * n_heads >= TC_ROWS_8BIT * hkv and dtype == BF16 and d in (64, 128) and ps % 16 == 0 and scale > 0 \
+            and not laid[6] and not (q_at | out_at) % 16 and not (ld[0] | ld[1]) % 8
+    max_keys = min(width * ps, window + laid[1] + max_n if window else 1 << 30)
+    splits, floats = (1, 0) if tc else _splits8(T, n_z, max_n, n_heads, hkv, d, max_keys, dtype, num_splits)
     # partial results of many splits: memory of the stream the call is on, given back to the allocator when it returns
-    floats = ctypes.c_longlong(0)
-    splits = _entry("attention_8bit", "sandy_attention_8bit_splits", (_I,) * 9 + (_V,))(T, n_z, max_n, n_heads, hkv, d, max_keys, dtype, num_splits,
-                                                                                        ctypes.addressof(floats))
-    scratch = torch.empty(floats.value, dtype=torch.float32, device=device) if floats.value else None
-    _run_on(device, _entry("attention_8bit", "sandy_attention_8bit", _ATTEND8),
-            (q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), page_stride,
-             scale_stride, block_table.data_ptr(), block_table.shape[1], block_table.shape[0], _at(token_seq), positions.data_ptr(), _at(q_start),
-             out.data_ptr(), out.stride(0), T, n_z, max_n, n_heads, hkv, d, ps, pages, scale, at, max_keys, splits, _at(scratch),
-             dtype, code, _status_word(device)), f"{what}(H={n_heads},Hkv={hkv},D={d},page={ps},splits={splits})")
-    if scratch is not None:
+    scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    call = _ATTEND8.pack(*at, *pitch, block_table.data_ptr(), _status_word(index), width, block_table.shape[0], hkv, d, ps, pages, code, dtype,
+                         q_at, out_at, *ld, _at(token_seq), positions.data_ptr(), _at(q_start), _at(scratch), *laid,
+                         T, n_z, max_n, n_heads, splits, max_keys, scale, 0)
+    entry = ("attention_8bit_tc", "sandy_prefill_attention_8bit_tc") if tc else ("attention_8bit", "sandy_attention_8bit")
+    _run_on(index, _entry(*entry, ctypes.c_char_p, _V), (call,), what)
+    if floats:
         global LAUNCHES
         LAUNCHES += 1
+
+
+@functools.lru_cache(maxsize=256)
+def _tokens8(what: str, T: int, table, token_seq, positions) -> int:
+    for name, (dtype, shape, stride) in (("block_table", table), ("token_seq", token_seq), ("positions", positions)):
+        if dtype != torch.int32 or not _dense(shape, stride):
+            raise KernelError(f"{what}: {name} must be a contiguous int32 tensor")
+    if len(table[1]) != 2 or token_seq[1] != (T,) or positions[1] != (T,):
+        raise KernelError(f"{what}: q, token_seq and positions disagree on the tokens")
+    if T > 65535:
+        raise UnsupportedShape(f"{what}: at most 65535 tokens")
+    return table[1][1]
 
 
 def decode_attention_8bit(q, cache: Cache8, block_table, token_seq, positions, out, *, n_heads: int, scale: float, num_splits: int = 0,
@@ -723,26 +775,9 @@ def decode_attention_8bit(q, cache: Cache8, block_table, token_seq, positions, o
     Head sizes 16..256 in steps of 16, any page size.  num_splits: blocks that share a request's keys (0: the kernel's choice).
     rules: window, keep_first, softcap, chunk, sink, out_gate, dist_bias, elem_gate as in paged_attention.  A token at a negative
     position (a padded one) or of no visible key gets zeros."""
-    _known_rules("decode_attention_8bit", rules)
-    _indices("decode_attention_8bit", block_table=block_table, token_seq=token_seq, positions=positions)
-    T = q.shape[0]
-    if block_table.dim() != 2 or token_seq.numel() != T or positions.numel() != T:
-        raise KernelError("decode_attention_8bit: q, token_seq and positions disagree on the tokens")
-    if T > 65535:
-        raise UnsupportedShape("decode_attention_8bit: at most 65535 tokens")
-    _attention_8bit("decode_attention_8bit", q, cache, block_table, token_seq, positions, None, out, T, 1, n_heads, scale, num_splits, rules)
-
-
-# From so many rows (tokens x heads of a group) of the longest portion on, 8-bit prompt attention goes to the tcgen05 kernel.
-TC_ROWS_8BIT = 64
-
-
-def prefill_8bit_on_tcgen05(q, cache: Cache8, out, n_heads: int, scale: float, dist_bias=None) -> bool:
-    """Whether the tcgen05 kernel of 8-bit prompt attention takes a call: bfloat16, heads of 64 or 128, pages of a multiple of 16 keys, rows
-    on 16-byte boundaries, a positive scale, no bias by distance."""
-    _, _, ps, d = cache.k.shape
-    return (q.dtype == torch.bfloat16 and d in (64, 128) and ps % 16 == 0 and scale > 0 and dist_bias is None
-            and not (q.data_ptr() | out.data_ptr()) % 16 and not (q.stride(0) | out.stride(0)) % 8)
+    what, T = "decode_attention_8bit", q.shape[0]
+    width = _tokens8(what, T, _layout(block_table), _layout(token_seq), _layout(positions))
+    _attention_8bit(what, q, cache, block_table, width, token_seq, positions, None, out, T, 1, n_heads, scale, num_splits, False, rules)
 
 
 def prefill_attention_8bit(q, cache: Cache8, block_table, q_start, kv_before, out, *, n_heads: int, max_q_len: int, scale: float,
@@ -750,23 +785,14 @@ def prefill_attention_8bit(q, cache: Cache8, block_table, q_start, kv_before, ou
     """Attention of prompt portions over a cache in 8 bits: request s of the block table's rows brings rows q_start[s] ..
     q_start[s + 1] - 1 (int32 [S + 1]) at its positions kv_before[s] on (int32 [S]), whose keys and values kv_append_8bit has
     written; max_q_len: the most that one request brings.  Types, sizes and rules as in decode_attention_8bit; portions of one
-    token are allowed.  Rows of no request are left as they were.  tc: True asks for the tcgen05 kernel (prefill_8bit_on_tcgen05),
-    False for the mma.sync one, None picks; num_splits is the latter's."""
-    _known_rules("prefill_attention_8bit", rules)
-    S = _portions("prefill_attention_8bit", block_table, q_start, kv_before)
+    token are allowed.  Rows of no request are left as they were.  tc: True asks for the tcgen05 kernel (bfloat16, heads of 64 or 128,
+    pages of a multiple of 16 keys, rows of q and out on 16-byte boundaries, a positive scale, no bias by distance), False for the
+    mma.sync one, None picks; num_splits is the latter's."""
+    what = "prefill_attention_8bit"
+    S, width = _requests8(what, _layout(block_table), _layout(q_start), _layout(kv_before))
     if max_q_len < 0:
-        raise KernelError("prefill_attention_8bit: max_q_len is negative")
-    if tc is None:
-        tc = not num_splits and max_q_len * n_heads >= TC_ROWS_8BIT * cache.k.shape[1] and prefill_8bit_on_tcgen05(
-            q, cache, out, n_heads, scale, rules.get("dist_bias"))
-    _attention_8bit("prefill_attention_8bit", q, cache, block_table, None, kv_before, q_start, out, S, max_q_len, n_heads, scale, num_splits,
-                    rules, tc)
-
-
-def _known_rules(what: str, rules: dict) -> None:
-    unknown = set(rules) - {"window", "keep_first", "softcap", "chunk", "sink", "out_gate", "dist_bias", "elem_gate"}
-    if unknown:
-        raise TypeError(f"{what}() got an unexpected keyword argument {sorted(unknown)[0]!r}")
+        raise KernelError(f"{what}: max_q_len is negative")
+    _attention_8bit(what, q, cache, block_table, width, None, kv_before, q_start, out, S, max_q_len, n_heads, scale, num_splits, tc, rules)
 
 
 def _f32(t, name: str) -> None:
@@ -1221,6 +1247,34 @@ MAX_TOP_LOGPROBS = 32
 _LOGPROBS = (_V, _L, _I, _I, _V, _I, _V, _V, _V, _V, _I, _V, _V)
 
 
+@functools.lru_cache(maxsize=1024)
+def _logprobs_sizes(logits, ids, logprob, entropy, top_ids, top_logprobs, status) -> tuple:
+    """(row pitch, rows, vocabulary), likeliest tokens, type code of a call with these layouts."""
+    what = "token_logprobs"
+    dtype, shape, stride = logits
+    if len(shape) != 2 or shape[1] < 1 or (stride[1] != 1 and shape[1] > 1):
+        raise KernelError(f"{what}: logits must be [n, vocab] with an innermost stride of 1")
+    n, vocab = shape
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise UnsupportedShape(f"{what}: kernels take float32 or bfloat16 tensors, got {dtype}")
+    if (ids is None) != (logprob is None) or (top_ids is None) != (top_logprobs is None):
+        raise KernelError(f"{what}: ids go with logprob, top_ids with top_logprobs")
+    for name, t, dt in (("ids", ids, torch.int32), ("logprob", logprob, torch.float32), ("entropy", entropy, torch.float32)):
+        if t is not None and (t[0] != dt or t[1] != (n,) or not _dense(t[1], t[2])):
+            raise KernelError(f"{what}: {name} must be a contiguous {dt} tensor of one value per row")
+    top = 0
+    if top_ids is not None:
+        top = top_ids[1][-1] if len(top_ids[1]) else 0
+        for name, t, dt in (("top_ids", top_ids, torch.int32), ("top_logprobs", top_logprobs, torch.float32)):
+            if t[0] != dt or t[1] != (n, top) or not _dense(t[1], t[2]):
+                raise KernelError(f"{what}: {name} must be a contiguous {dt} tensor [n, k]")
+        if top > MAX_TOP_LOGPROBS or top > vocab:
+            raise UnsupportedShape(f"{what}: at most {MAX_TOP_LOGPROBS} likeliest tokens, and no more than the vocabulary has")
+    if status is not None and (status[0] != torch.int32 or 0 in status[1]):
+        raise KernelError(f"{what}: status must be an int32 tensor")
+    return (stride[0], n, vocab), top, F32 if dtype == torch.float32 else BF16
+
+
 def token_logprobs(logits, ids, logprob, *, entropy=None, top_ids=None, top_logprobs=None, status=None) -> None:
     """Of every row of `logits` ([n, vocab], float32 or bfloat16, any row pitch): logprob (float32 [n]) of the token ids[r] (int32
     [n]; -1: none, its logprob is 0), the row's entropy (float32 [n], in nats) and its k likeliest tokens, the likeliest first and of
@@ -1228,32 +1282,14 @@ def token_logprobs(logits, ids, logprob, *, entropy=None, top_ids=None, top_logp
     may each of the others.  A logit of minus infinity has probability 0.  A row with a NaN or plus infinity, or of minus
     infinities alone, gives NaN; with a NaN its top_ids are -1.  status (int32 [1]): bit 0 is raised for a NaN and for an id that is
     not in the vocabulary (its logprob is NaN)."""
-    what = "token_logprobs"
-    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.stride(1) != 1 and logits.shape[1] > 1):
-        raise KernelError(f"{what}: logits must be [n, vocab] with an innermost stride of 1")
-    n, vocab = logits.shape
-    dtype = _dt(logits)
-    if (ids is None) != (logprob is None) or (top_ids is None) != (top_logprobs is None):
-        raise KernelError(f"{what}: ids go with logprob, top_ids with top_logprobs")
-    for name, t, dt in (("ids", ids, torch.int32), ("logprob", logprob, torch.float32), ("entropy", entropy, torch.float32)):
-        if t is not None and (t.dtype != dt or t.shape != (n,) or not t.is_contiguous()):
-            raise KernelError(f"{what}: {name} must be a contiguous {dt} tensor of one value per row")
-    top = 0
-    if top_ids is not None:
-        top = top_ids.shape[-1]
-        for name, t, dt in (("top_ids", top_ids, torch.int32), ("top_logprobs", top_logprobs, torch.float32)):
-            if t.dtype != dt or t.shape != (n, top) or not t.is_contiguous():
-                raise KernelError(f"{what}: {name} must be a contiguous {dt} tensor [n, k]")
-        if top > MAX_TOP_LOGPROBS or top > vocab:
-            raise UnsupportedShape(f"{what}: at most {MAX_TOP_LOGPROBS} likeliest tokens, and no more than the vocabulary has")
-    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
-        raise KernelError(f"{what}: status must be an int32 tensor")
-    device = _device_of(what, logits, ids, logprob, entropy, top_ids, top_logprobs, status)
-    if n == 0:
+    sizes, top, dtype = _logprobs_sizes(_layout(logits), _layout(ids), _layout(logprob), _layout(entropy), _layout(top_ids), _layout(top_logprobs),
+                                        _layout(status))
+    index = _one_device("token_logprobs", logits, ids, logprob, entropy, top_ids, top_logprobs, status)
+    if sizes[1] == 0:
         return
-    _run_on(device, _entry("logprobs", "sandy_token_logprobs", _LOGPROBS),
-            (logits.data_ptr(), logits.stride(0), n, vocab, _at(ids), top, _at(logprob), _at(entropy), _at(top_ids), _at(top_logprobs), dtype,
-             _at(status)), f"{what}(vocab={vocab},top={top})")
+    _run_on(index, _entry("logprobs", "sandy_token_logprobs", *_LOGPROBS),
+            (logits.data_ptr(), *sizes, _at(ids), top, _at(logprob), _at(entropy), _at(top_ids), _at(top_logprobs), dtype, _at(status)),
+            "token_logprobs")
 
 
 def sample(logits, out_tokens, *, temperature=None, top_k=None, top_p=None, uniform=None, status=None,

@@ -10,6 +10,7 @@
 #include <cuda_runtime.h>
 
 #include "attention_rules.h"
+#include "cache8.h"
 #include "gated_linear.h"
 #include "matrix_state.h"
 
@@ -467,31 +468,16 @@ int sandy_sample(const float* logits, int ld, int n_rows, int vocab, const float
                  const int* logit_rows, int* positions, int* out_tokens, int* row_step, cudaStream_t stream);
 
 /* kv_8bit.cu */
-int sandy_kv_append_8bit(const void* k_src, const void* v_src, long long ld_k, long long ld_v, void* k, void* v, float* k_scale,
-                         float* v_scale, long long page_stride, long long scale_stride, const int* block_table, int max_blocks,
-                         const int* q_start, const int* kv_before, int n_seqs, int n_rows, int max_q_len, int n_kv_heads, int head_dim,
-                         int page_size, int num_pages, int dtype, int code, int* status, cudaStream_t stream);
-int sandy_kv_read_8bit(const void* k, const void* v, const float* k_scale, const float* v_scale, long long page_stride,
-                       long long scale_stride, const int* block_table, int max_blocks, const int* first, const int* out_start,
-                       void* k_out, void* v_out, long long ld_k, long long ld_v, int n_seqs, int n_rows, int max_len, int n_kv_heads,
-                       int head_dim, int page_size, int num_pages, int dtype, int code, int* status, cudaStream_t stream);
+int sandy_kv_append_8bit(const SandyRows8* rows, cudaStream_t stream);
+int sandy_kv_read_8bit(const SandyRows8* rows, cudaStream_t stream);
 
 /* attention_8bit.cu */
 int sandy_attention_8bit_splits(int n_rows, int n_z, int max_n, int n_heads, int n_kv_heads, int head_dim, int max_keys, int dtype, int asked,
                                 long long* scratch_floats);
-int sandy_attention_8bit(const void* q, long long ld_q, const void* k, const void* v, const float* k_scale, const float* v_scale,
-                         long long page_stride, long long scale_stride, const int* block_table, int max_blocks, int n_seqs,
-                         const int* token_seq, const int* positions, const int* q_start, void* out, long long ld_out, int n_rows, int n_z,
-                         int max_n, int n_heads, int n_kv_heads, int head_dim, int page_size, int num_pages, float scale,
-                         const SandyAttentionRules* rules, int max_keys, int num_splits, float* scratch, int dtype, int code, int* status,
-                         cudaStream_t stream);
+int sandy_attention_8bit(const SandyAttend8* call, cudaStream_t stream);
 
 /* attention_8bit_tc.cu */
-int sandy_prefill_attention_8bit_tc(const void* q, long long ld_q, const void* k, const void* v, const float* k_scale,
-                                    const float* v_scale, long long page_stride, long long scale_stride, const int* block_table,
-                                    int max_blocks, const int* kv_before, const int* q_start, void* out, long long ld_out, int n_rows,
-                                    int n_seqs, int max_q_len, int n_heads, int n_kv_heads, int head_dim, int page_size, int num_pages,
-                                    float scale, const SandyAttentionRules* rules, int code, int* status, cudaStream_t stream);
+int sandy_prefill_attention_8bit_tc(const SandyAttend8* call, cudaStream_t stream);
 
 /* logprobs.cu */
 int sandy_token_logprobs(const void* logits, long long ld, int n_rows, int vocab, const int* ids, int top, float* logprob,
