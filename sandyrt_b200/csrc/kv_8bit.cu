@@ -28,32 +28,64 @@ struct Planes {
     long long page_stride, scale_stride;
 };
 
-// Eight values as floats; ALIGNED: they start on 16 bytes.
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void load8(const T* __restrict__ p, float (&x)[8]) {
-    if (ALIGNED) {
-        if (sizeof(T) == 4) {
-            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-            x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-        } else {
-            const uint4 raw = *reinterpret_cast<const uint4*>(p);
-            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+// Eight values as they lie in memory; ALIGNED: they start on 16 bytes.
+template <typename T>
+struct Eight {
+    uint4 raw[sizeof(T) / 2];
+    template <bool ALIGNED>
+    __device__ __forceinline__ void load(const T* __restrict__ p) {
+        if (ALIGNED) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 f = __bfloat1622float2(h[i]);
-                x[2 * i] = f.x;
-                x[2 * i + 1] = f.y;
+            for (int i = 0; i < (int)sizeof(T) / 2; i++) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else if (sizeof(T) == 4) {
+            const unsigned* w = reinterpret_cast<const unsigned*>(p);
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; i++) raw[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        } else {
+            const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+            raw[0] = make_uint4(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16, h[4] | (unsigned)h[5] << 16, h[6] | (unsigned)h[7] << 16);
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    // the bits of the largest |x| as a float: as unsigned numbers floats without their sign keep their order, infinities and NaN above
+    __device__ __forceinline__ unsigned largest() const {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+            const uint4 r = raw[i];
+            if (sizeof(T) == 4) {
+                m = max(max(m, r.x & 0x7fffffffu), max(r.y & 0x7fffffffu, max(r.z & 0x7fffffffu, r.w & 0x7fffffffu)));
+            } else {
+                const unsigned h = __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+                m = max(h << 16, h & 0xffff0000u);
             }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = to_f32(p[i]);
+        return m;
     }
-}
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+            const unsigned w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (sizeof(T) == 4) {
+                    x[(4 * i + e) & 7] = __uint_as_float(w[e]);
+                } else {
+                    x[2 * e] = __uint_as_float(w[e] << 16);
+                    x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+                }
+            }
+        }
+    }
+};
 
-template <int CODE>
-__device__ __forceinline__ uint2 encode8(const float (&x)[8], float inv) {
+template <int CODE, typename T>
+__device__ __forceinline__ uint2 encode8(const Eight<T>& values, float inv) {
+    float x[8];
+    values.floats(x);
     const float most = __uint_as_float(LARGEST_KEPT_BITS);
     float y[8];
 #pragma unroll
@@ -82,42 +114,35 @@ append_kernel(const T* __restrict__ k_src, const T* __restrict__ v_src, long lon
     const int block = before / page_size + nth;
     const int lo = max(before, block * page_size), hi = min(before + n, (block + 1) * page_size);     // new positions in the block
     if (lo >= hi && before >= 0) return;
+    // the values, which hang on no page, and at the same time the page and the block's old scale
+    const int h = unit >> 1, plane = unit & 1;                      // neighbouring warps: keys and values of one head
+    const long long ld = plane ? ld_v : ld_k;
+    const T* src = (plane ? v_src : k_src) + (size_t)(first_row + max(lo - before, 0)) * ld + (size_t)h * head_dim;
+    const int per_row = head_dim >> 3, pieces = before >= 0 ? (hi - lo) * per_row : 0;
+    Eight<T> x[HELD];
+#pragma unroll
+    for (int k = 0; k < HELD; k++) {
+        const int i = lane + 32 * k, row = i / per_row;
+        if (i < pieces) x[k].template load<ALIGNED>(src + (size_t)row * ld + (i - row * per_row) * 8);
+        else x[k].clear();
+    }
     const int page = before >= 0 && block < max_blocks ? block_table[(size_t)s * max_blocks + block] : -1;
     if (page < 0 || page >= num_pages) {                            // no page behind these positions: nothing may be written
         if (lane == 0 && unit == 0 && status) atomicOr(status, 8);
         return;
     }
-    const int h = unit >> 1, plane = unit & 1;                      // neighbouring warps: keys and values of one head
-    const T* src = (plane ? v_src : k_src) + (size_t)(first_row + lo - before) * (plane ? ld_v : ld_k) + (size_t)h * head_dim;
-    const long long ld = plane ? ld_v : ld_k;
     uint8_t* codes = (plane ? cache.v : cache.k) + (size_t)page * cache.page_stride + (size_t)h * page_size * head_dim;
     float* scale_at = (plane ? cache.v_scale : cache.k_scale) + (size_t)page * cache.scale_stride + h;
     const int kept = lo - block * page_size;                        // positions of the block that were there before
     const float old = kept > 0 ? *scale_at : 0.0f;
-    const int per_row = head_dim >> 3, pieces = (hi - lo) * per_row;
 
-    // the largest |x|: as unsigned numbers floats without their sign keep their order, with infinities and NaN above all
-    float x[HELD][8];
     unsigned amax = 0;
 #pragma unroll
-    for (int k = 0; k < HELD; k++) {
-        const int i = lane + 32 * k;
-        if (i < pieces) {
-            load8<T, ALIGNED>(src + (size_t)(i / per_row) * ld + (i % per_row) * 8, x[k]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[k][e] = 0.0f;
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < HELD; k++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) amax = max(amax, __float_as_uint(x[k][e]) & 0x7fffffffu);
+    for (int k = 0; k < HELD; k++) amax = max(amax, x[k].largest());
     for (int i = lane + 32 * HELD; i < pieces; i += 32) {
-        float y[8];
-        load8<T, ALIGNED>(src + (size_t)(i / per_row) * ld + (i % per_row) * 8, y);
-#pragma unroll
-        for (int e = 0; e < 8; e++) amax = max(amax, __float_as_uint(y[e]) & 0x7fffffffu);
+        Eight<T> y;
+        y.template load<ALIGNED>(src + (size_t)(i / per_row) * ld + (i % per_row) * 8);
+        amax = max(amax, y.largest());
     }
     amax = __reduce_max_sync(0xffffffffu, amax);
 
@@ -145,8 +170,8 @@ append_kernel(const T* __restrict__ k_src, const T* __restrict__ v_src, long lon
         if (i < pieces) dst[i] = sound ? encode8<CODE>(x[k], inv) : make_uint2(0u, 0u);
     }
     for (int i = lane + 32 * HELD; i < pieces; i += 32) {
-        float y[8];
-        load8<T, ALIGNED>(src + (size_t)(i / per_row) * ld + (i % per_row) * 8, y);
+        Eight<T> y;
+        y.template load<ALIGNED>(src + (size_t)(i / per_row) * ld + (i % per_row) * 8);
         dst[i] = sound ? encode8<CODE>(y, inv) : make_uint2(0u, 0u);
     }
     if (lane == 0) *scale_at = now;

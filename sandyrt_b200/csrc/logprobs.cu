@@ -10,9 +10,10 @@
 // What bounds it: the logits' bytes, read once.  A block walks a row, or a cluster of 2, 4 or 8 blocks a row where rows are few
 // (partial sums and candidates meet in the first block's shared memory), 16 logits a thread at a time, the next 16 on their way.
 // Sums: a thread carries (m, Z, sum e (x - m)) of its own logits in 32 bits and rescales when a group of 16 raises m.
-// Top: the first group's maxima, one a thread, give a bound -- the `top`-th largest of them is at most the row's `top`-th largest
-// -- and only logits at or above it, in the order of (value, lower id), go to a list in shared memory (some top * vocabulary /
-// 4096 of them); at the end each counts how many of the list are before it.  No list is sorted, and no logit is read twice.
+// Top: the first group's maxima, one for four threads, give a bound -- the `top`-th largest of them is at most the row's `top`-th largest
+// -- and only logits at or above it, in the order of (value, lower id), go to a list in shared memory; after two groups and after
+// five the list's own `top`-th best is the bound.  At the end each of the list counts how many of it are in front.  No logit is
+// read twice.
 // Where a list runs over (logits that rise along the row) the block finds the bound by bisection over its part of the row instead.
 #include <cooperative_groups.h>
 
@@ -26,6 +27,7 @@ constexpr int THREADS = 256;
 constexpr int EACH = 16;                   // logits a thread takes at a time
 constexpr int LIST = 1024;                 // candidates a block keeps
 constexpr int MAX_TOP = 32;
+constexpr int GROUPS = THREADS / 4;        // threads by fours: whose maxima give the first bound
 constexpr int MAX_CLUSTER = 8;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -66,10 +68,25 @@ __device__ __forceinline__ Sums joined(Sums a, Sums b) {
     return {m, a.z + b.z, a.w + b.w};
 }
 __device__ __forceinline__ void add(Sums& s, float x) {       // x <= s.m, or not a number
-    const float d = fmaxf(x - s.m, -1e30f);                    // of minus infinity: e = 0, and 0 * d must be 0
-    const float e = ex2((x - s.m) * LOG2E);
+    const float d = x - s.m, e = ex2(d * LOG2E);
     s.z += e;
-    s.w = fmaf(e, d, s.w);
+    s.w = fmaf(e, fmaxf(d, -1e30f), s.w);                      // of minus infinity: e = 0, and 0 * d must be 0
+}
+// two 32-bit operations in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
 }
 
 // What a block knows of its part of a row.
@@ -107,7 +124,8 @@ logprobs_kernel(const T* __restrict__ logits, long long ld, int vocab, const int
                 float* __restrict__ entropy, int* __restrict__ top_ids, float* __restrict__ top_logprobs, int parts,
                 int* __restrict__ status) {
     __shared__ u64 list[LIST];
-    __shared__ u64 maxima[THREADS];
+    __shared__ u64 maxima[GROUPS];
+    __shared__ u64 best[MAX_TOP];
     __shared__ Sums warp_sums[THREADS / 32];
     __shared__ Part got[MAX_CLUSTER];                           // in the first block of a cluster: every block's
     __shared__ u64 s_bound;
@@ -147,35 +165,75 @@ logprobs_kernel(const T* __restrict__ logits, long long ld, int vocab, const int
         const int at = atomicAdd(&s_count, 1);
         if (at < LIST) list[at] = key;
     };
-    bool first = true;
-    for (int at = begin + tid; first || at - tid < end; at += THREADS * Group<T>::N) {
+    // The list's `top` best alone, in order; the last of them is the new bound.
+    auto tighten = [&]() {
+        __syncthreads();
+        const int n = s_count;
+        if (n > top && n <= LIST) {
+            for (int i = tid; i < n; i += THREADS) {
+                const u64 mine = list[i];
+                int before = 0;
+                for (int j = 0; j < n; j++) before += list[j] > mine;
+                if (before < top) best[before] = mine;
+            }
+            __syncthreads();
+            if (tid < top) list[tid] = best[tid];
+            if (tid == 0) s_count = top;
+            bound = best[top - 1];
+            bound_x = key_value(bound);
+        }
+        __syncthreads();
+    };
+    float2 z = {0.0f, 0.0f}, w = {0.0f, 0.0f};                   // s.z and s.w, by the logits' parity
+    int nth = 0;                                                  // groups of 16 taken
+    for (int at = begin + tid; nth == 0 || at - tid < end; at += THREADS * Group<T>::N, nth++) {
         next.load(body, at + THREADS * Group<T>::N, end);
         float most = now[0];
 #pragma unroll
         for (int i = 1; i < EACH; i++) most = fmaxf(most, now[i]);
-        if (first && top > 0) {
-            // the `top`-th largest of the threads' maxima, loose logits among them
+        if (nth == 0 && top > 0) {
+            // the `top`-th largest of the maxima of four threads each, loose logits among them
             u64 mine = my_loose >= 0 ? rank_key(loose_x, my_loose) : 0;
 #pragma unroll
             for (int i = 0; i < EACH; i++) {
                 const int v = at + i / PER * THREADS;
                 if (v < end && now[i] == now[i]) mine = max(mine, rank_key(now[i], head + v * PER + i % PER));
             }
-            maxima[tid] = mine;
+            mine = max(mine, (u64)__shfl_xor_sync(0xffffffffu, mine, 1));
+            mine = max(mine, (u64)__shfl_xor_sync(0xffffffffu, mine, 2));
+            if ((tid & 3) == 0) maxima[tid >> 2] = mine;
             __syncthreads();
-            int before = 0;
-#pragma unroll 8
-            for (int j = 0; j < THREADS; j++) before += maxima[j] > mine;
-            if (before == top - 1 && mine) s_bound = mine;       // keys differ; with fewer than `top` the bound stays 0
+            if (tid < GROUPS) {
+                mine = maxima[tid];
+                int before = 0;
+#pragma unroll 16
+                for (int j = 0; j < GROUPS; j++) before += maxima[j] > mine;
+                if (before == top - 1 && mine) s_bound = mine;   // keys differ; with fewer than `top` the bound stays 0
+            }
             __syncthreads();
             bound = s_bound;
             bound_x = bound ? key_value(bound) : -INFINITY;
             if (my_loose >= 0 && loose_x >= bound_x) offer(loose_x, my_loose);
         }
-        first = false;
-        if (most > s.m) s = raised(s, most);
+        // what the bound lets through falls with the logits it was taken from: after two groups and after five it is taken anew
+        if (top > 0 && (nth == 2 || nth == 5)) tighten();
+        if (most > s.m) {
+            s.z = z.x + z.y;
+            s.w = w.x + w.y;
+            s = raised(s, most);
+            z = {s.z, 0.0f};
+            w = {s.w, 0.0f};
+        }
+        const float2 minus = {-s.m, -s.m}, l2e = {LOG2E, LOG2E}, none = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < EACH; i++) add(s, now[i]);
+        for (int i = 0; i < EACH; i += 2) {
+            float2 d = add2(make_float2(now[i], now[i + 1]), minus);
+            const float2 t = fma2(d, l2e, none);
+            const float2 e = {ex2(t.x), ex2(t.y)};
+            d = make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f));       // see add()
+            z = add2(z, e);
+            w = fma2(e, d, w);
+        }
         if (top > 0 && most >= bound_x) {
 #pragma unroll
             for (int i = 0; i < EACH; i++) {
@@ -185,6 +243,8 @@ logprobs_kernel(const T* __restrict__ logits, long long ld, int vocab, const int
         }
         now = next;
     }
+    s.z = z.x + z.y;
+    s.w = w.x + w.y;
     if (my_loose >= 0) {
         if (loose_x > s.m) s = raised(s, loose_x);
         add(s, loose_x);
