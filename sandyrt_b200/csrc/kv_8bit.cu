@@ -82,16 +82,17 @@ struct Eight {
     }
 };
 
+// huge: some |x| of the block is above what a code times its scale may reach.
 template <int CODE, typename T>
-__device__ __forceinline__ uint2 encode8(const Eight<T>& values, float inv) {
+__device__ __forceinline__ uint2 encode8(const Eight<T>& values, float inv, bool huge) {
     float x[8];
     values.floats(x);
-    const float most = __uint_as_float(LARGEST_KEPT_BITS);
-    float y[8];
+    if (huge) {
+        const float most = __uint_as_float(LARGEST_KEPT_BITS);
 #pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = fminf(fmaxf(x[i], -most), most) * inv;
-    return make_uint2(encode2<CODE>(y[0], y[1]) | encode2<CODE>(y[2], y[3]) << 16,
-                      encode2<CODE>(y[4], y[5]) | encode2<CODE>(y[6], y[7]) << 16);
+        for (int i = 0; i < 8; i++) x[i] = fminf(fmaxf(x[i], -most), most);
+    }
+    return make_uint2(encode4<CODE>(x[0], x[1], x[2], x[3], inv), encode4<CODE>(x[4], x[5], x[6], x[7], inv));
 }
 
 template <typename T, int CODE, bool ALIGNED>
@@ -99,19 +100,18 @@ __global__ void __launch_bounds__(WARPS * 32)
 append_kernel(const T* __restrict__ k_src, const T* __restrict__ v_src, long long ld_k, long long ld_v, Planes cache,
               const int* __restrict__ block_table, int max_blocks, const int* __restrict__ q_start,
               const int* __restrict__ kv_before, int n_rows, int n_kv_heads, int head_dim, int page_size, int num_pages,
-              int groups_of_heads, int* __restrict__ status) {
+              int page_shift, int row_shift, int* __restrict__ status) {
     pdl_launch_dependents();
     pdl_wait();
-    const int s = blockIdx.y;
-    const int nth = blockIdx.x / groups_of_heads;                   // which of the request's touched pages
-    const int unit = (blockIdx.x % groups_of_heads) * WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int s = blockIdx.z, nth = blockIdx.x;                     // which of the request's touched pages
+    const int unit = blockIdx.y * WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int first_row = q_start[s], n = q_start[s + 1] - first_row, before = kv_before[s];
     if (unit >= 2 * n_kv_heads || n <= 0) return;
     if (first_row < 0 || n > n_rows - first_row) {                  // rows that are not there
         if (lane == 0 && status) atomicOr(status, 8);
         return;
     }
-    const int block = before / page_size + nth;
+    const int block = (page_shift >= 0 ? before >> page_shift : before / page_size) + nth;
     const int lo = max(before, block * page_size), hi = min(before + n, (block + 1) * page_size);     // new positions in the block
     if (lo >= hi && before >= 0) return;
     // the values, which hang on no page, and at the same time the page and the block's old scale
@@ -122,7 +122,7 @@ append_kernel(const T* __restrict__ k_src, const T* __restrict__ v_src, long lon
     Eight<T> x[HELD];
 #pragma unroll
     for (int k = 0; k < HELD; k++) {
-        const int i = lane + 32 * k, row = i / per_row;
+        const int i = lane + 32 * k, row = row_shift >= 0 ? i >> row_shift : i / per_row;
         if (i < pieces) x[k].template load<ALIGNED>(src + (size_t)row * ld + (i - row * per_row) * 8);
         else x[k].clear();
     }
@@ -150,7 +150,7 @@ append_kernel(const T* __restrict__ k_src, const T* __restrict__ v_src, long lon
     float now = amax >= 0x7f800000u ? nan : scale_for<CODE>(min(amax, LARGEST_KEPT_BITS));
     if (kept > 0 && !(old <= now)) now = old;                       // the old one is larger, or one of the two is NaN
     if (amax >= 0x7f800000u) now = nan;
-    const bool sound = now == now;
+    const bool sound = now == now, huge = amax > LARGEST_KEPT_BITS;
     const float inv = sound ? 1.0f / now : 0.0f;                    // of a power of two: exact
 
     if (kept > 0 && sound && now > old) {                           // the block's earlier codes at its new scale
@@ -160,19 +160,19 @@ append_kernel(const T* __restrict__ k_src, const T* __restrict__ v_src, long lon
             unsigned a, b;
             decode4<CODE>(*w, a, b);
             const float2 p = half2_floats(a), q = half2_floats(b);
-            *w = encode2<CODE>(p.x * shrink, p.y * shrink) | encode2<CODE>(q.x * shrink, q.y * shrink) << 16;
+            *w = encode4<CODE>(p.x, p.y, q.x, q.y, shrink);
         }
     }
     uint2* dst = reinterpret_cast<uint2*>(codes + (size_t)kept * head_dim);      // the new rows follow one another in a block
 #pragma unroll
     for (int k = 0; k < HELD; k++) {
         const int i = lane + 32 * k;
-        if (i < pieces) dst[i] = sound ? encode8<CODE>(x[k], inv) : make_uint2(0u, 0u);
+        if (i < pieces) dst[i] = sound ? encode8<CODE>(x[k], inv, huge) : make_uint2(0u, 0u);
     }
     for (int i = lane + 32 * HELD; i < pieces; i += 32) {
         Eight<T> y;
         y.template load<ALIGNED>(src + (size_t)(i / per_row) * ld + (i % per_row) * 8);
-        dst[i] = sound ? encode8<CODE>(y, inv) : make_uint2(0u, 0u);
+        dst[i] = sound ? encode8<CODE>(y, inv, huge) : make_uint2(0u, 0u);
     }
     if (lane == 0) *scale_at = now;
 }
@@ -273,13 +273,15 @@ SANDY_API int sandy_kv_append_8bit(const SandyRows8* r, cudaStream_t stream) {
     if (const int code = refused(r)) return code;
     const int groups = (2 * c.n_kv_heads + WARPS - 1) / WARPS;
     const long long touched = ((long long)r->max_len + c.page_size - 2) / c.page_size + 1;      // by one request, wherever it starts
-    if (touched * groups > 0x7fffffffll) return SANDY_ERR_UNSUPPORTED;
+    if (touched > 0x7fffffffll || groups > 65535) return SANDY_ERR_UNSUPPORTED;
     const Planes cache = {(uint8_t*)c.k, (uint8_t*)c.v, c.k_scale, c.v_scale, c.page_stride, c.scale_stride};
-    const dim3 grid((unsigned)(touched * groups), c.n_seqs), block(WARPS * 32);
+    const dim3 grid((unsigned)touched, groups, c.n_seqs), block(WARPS * 32);
+    auto shift = [](int n) { return (n & (n - 1)) == 0 ? __builtin_ctz(n) : -1; };      // -1: no power of two
 #define APPEND(T, CODE)                                                                                                         \
     return sandy_launch(on_16_bytes<T>(*r) ? append_kernel<T, CODE, true> : append_kernel<T, CODE, false>, grid, block, 0, stream, \
                         (const T*)r->k_rows, (const T*)r->v_rows, r->ld_k, r->ld_v, cache, c.block_table, c.max_blocks, r->start, \
-                        r->first, r->n_rows, c.n_kv_heads, c.head_dim, c.page_size, c.num_pages, groups, c.status)
+                        r->first, r->n_rows, c.n_kv_heads, c.head_dim, c.page_size, c.num_pages, shift(c.page_size), \
+                        shift(c.head_dim / 8), c.status)
     if (c.dtype == SANDY_F32 && c.code == SANDY_E4M3) APPEND(float, SANDY_E4M3);
     if (c.dtype == SANDY_F32 && c.code == SANDY_INT8) APPEND(float, SANDY_INT8);
     if (c.dtype == SANDY_BF16 && c.code == SANDY_E4M3) APPEND(bf16, SANDY_E4M3);

@@ -30,16 +30,20 @@ __device__ __forceinline__ float scale_for(unsigned amax) {
     return __uint_as_float((unsigned)(max(e, SMALLEST_SCALE_EXPONENT) + 127) << 23);
 }
 
-// Two numbers, already divided by their scale, as two codes (the first in the low byte).  Round to nearest, ties to even.
+// Four numbers, times inv, as four codes (the first in the low byte).  Round to nearest, ties to even; |x * inv| at most the largest code.
 template <int CODE>
-__device__ __forceinline__ unsigned encode2(float a, float b) {
+__device__ __forceinline__ unsigned encode4(float a, float b, float c, float d, float inv) {
     if (CODE == SANDY_E4M3) {
-        unsigned short r;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+        unsigned r;
+        asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\tmov.b32 %0, {l, h};\n\t}"
+            : "=r"(r)
+            : "f"(a * inv), "f"(b * inv), "f"(c * inv), "f"(d * inv));
         return r;
     }
-    const int x = max(-127, min(127, __float2int_rn(a))), y = max(-127, min(127, __float2int_rn(b)));
-    return (unsigned)(x & 0xff) | ((unsigned)(y & 0xff) << 8);
+    // 1.5 * 2^23 added: the last place is 1, so the sum is rounded to a whole number, which is its low byte
+    const unsigned p = __float_as_uint(fmaf(a, inv, 12582912.0f)), q = __float_as_uint(fmaf(b, inv, 12582912.0f));
+    const unsigned r = __float_as_uint(fmaf(c, inv, 12582912.0f)), s = __float_as_uint(fmaf(d, inv, 12582912.0f));
+    return __byte_perm(__byte_perm(p, q, 0x0040), __byte_perm(r, s, 0x0040), 0x5410);
 }
 
 // Four codes as two pairs of half-precision numbers: bytes 0, 1 and bytes 2, 3.  Exact for every code.

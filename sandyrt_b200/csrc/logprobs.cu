@@ -23,11 +23,10 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int THREADS = 256;
 constexpr int EACH = 16;                   // logits a thread takes at a time
 constexpr int LIST = 1024;                 // candidates a block keeps
 constexpr int MAX_TOP = 32;
-constexpr int GROUPS = THREADS / 4;        // threads by fours: whose maxima give the first bound
+constexpr int GROUPS = 64;                 // of neighbouring threads, whose maxima give the first bound
 constexpr int MAX_CLUSTER = 8;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -96,12 +95,18 @@ struct Part {
     u64 top[MAX_TOP];
 };
 
-template <typename T>
+template <typename T, int THREADS>
 struct Group {                                                  // a thread's 16 logits, as they come from memory
     static constexpr int PER = 16 / (int)sizeof(T), N = EACH / PER;
     uint4 raw[N];
     // pieces first, first + THREADS, .. of the row's 16-byte pieces; those at or past `end` are minus infinities
     __device__ __forceinline__ void load(const T* p, int first, int end) {
+        if (first - (int)threadIdx.x + N * THREADS <= end) {     // all of them are there
+            const uint4* from = reinterpret_cast<const uint4*>(p) + first;
+#pragma unroll
+            for (int u = 0; u < N; u++) raw[u] = __ldcs(from + u * THREADS);
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < N; u++) {
             const int v = first + u * THREADS;
@@ -118,8 +123,10 @@ struct Group {                                                  // a thread's 16
     }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS)
+// THREADS: 256, or 128 where every block has a row to itself: then twice as many rows are under way at a time, and what a row needs before
+// and behind its walk is hidden behind the others'.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 logprobs_kernel(const T* __restrict__ logits, long long ld, int vocab, const int* __restrict__ ids, int top, float* __restrict__ logprob,
                 float* __restrict__ entropy, int* __restrict__ top_ids, float* __restrict__ top_logprobs, int parts,
                 int* __restrict__ status) {
@@ -138,7 +145,7 @@ logprobs_kernel(const T* __restrict__ logits, long long ld, int vocab, const int
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const T* row = logits + (size_t)row_at * ld;
     // the row's 16-byte pieces, and in front of and behind them what is left; the first block takes that too
-    constexpr int PER = Group<T>::PER;
+    constexpr int PER = Group<T, THREADS>::PER;
     const int head = min(vocab, (int)(((16 - ((uintptr_t)row & 15)) & 15) / sizeof(T)));
     const T* body = row + head;
     const int pieces = (vocab - head) / PER, per_part = (pieces + parts - 1) / parts;
@@ -151,7 +158,7 @@ logprobs_kernel(const T* __restrict__ logits, long long ld, int vocab, const int
     }
     const int given = ids ? ids[row_at] : -1;
 
-    Group<T> now, next;
+    Group<T, THREADS> now, next;
     now.load(body, begin + tid, end);
     int my_loose = tid < loose ? (tid < head ? tid : tail + tid - head) : -1;
     const float loose_x = my_loose >= 0 ? to_f32(row[my_loose]) : -INFINITY;
@@ -186,11 +193,12 @@ logprobs_kernel(const T* __restrict__ logits, long long ld, int vocab, const int
     };
     float2 z = {0.0f, 0.0f}, w = {0.0f, 0.0f};                   // s.z and s.w, by the logits' parity
     int nth = 0;                                                  // groups of 16 taken
-    for (int at = begin + tid; nth == 0 || at - tid < end; at += THREADS * Group<T>::N, nth++) {
-        next.load(body, at + THREADS * Group<T>::N, end);
-        float most = now[0];
+    int at = begin + tid;
+    auto take = [&](const Group<T, THREADS>& now) {
+        float part_most[4], most;                                // of its fours
 #pragma unroll
-        for (int i = 1; i < EACH; i++) most = fmaxf(most, now[i]);
+        for (int q = 0; q < 4; q++) part_most[q] = fmaxf(fmaxf(now[4 * q], now[4 * q + 1]), fmaxf(now[4 * q + 2], now[4 * q + 3]));
+        most = fmaxf(fmaxf(part_most[0], part_most[1]), fmaxf(part_most[2], part_most[3]));
         if (nth == 0 && top > 0) {
             // the `top`-th largest of the maxima of four threads each, loose logits among them
             u64 mine = my_loose >= 0 ? rank_key(loose_x, my_loose) : 0;
@@ -199,9 +207,10 @@ logprobs_kernel(const T* __restrict__ logits, long long ld, int vocab, const int
                 const int v = at + i / PER * THREADS;
                 if (v < end && now[i] == now[i]) mine = max(mine, rank_key(now[i], head + v * PER + i % PER));
             }
-            mine = max(mine, (u64)__shfl_xor_sync(0xffffffffu, mine, 1));
-            mine = max(mine, (u64)__shfl_xor_sync(0xffffffffu, mine, 2));
-            if ((tid & 3) == 0) maxima[tid >> 2] = mine;
+            constexpr int EACH_GROUP = THREADS / GROUPS;
+#pragma unroll
+            for (int o = 1; o < EACH_GROUP; o <<= 1) mine = max(mine, (u64)__shfl_xor_sync(0xffffffffu, mine, o));
+            if (tid % EACH_GROUP == 0) maxima[tid / EACH_GROUP] = mine;
             __syncthreads();
             if (tid < GROUPS) {
                 mine = maxima[tid];
@@ -215,8 +224,9 @@ logprobs_kernel(const T* __restrict__ logits, long long ld, int vocab, const int
             bound_x = bound ? key_value(bound) : -INFINITY;
             if (my_loose >= 0 && loose_x >= bound_x) offer(loose_x, my_loose);
         }
+        nth++;
         // what the bound lets through falls with the logits it was taken from: after two groups and after five it is taken anew
-        if (top > 0 && (nth == 2 || nth == 5)) tighten();
+        if (top > 0 && (nth == 3 || nth == 6 || nth == 12)) tighten();
         if (most > s.m) {
             s.z = z.x + z.y;
             s.w = w.x + w.y;
@@ -224,24 +234,42 @@ logprobs_kernel(const T* __restrict__ logits, long long ld, int vocab, const int
             z = {s.z, 0.0f};
             w = {s.w, 0.0f};
         }
-        const float2 minus = {-s.m, -s.m}, l2e = {LOG2E, LOG2E}, none = {0.0f, 0.0f};
+        if (at - tid + Group<T, THREADS>::N * THREADS <= end) {
+            const float2 minus = {-s.m, -s.m}, l2e = {LOG2E, LOG2E}, none = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < EACH; i += 2) {
-            float2 d = add2(make_float2(now[i], now[i + 1]), minus);
-            const float2 t = fma2(d, l2e, none);
-            const float2 e = {ex2(t.x), ex2(t.y)};
-            d = make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f));       // see add()
-            z = add2(z, e);
-            w = fma2(e, d, w);
+            for (int i = 0; i < EACH; i += 2) {
+                // of a logit of minus infinity e * d is 0 times infinity: the sum w becomes NaN and is made again behind the walk
+                const float2 d = add2(make_float2(now[i], now[i + 1]), minus), t = fma2(d, l2e, none);
+                const float2 e = {ex2(t.x), ex2(t.y)};
+                z = add2(z, e);
+                w = fma2(e, d, w);
+            }
+        } else {                                                  // the last ones, with minus infinities behind them
+            Sums few = {s.m, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < EACH; i++) add(few, now[i]);
+            z.x += few.z;
+            w.x += few.w;
         }
         if (top > 0 && most >= bound_x) {
 #pragma unroll
-            for (int i = 0; i < EACH; i++) {
-                const int v = at + i / PER * THREADS;
-                if (now[i] >= bound_x && v < end) offer(now[i], head + v * PER + i % PER);
-            }
+            for (int q = 0; q < 4; q++)
+                if (part_most[q] >= bound_x) {
+#pragma unroll
+                    for (int i = 4 * q; i < 4 * q + 4; i++) {
+                        const int v = at + i / PER * THREADS;
+                        if (now[i] >= bound_x && v < end) offer(now[i], head + v * PER + i % PER);
+                    }
+                }
         }
-        now = next;
+    };
+    for (; nth == 0 || at - tid < end; at += THREADS * Group<T, THREADS>::N) {
+        next.load(body, at + THREADS * Group<T, THREADS>::N, end);
+        take(now);
+        at += THREADS * Group<T, THREADS>::N;
+        if (at - tid >= end) break;
+        now.load(body, at + THREADS * Group<T, THREADS>::N, end);
+        take(next);
     }
     s.z = z.x + z.y;
     s.w = w.x + w.y;
@@ -261,6 +289,20 @@ logprobs_kernel(const T* __restrict__ logits, long long ld, int vocab, const int
     s = warp_sums[0];
 #pragma unroll
     for (int i = 1; i < THREADS / 32; i++) s = joined(s, warp_sums[i]);
+
+    if (s.w != s.w && s.z == s.z) {                              // minus infinities among the block's logits: w over its part again
+        __syncthreads();
+        Sums mine = {s.m, 0.0f, 0.0f};
+        for (int v = begin + tid; v < end; v += THREADS)
+            for (int e = 0; e < PER; e++) add(mine, to_f32(body[(size_t)v * PER + e]));
+        if (my_loose >= 0) add(mine, loose_x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mine.w += __shfl_xor_sync(0xffffffffu, mine.w, o);
+        if (lane == 0) warp_sums[warp].w = mine.w;
+        __syncthreads();
+        s.w = 0.0f;
+        for (int i = 0; i < THREADS / 32; i++) s.w += warp_sums[i].w;
+    }
 
     // ---- the block's `top` best ----------------------------------------------------------------------------------------
     auto each = [&](auto&& f) {                                  // f(x, id) over the thread's share of the block's part, again
@@ -369,11 +411,12 @@ SANDY_API int sandy_token_logprobs(const void* logits, long long ld, int n_rows,
     if ((uintptr_t)logits % (dtype == SANDY_F32 ? 4 : 2)) return SANDY_ERR_UNSUPPORTED;
     // Few rows: blocks share one, each with at least a group of 4,096 logits.
     int parts = 1;
-    while (parts < MAX_CLUSTER && (long long)n_rows * parts * 2 <= 4ll * sandy_sm_count() && vocab / (parts * 2) >= THREADS * EACH) parts *= 2;
+    while (parts < MAX_CLUSTER && (long long)n_rows * parts * 2 <= 4ll * sandy_sm_count() && vocab / (parts * 2) >= 256 * EACH) parts *= 2;
     if ((long long)n_rows * parts > 0x7fffffffll) return SANDY_ERR_UNSUPPORTED;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(n_rows * parts));
-    cfg.blockDim = dim3(THREADS);
+    const int threads = parts > 1 ? 256 : 128;
+    cfg.blockDim = dim3(threads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     int na = 0;
@@ -391,8 +434,17 @@ SANDY_API int sandy_token_logprobs(const void* logits, long long ld, int n_rows,
     }
     cfg.attrs = attr;
     cfg.numAttrs = na;
-    const cudaError_t e = dtype == SANDY_F32
-        ? cudaLaunchKernelEx(&cfg, logprobs_kernel<float>, (const float*)logits, ld, vocab, ids, top, logprob, entropy, top_ids, top_logprobs, parts, status)
-        : cudaLaunchKernelEx(&cfg, logprobs_kernel<bf16>, (const bf16*)logits, ld, vocab, ids, top, logprob, entropy, top_ids, top_logprobs, parts, status);
+    cudaError_t e;
+#define LAUNCH(T, THREADS)                                                                                                       \
+    e = cudaLaunchKernelEx(&cfg, logprobs_kernel<T, THREADS>, (const T*)logits, ld, vocab, ids, top, logprob, entropy, top_ids,  \
+                           top_logprobs, parts, status)
+    if (dtype == SANDY_F32) {
+        if (threads == 256) LAUNCH(float, 256);
+        else LAUNCH(float, 128);
+    } else {
+        if (threads == 256) LAUNCH(bf16, 256);
+        else LAUNCH(bf16, 128);
+    }
+#undef LAUNCH
     return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
