@@ -1,6 +1,7 @@
 """Command line of the engine.
 
     python -m sandyrt_b200 generate --model DIR --prompt-ids 1,2,3 [options]
+    python -m sandyrt_b200 score --model DIR --ids 1,2,3 [--top K]
     python -m sandyrt_b200 random-model --config config.json --out DIR [--seed S] [--dtype bfloat16]
     python -m sandyrt_b200 replay --model DIR --dtype float32 --out DIR --max-tokens N < steps.jsonl
 
@@ -51,6 +52,21 @@ def cmd_generate(a) -> int:
     return 0
 
 
+def cmd_score(a) -> int:
+    from .engine.llm import LLM
+
+    texts = [_ids(t) for t in a.ids]
+    longest = max(len(t) for t in texts)
+    llm = LLM(a.model, dtype=a.dtype, cache_tokens=longest + a.page_size, page_size=a.page_size, max_live=1)
+    for i, (t, s) in enumerate(zip(texts, llm.score(texts, top=a.top))):
+        line = {"text": i, "tokens": len(t), "logprob": float(s.logprobs.astype("float64").sum()), "logprobs": s.logprobs.tolist(),
+                "entropies": s.entropies.tolist()}
+        if a.top:
+            line.update(top_ids=s.top_ids.tolist(), top_logprobs=s.top_logprobs.tolist())
+        print(json.dumps(line))
+    return 0
+
+
 def cmd_random_model(a) -> int:
     import torch
 
@@ -97,6 +113,14 @@ def main(argv: Optional[List[str]] = None) -> int:
     g.add_argument("--profile", action="store_true", help="print the throughput line per request")
     g.add_argument("--debug", action="store_true")
     g.set_defaults(fn=cmd_generate)
+
+    c = sub.add_parser("score", help="log-probabilities of the tokens of one or more texts")
+    c.add_argument("--model", required=True, help="folder with config.json and model.safetensors")
+    c.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    c.add_argument("--ids", action="append", required=True, help="comma- or space-separated ids (repeatable)")
+    c.add_argument("--top", type=int, default=0, help="also the likeliest tokens of every place, at most 32")
+    c.add_argument("--page-size", type=int, default=16)
+    c.set_defaults(fn=cmd_score)
 
     r = sub.add_parser("random-model", help="write a model folder with seeded random weights")
     r.add_argument("--config", required=True, help="a config.json of a registered architecture")

@@ -140,13 +140,14 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
 
     pdl_launch_dependents();
     pdl_wait();
-    const int z = blockIdx.z, kvh = blockIdx.y;
+    // tiles in the slowest dimension: all requests' blocks with the most keys start first, and what is left for the end is small
+    const int z = blockIdx.y, kvh = blockIdx.x, nth = blockIdx.z;
     const int row0 = a.q_start[z], n = a.q_start[z + 1] - row0, before = a.kv_before[z];
     const bool there = row0 >= 0 && n <= a.n_rows - row0;            // the portion's rows
     if (!there && n > 0 && threadIdx.x == 0 && a.status) atomicOr(a.status, 16);
     const int tiles = there && n > 0 ? (int)(((long long)n * a.group + 255) / 256) : 0;
-    if ((int)blockIdx.x >= tiles) return;
-    const int first = (tiles - 1 - blockIdx.x) * 256;                // the rows with the most keys start first
+    if (nth >= tiles) return;
+    const int first = (tiles - 1 - nth) * 256;
     const int n_valid = min(256, n * a.group - first);
     const int groups = n_valid > 128 ? 2 : 1;
     const int pos_first = before + first / a.group, pos_last = before + (first + n_valid - 1) / a.group;
@@ -556,7 +557,7 @@ int launch(const Args& a, int n_seqs, int max_q_len, cudaStream_t stream) {
         if (e != cudaSuccess) return (int)e;
         told.fetch_or(bit);
     }
-    const dim3 grid((unsigned)(((long long)max_q_len * a.group + 255) / 256), a.n_kv_heads, n_seqs);
+    const dim3 grid(a.n_kv_heads, n_seqs, (unsigned)(((long long)max_q_len * a.group + 255) / 256));
     return sandy_launch(prefill_8bit_kernel<CODE, HD>, grid, dim3(THREADS), SMEM, stream, a);
 }
 
@@ -578,7 +579,7 @@ SANDY_API int sandy_prefill_attention_8bit_tc(const SandyAttend8* r, cudaStream_
         return SANDY_ERR_UNSUPPORTED;
     if ((c.head_dim != 64 && c.head_dim != 128) || c.page_size % 16 || c.n_kv_heads < 1 || r->n_heads % c.n_kv_heads) return SANDY_ERR_UNSUPPORTED;
     if (c.page_stride % 16 || (((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)r->q | (uintptr_t)r->out) & 15) || r->ld_q % 8 || r->ld_out % 8 ||
-        r->n_z > 65535 || c.n_kv_heads > 65535 || (long long)r->max_n * (r->n_heads / c.n_kv_heads) > (1 << 28))
+        r->n_z > 65535 || (long long)r->max_n * (r->n_heads / c.n_kv_heads) > 65535 * 256ll)
         return SANDY_ERR_UNSUPPORTED;
     Args a = {};
     a.q = (const bf16*)r->q;

@@ -27,10 +27,10 @@ from typing import Callable, Dict, Hashable, List, Optional, Sequence, Tuple, Un
 
 from .. import core
 from ..cache.pages import RequestIds
-from ..errors import RequestRefused  # noqa: F401  (re-exported)
+from ..errors import RequestRefused, StepError  # noqa: F401  (re-exported)
 from ..models.model import Model, _device_index, load_model
 from ..sampling.params import SamplingParams
-from .step import MAX_BURST, Engine
+from .step import MAX_BURST, Engine, Score  # noqa: F401  (Score: re-exported)
 
 _DTYPES = {"bfloat16": "bfloat16", "bf16": "bfloat16", "float32": "float32", "fp32": "float32"}
 
@@ -177,6 +177,15 @@ class LLM:
     def abort(self, rid: Hashable) -> None:
         self._h.call("abort", rid=self._lib_id[rid])
 
+    def score(self, texts: Union[Sequence[int], Sequence[Sequence[int]]], *, top: int = 0) -> List[Score]:
+        """Log-probabilities of the tokens of one text (a list of ids) or several (a list of lists), with entropies and the `top`
+        likeliest tokens of every place (Engine.score).  Only while no request is waiting or running: a text takes cache pages
+        that the scheduler counts on."""
+        if self.has_work():
+            raise StepError("score: requests are waiting or running")
+        single = len(texts) > 0 and not isinstance(texts[0], (list, tuple))
+        return [self.engine.score(t, top) for t in ([texts] if single else texts)]
+
     # ---- the blocking convenience -----------------------------------------------------------
     def generate(self, prompts: Union[Sequence[int], Sequence[Sequence[int]]], *, max_tokens: int = 16,
                  temperature: float = 0.0, top_p: float = 1.0, top_k: int = 0, seed: Optional[int] = None,
@@ -230,3 +239,6 @@ class _LLMIds:
 
     def known(self, rid: Hashable) -> bool:
         return rid in self._llm._lib_id or self._own.known(rid)
+
+    def forget(self, rid: Hashable) -> None:
+        self._own.forget(rid)

@@ -54,6 +54,15 @@ class SampleRow:
 
 
 @dataclasses.dataclass
+class Score:
+    """What a model says of a text of n tokens (Engine.score).  Entry i of each array is of the distribution that follows tokens[: i + 1]."""
+    logprobs: np.ndarray          # float32 [n - 1]: log-probability of tokens[i + 1]
+    entropies: np.ndarray         # float32 [n], in nats
+    top_ids: np.ndarray           # int32 [n, top], the likeliest first
+    top_logprobs: np.ndarray      # float32 [n, top]
+
+
+@dataclasses.dataclass
 class BurstHandle:
     """A burst of decode steps queued on the device (Engine.decode_burst_async)."""
     n: int                       # steps
@@ -194,6 +203,42 @@ class Engine:
             core.raise_last_error()
         self.synchronize()
         return wrap_device(logits.value, (rows.value, cols.value), 0)
+
+    def score(self, tokens: Sequence[int], top: int = 0, portion: int = 256) -> Score:
+        """Log-probabilities of a text's tokens, each given those before it, with the entropy of every place's distribution and its
+        `top` likeliest tokens (at most 32).  The text runs as a request of its own in steps of `portion` tokens (their logits are
+        workspace memory: portion * vocabulary * 4 bytes) and leaves the cache when it is done."""
+        from ..csrc import ops
+
+        ids = [int(t) for t in tokens]
+        if not ids:
+            raise StepError("a text to score needs at least one token")
+        if portion < 1 or not 0 <= top <= min(ops.MAX_TOP_LOGPROBS, self.vocab_size):
+            raise StepError(f"score: a portion is at least one token, top 0 .. {min(ops.MAX_TOP_LOGPROBS, self.vocab_size)}")
+        rid, got = ("score", object()), []
+        self.admit(rid)
+        try:
+            for at in range(0, len(ids), portion):
+                part = ids[at:at + portion]
+                n = len(part)
+                logits = self.step([StepEntry(rid, part, want=range(n))])
+                self.check_status()                               # a token outside the vocabulary
+                with torch.cuda.device(logits.device):
+                    made = lambda *shape, dtype=torch.float32: torch.empty(*shape, dtype=dtype, device=logits.device)
+                    given = torch.tensor((ids[at + 1:at + n + 1] + [-1])[:n], dtype=torch.int32).to(logits.device)
+                    out = [made(n), made(n), made(n, top, dtype=torch.int32), made(n, top)]
+                    status = torch.zeros(1, dtype=torch.int32, device=logits.device)
+                    ops.token_logprobs(logits, given, out[0], entropy=out[1], top_ids=out[2] if top else None,
+                                       top_logprobs=out[3] if top else None, status=status)
+                    # on the host before the next step writes over the logits
+                    got.append([t.cpu().numpy() for t in out])
+                    if int(status.item()):
+                        raise StepError("the logits of a scored text must not contain NaN")
+        finally:
+            self.release(rid)
+            self.ids.forget(rid)
+        logprobs, entropies, top_ids, top_logprobs = (np.concatenate(parts) for parts in zip(*got))
+        return Score(logprobs[:-1], entropies, top_ids, top_logprobs)
 
     def read_sampled(self, n: int) -> List[int]:
         """The tokens drawn by the last step with `sampling`, on the host.  The step's status words
