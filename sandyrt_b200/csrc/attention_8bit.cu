@@ -11,9 +11,13 @@
 // group), and what the conversion costs (one cvt for two e4m3 codes, five operations for four int8 codes) is paid once for all
 // columns.  The order of dims inside the first product and of keys inside the second is free; it is chosen so that a lane's
 // operands are pieces of rows as they lie in the cache: for K 16 consecutive dims of keys g and g + 8 (g = lane / 4), for V
-// consecutive dims of keys 2t, 2t+1, 2t+8, 2t+9 (t = lane % 4), whose bytes are paired by a byte permutation.  So codes go from
-// memory to registers to the tensor cores, with no shared memory and no barrier between them.  S comes out with keys in the lane
-// groups; movmatrix turns P, as half-precision pairs, into the operand of the second product.
+// consecutive dims of keys 2t, 2t+1, 2t+8, 2t+9 (t = lane % 4), whose bytes are paired by a byte permutation.  S comes out with keys in
+// the lane groups; movmatrix turns P, as half-precision pairs, into the operand of the second product.
+//
+// A warp walks keys of its own: it copies them (cp.async, 16 bytes a lane) into a ring of three stages that no other warp touches, so
+// that there is no barrier before the end.  A row's pieces are exchanged and a tile's keys are taken in an order by which a
+// quarter warp's reads of keys and half a warp's of values meet all banks.  Pages and scales of the next 16 tiles are looked up at
+// once, a run of keys a lane, so that the chain from the block table over the scale to the copy is not walked for every tile.
 //
 // Scales.  A score is S * sk * (2^eq * scale), a factor a key.  A value's scale joins the weight: with M the running maximum of
 // s_j + log2(sv_j) (s in units of log 2), p_j = 2^(s_j - M) is summed for the denominator and p_j * sv_j <= 1 (2 if the scale is
@@ -25,10 +29,16 @@
 // before.  For float32 both are split into two half-precision pieces (22 bits), which lie in neighbouring columns; the two
 // columns' results are in the same lane and are added there.
 //
-// What bounds it.  Single tokens: the codes' bytes.  A warp asks for 64 keys' codes at a time (4 KB of keys and 4 KB of values
-// at heads of 64), so 16 warps an SM keep more than 100 KB on their way; a block's four warps take turns along the keys, and
-// `num_splits` blocks share a request's keys where there are few requests (partial results in scratch, joined by a second
-// kernel in a fixed order).  Prompt portions: the tensor cores' warp-level instructions.
+// The maximum that a column refers to moves only when a score runs ahead of it by more than 2^8 (RESCALE); weights stay below 256.
+//
+// What bounds it.  Single tokens: the codes' bytes.  16 warps an SM (in blocks of four, or two where there are very many) with
+// three stages of 4 KB each keep 190 KB on their way.  Where there are few requests `num_splits` blocks share one's keys: up to 8 are a
+// cluster, whose first block takes the others' results over its shared memory; more leave theirs in scratch, which a second kernel joins
+// in a fixed order.  Measured (e4m3, bfloat16): 8 tokens x 12 heads of 64 behind some 1,000 keys 7.5 us, of which half is the launch, the
+// lookup and the join; 64 x 25 heads behind 64 to 1,000 (int8) 37 us, 2.8 TB/s of codes: blocks of unlike length, 14 us with 64 keys each;
+// behind 8,000 keys each 266 us, 94% of 6.57 TB/s (int8 293); 4 requests of 8 heads of 128, each read by 4, behind 30,000 to 100,000
+// keys 119 us, 81%.
+// Prompt portions: the tensor cores' warp-level instructions; the tcgen05 kernel takes over from 64 query rows on where it can.
 #include <algorithm>
 #include <atomic>
 
@@ -56,9 +66,10 @@ struct Args {
     const float *sink, *out_gate, *dist_bias;
     const void* elem_gate;
     long long ld_q, ld_out, page_stride, scale_stride;
-    int max_blocks, n_rows, n_seqs, n_heads, n_kv_heads, head_dim, page_size, num_pages, num_splits, split_tiles, group, page_shift;    // heads of a key/value head; -1: no power of two
+    int max_blocks, n_rows, max_n, n_seqs, n_heads, n_kv_heads, head_dim, page_size, num_pages, num_splits, split_tiles, group, page_shift;    // heads of a key/value head; -1: no power of two
     int window, keep_first, chunk, n_dist, ld_elem_gate, gate_dim;
     float scale, softcap;
+    bool two_warps;                                                  // blocks of two warps instead of four
     bool in_cluster;                                                 // the splits of a block of queries are a cluster
     bool q_aligned;                                                  // q's rows start on 16 bytes
 };
@@ -134,7 +145,7 @@ __device__ __forceinline__ Portion portion_of(const Args& a, int z) {
     p.row0 = a.q_start ? a.q_start[z] : z;
     p.n = a.q_start ? a.q_start[z + 1] - p.row0 : 1;
     p.before = a.positions[z];
-    if (p.row0 < 0 || p.n > a.n_rows - p.row0) {                     // rows that are not there
+    if (p.row0 < 0 || p.n > a.n_rows - p.row0 || p.n > a.max_n) {    // rows that are not there, or no block is there for
         if (p.n > 0 && a.status && threadIdx.x == 0) atomicOr(a.status, 16);
         p.n = 0;
     }
@@ -198,20 +209,22 @@ __device__ __forceinline__ void lds64(unsigned (&w)[2], uint32_t at) {
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
 }
 
-// ev and inv of a value's scale.  Of one that is not finite ev = 0, so that its weights are NaN and the others stay numbers.
+// ev and inv of a value's scale: log2 of it, but at least -60.  With the 2^-100 of a block of zeros in the reference, weights beside blocks
+// of large values would run out of float's exponents, and be missing in the denominator.  Of a scale that is not finite ev = 0, so
+// that its weights are NaN and the others stay numbers.
 __device__ __forceinline__ unsigned power_of(float vs, float& ev, float& inv) {
     const unsigned bits = __float_as_uint(vs);
-    const int e = (int)(bits >> 23) & 255;
-    ev = e == 255 ? 0.0f : (float)(e - 127);
-    inv = e == 255 ? 1.0f : e == 0 ? 1.7014118e38f : __uint_as_float((unsigned)max(254 - e, 0) << 23);
-    return e == 255 || e == 0 || (bits & 0x807fffffu) ? NO_POWER : 0u;
+    const int biased = (int)(bits >> 23) & 255, e = biased == 255 ? 127 : max(biased, 127 - 60);
+    ev = (float)(e - 127);
+    inv = __uint_as_float((unsigned)max(254 - e, 0) << 23);
+    return bits != (unsigned)e << 23 || biased == 255 ? NO_POWER : 0u;
 }
 
 // WARPS: of a block; DMAX: 64, 128 or 256, the head size rounded up; DK: the head size, or 0 where it is known at run time only; NT: column tiles of
 // 8; KT: key tiles of 16 that a warp takes at a time; RUN: 16 or 8, pages are a multiple of it, so that a tile or half a tile lies in
 // one page; 0: every row is looked up by itself.
 template <typename T, int CODE, int WARPS, int DMAX, int DK, int NT, int KT, int RUN>
-__global__ void __launch_bounds__(WARPS * 32, NT == 1 && DMAX < 256 ? 4 : 1)
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 && DMAX < 256 ? 16 / WARPS : 1)
 attention_8bit_kernel(const __grid_constant__ Args a) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1;            // pieces a number is split into
     constexpr int QT = 8 * NT / P;                       // queries of a block
@@ -245,10 +258,13 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
     // ---- the block's keys, as tiles of 16 positions: kept first ones, then from the first query's first to the last query's own ----
     const int pos_first = at.before + token_of(tile * QT), pos_last = at.before + token_of(tile * QT + n_queries - 1);
     const int lo_first = first_key(a, max(pos_first, 0)), lo_last = first_key(a, max(pos_last, 0));
-    const int kept_tiles = lo_first > 0 ? min((a.keep_first + 15) >> 4, lo_first >> 4) : 0;
+    // positions behind the block table's end have no page: no tile is walked for them, however far they are
+    const long long in_table = (long long)a.max_blocks * ps;
+    const int key_last = (int)min((long long)pos_last, in_table - 1);
+    const int kept_tiles = lo_first > 0 ? min((int)((min((long long)a.keep_first, in_table) + 15) >> 4), lo_first >> 4) : 0;
     const bool request = (unsigned)at.seq < (unsigned)a.n_seqs;
-    if (!request && tid == 0 && a.status) atomicOr(a.status, 16);
-    const int n_tiles = request && pos_last >= 0 ? kept_tiles + (pos_last >> 4) - (lo_first >> 4) + 1 : 0;
+    if ((!request || key_last < pos_last) && tid == 0 && a.status) atomicOr(a.status, 16);
+    const int n_tiles = request && pos_last >= 0 ? kept_tiles + max((key_last >> 4) - (lo_first >> 4) + 1, 0) : 0;
     const int tile_end = split == a.num_splits - 1 ? n_tiles : min(n_tiles, (split + 1) * a.split_tiles);
     const int* table = a.block_table + (size_t)(request ? at.seq : 0) * a.max_blocks;
     const size_t head_at = (size_t)kvh * ps * D;
@@ -712,9 +728,9 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args 
 
 constexpr int MAX_CLUSTER = 8;           // splits up to here join in a cluster, if the blocks are of single tokens' size
 
-// A kernel of four warps with more shared memory than a launch has by itself; the kernel is told so once on each device.
+// A kernel with more shared memory than a launch has by itself; the kernel is told so once on each device.
 template <auto KERNEL>
-int start(const Args& a, dim3 grid, int smem, int most_smem, cudaStream_t stream) {
+int start(const Args& a, dim3 grid, int threads, int smem, int most_smem, cudaStream_t stream) {
     static std::atomic<unsigned long long> told{0};
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
@@ -727,7 +743,7 @@ int start(const Args& a, dim3 grid, int smem, int most_smem, cudaStream_t stream
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -758,32 +774,33 @@ int launch(const Args& a, int n_z, int max_queries, int max_n, cudaStream_t stre
     constexpr int P = sizeof(T) == 4 ? 2 : 1;
     const bool wide = is_wide(max_queries, a.head_dim, sizeof(T) == 4 ? SANDY_F32 : SANDY_BF16);
     int e;
-#define LAUNCH(DMAX, DK, NT, KT, RUN)                                                                                            \
+#define LAUNCH(WARPS, DMAX, DK, NT, KT, RUN)                                                                                     \
     do {                                                                                                                         \
-        constexpr int QT = 8 * NT / P, ring = 4 * stages_of(DMAX, KT) * 2 * KT * 16 * DMAX, sums = 4 * QT * (DMAX + 1) * 4;       \
+        constexpr int QT = 8 * NT / P, ring = WARPS * stages_of(DMAX, KT) * 2 * KT * 16 * DMAX, sums = WARPS * QT * (DMAX + 1) * 4; \
         constexpr int alone = std::max(ring, sums), together = std::max(ring, sums + MAX_CLUSTER * QT * (DMAX + 2) * 4);          \
-        e = start<attention_8bit_kernel<T, CODE, 4, DMAX, DK, NT, KT, RUN>>(                                                     \
-            a, dim3((unsigned)((max_queries + QT - 1) / QT * a.num_splits), a.n_kv_heads, n_z), a.in_cluster ? together : alone,  \
-            NT == 1 ? together : alone, stream);                                                                                 \
+        e = start<attention_8bit_kernel<T, CODE, WARPS, DMAX, DK, NT, KT, RUN>>(                                                 \
+            a, dim3((unsigned)((max_queries + QT - 1) / QT * a.num_splits), a.n_kv_heads, n_z), WARPS * 32,                      \
+            a.in_cluster ? together : alone, NT == 1 ? together : alone, stream);                                                \
     } while (0)
     if (a.page_size % 8 != 0) {                          // rows one by one
-        if (a.head_dim <= 64) LAUNCH(64, 0, 1, 1, 0);
-        else if (a.head_dim <= 128) LAUNCH(128, 0, 1, 1, 0);
-        else LAUNCH(256, 0, 1, 1, 0);
+        if (a.head_dim <= 64) LAUNCH(4, 64, 0, 1, 1, 0);
+        else if (a.head_dim <= 128) LAUNCH(4, 128, 0, 1, 1, 0);
+        else LAUNCH(4, 256, 0, 1, 1, 0);
     } else if (a.page_size % 16 == 0 && a.head_dim == 64) {
-        if (wide) LAUNCH(64, 64, 4, 1, 16);
-        else LAUNCH(64, 64, 1, 2, 16);
+        if (wide) LAUNCH(4, 64, 64, 4, 1, 16);
+        else if (a.two_warps) LAUNCH(2, 64, 64, 1, 2, 16);
+        else LAUNCH(4, 64, 64, 1, 2, 16);
     } else if (a.page_size % 16 == 0 && a.head_dim == 128) {
-        if (wide) LAUNCH(128, 128, 2, 1, 16);
-        else LAUNCH(128, 128, 1, 1, 16);
+        if (wide) LAUNCH(4, 128, 128, 2, 1, 16);
+        else LAUNCH(4, 128, 128, 1, 1, 16);
     } else if (a.head_dim <= 64) {
-        if (wide) LAUNCH(64, 0, 4, 1, 8);
-        else LAUNCH(64, 0, 1, 2, 8);
+        if (wide) LAUNCH(4, 64, 0, 4, 1, 8);
+        else LAUNCH(4, 64, 0, 1, 2, 8);
     } else if (a.head_dim <= 128) {
-        if (wide) LAUNCH(128, 0, 2, 1, 8);
-        else LAUNCH(128, 0, 1, 1, 8);
+        if (wide) LAUNCH(4, 128, 0, 2, 1, 8);
+        else LAUNCH(4, 128, 0, 1, 1, 8);
     } else {
-        LAUNCH(256, 0, 1, 1, 8);
+        LAUNCH(4, 256, 0, 1, 1, 8);
     }
 #undef LAUNCH
     if (e != SANDY_OK || a.num_splits == 1 || a.in_cluster) return e;
@@ -858,6 +875,7 @@ SANDY_API int sandy_attention_8bit(const SandyAttend8* r, cudaStream_t stream) {
     a.scale_stride = c.scale_stride;
     a.max_blocks = c.max_blocks;
     a.n_rows = r->n_rows;
+    a.max_n = r->max_n;
     a.n_seqs = c.n_seqs;
     a.n_heads = r->n_heads;
     a.n_kv_heads = c.n_kv_heads;
@@ -878,6 +896,11 @@ SANDY_API int sandy_attention_8bit(const SandyAttend8* r, cudaStream_t stream) {
     a.scale = r->scale;
     a.softcap = rules.softcap;
     a.in_cluster = in_cluster;
+    // Blocks by the thousand, one for a (token, key/value head): what a block does before its keys and after them is paid once a warp, and
+    // other blocks are there to hide the copies' latency.  256 tokens x 12 heads of 64 with 300 keys: 38 us in blocks of two warps,
+    // 48 in blocks of four; 256 x 25 with 1,000 keys: 162 and 178.  Below four rounds of blocks the longest ones are left alone at the
+    // end: 64 x 25 with 2,000 keys: 93 and 86; 32 x 12 with 1,000: 28 and 19.  Heads of 128 (256 x 8): 79 and 74.
+    a.two_warps = r->num_splits == 1 && !r->q_start && (long long)r->n_z * c.n_kv_heads >= 16ll * sandy_sm_count();
     a.q_aligned = (((uintptr_t)r->q | (uintptr_t)(r->ld_q * es)) & 15) == 0;
     if (c.dtype == SANDY_F32 && c.code == SANDY_E4M3) return launch<float, SANDY_E4M3>(a, r->n_z, (int)queries, r->max_n, stream);
     if (c.dtype == SANDY_F32 && c.code == SANDY_INT8) return launch<float, SANDY_INT8>(a, r->n_z, (int)queries, r->max_n, stream);

@@ -53,7 +53,7 @@ struct Args {
     const float *sink, *out_gate;
     const bf16* elem_gate;
     long long ld_q, ld_out, page_stride, scale_stride;
-    int max_blocks, n_rows, n_heads, n_kv_heads, group, page_size, page_shift, num_pages;
+    int max_blocks, n_rows, max_n, n_heads, n_kv_heads, group, page_size, page_shift, num_pages;
     int window, keep_first, chunk, ld_elem_gate, gate_dim;
     float scale, softcap;
 };
@@ -133,7 +133,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
     extern __shared__ uint8_t smem_raw[];
     __shared__ RunConsts s_consts[CONSTS][BN / 16];
     __shared__ long long s_off[CONSTS][BN / 16];         // where a run's rows lie in keys and values (page 0's, if nowhere)
-    __shared__ unsigned s_good[CONSTS];                  // the tile's runs that have a page, a bit each
+    __shared__ unsigned s_runs[CONSTS];                  // the tile's runs: bit i, it has a page; bit 8 + i, its values' scale is not 2^ev
+    __shared__ float s_rest[CONSTS][BN / 16];            // of these: the scale over 2^ev
     __shared__ uint64_t q_ready[2], first_k, k_empty[STAGES], v_empty[STAGES], s_full[2], go[2][2], o_full[2], c_full[CONSTS];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int s_failed;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
     // tiles in the slowest dimension: all requests' blocks with the most keys start first, and what is left for the end is small
     const int z = blockIdx.y, kvh = blockIdx.x, nth = blockIdx.z;
     const int row0 = a.q_start[z], n = a.q_start[z + 1] - row0, before = a.kv_before[z];
-    const bool there = row0 >= 0 && n <= a.n_rows - row0;            // the portion's rows
+    const bool there = row0 >= 0 && n <= a.n_rows - row0 && n <= a.max_n;      // the portion's rows, and blocks for them
     if (!there && n > 0 && threadIdx.x == 0 && a.status) atomicOr(a.status, 16);
     const int tiles = there && n > 0 ? (int)(((long long)n * a.group + 255) / 256) : 0;
     if (nth >= tiles) return;
@@ -157,9 +158,13 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
         return lo;
     };
     const int lo_first = first_key(max(pos_first, 0)), lo_last = first_key(max(pos_last, 0));
+    // positions behind the block table's end have no page: no tile is walked for them, however far they are
+    const long long in_table = (long long)a.max_blocks * a.page_size;
+    const int key_last = (int)min((long long)pos_last, in_table - 1);
+    if (key_last < pos_last && threadIdx.x == 0 && a.status) atomicOr(a.status, 16);
     const int kt_window = lo_first / BN;
-    const int kept_tiles = lo_first > 0 ? min((a.keep_first + BN - 1) / BN, kt_window) : 0;
-    const int n_it = pos_last >= 0 ? kept_tiles + pos_last / BN - kt_window + 1 : 0;
+    const int kept_tiles = lo_first > 0 ? min((int)((min((long long)a.keep_first, in_table) + BN - 1) / BN), kt_window) : 0;
+    const int n_it = pos_last >= 0 ? kept_tiles + max(key_last / BN - kt_window + 1, 0) : 0;
     auto first_of = [&](int t) { return (t < kept_tiles ? t : t - kept_tiles + kt_window) * BN; };
     const int tid = threadIdx.x, warp = tid >> 5;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -388,7 +393,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
         auto look_up = [&](int it) {
             if (p >= BN / 16 || it >= n_it) return;
             const int j = first_of(it) + 16 * p;
-            bool good = false;
+            bool good = false, odd = false;
             RunConsts c = {0.0f, -INFINITY, 0.0f, 0.0f};             // keys of no page weigh nothing
             long long off = 0;
             if (j <= pos_last && (j + 15 >= lo_first || j < a.keep_first)) {
@@ -399,14 +404,12 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                     off = page * a.page_stride + ((long long)kvh * a.page_size + (j - b * a.page_size)) * HD;
                     const float vs = a.v_scale[(size_t)page * a.scale_stride + kvh];
                     c.ks = a.k_scale[(size_t)page * a.scale_stride + kvh];
-                    const int e = (int)(__float_as_uint(vs) >> 23) & 255;
-                    c.ev = (float)(e - 127);
+                    const int biased = (int)(__float_as_uint(vs) >> 23) & 255, e = biased == 255 ? 127 : max(biased, 127 - 60);
+                    c.ev = (float)(e - 127);                         // at least -60: see attention_8bit.cu
                     c.inv = __uint_as_float((unsigned)max(254 - e, 0) << 23);
-                    if (e == 255) {
-                        c.ks = __uint_as_float(0x7fffffffu);
-                        c.ev = 0.0f;
-                        c.inv = 1.0f;
-                    }
+                    if (biased == 255) c.ks = __uint_as_float(0x7fffffffu);
+                    else odd = __float_as_uint(vs) != (unsigned)e << 23;
+                    s_rest[it % CONSTS][p] = vs * c.inv;
                 } else if (a.status) {
                     atomicOr(a.status, 16);
                 }
@@ -414,7 +417,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             s_consts[it % CONSTS][p] = c;
             s_off[it % CONSTS][p] = off;
             const unsigned all = __ballot_sync(0xffu, good);
-            if (p == 0) s_good[it % CONSTS] = all;
+            const unsigned odds = __ballot_sync(0xffu, odd);
+            if (p == 0) s_runs[it % CONSTS] = all | odds << 8;
             mbar_arrive(&c_full[it % CONSTS]);
         };
         // A thread's pieces of a tile; bit i of the result: piece i is one that counts.  The others are read from where something is, so
@@ -422,7 +426,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
         auto load = [&](const uint8_t* from, int it, uint4 (&w)[EACH]) {
             if (it >= n_it) return 0u;
             const int j0 = first_of(it), at = it % CONSTS;
-            const unsigned good = s_good[at];
+            const unsigned good = s_runs[at] & 0xff;
             unsigned counts = (1u << EACH) - 1;
             if (good != 0xff || j0 + BN - 1 > pos_last || j0 < lo_first) {       // not every key has a page and is seen by a query
 #pragma unroll
@@ -458,6 +462,25 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                 sts128(at + ((((c & 7) + 1) ^ (row & 7)) << 4), x[4], x[5], x[6], x[7]);
             }
         };
+        // Values whose scale is not a power of two, as appending gives them: what is left of it, once more over what this thread has
+        // stored, so that the ordinary way carries no test for it (in `store` it cost 5%, here 1.5%).
+        auto multiply = [&](uint32_t to, unsigned odd, const float* rest) {
+#pragma unroll 1
+            for (int i = 0; i < 2 * EACH; i++) {
+                const int row = (i >> 1) * STEP + my_row, c = 2 * piece;
+                if (!((odd >> (row >> 4)) & 1)) continue;
+                const uint32_t at = to + (c >> 3) * HALF_TILE + row * 128 + ((((c & 7) + (i & 1)) ^ (row & 7)) << 4);
+                const __half2 f = __float2half2_rn(rest[row >> 4]);
+                uint32_t x[4];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[e]), f);
+                    x[e] = *reinterpret_cast<const uint32_t*>(&y);
+                }
+                sts128(at, x[0], x[1], x[2], x[3]);
+            }
+        };
         uint4 kw[EACH], vw[EACH];
         look_up(0);
         look_up(1);
@@ -480,6 +503,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             k_counts = load(a.k, it + 1, kw);
             if (it >= STAGES) wait_for(&v_empty[stage], (it / STAGES - 1) & 1);
             store(base + OFF_V + stage * KV_BYTES, vw, v_counts);
+            const unsigned odd = s_runs[it % CONSTS] >> 8;
+            if (odd) multiply(base + OFF_V + stage * KV_BYTES, odd, s_rest[it % CONSTS]);
             fence_async_proxy();
             for (int g = 0; g < groups; g++) {
                 warp_arrive(&go[g][it & 1]);
@@ -565,7 +590,7 @@ int launch(const Args& a, int n_seqs, int max_q_len, cudaStream_t stream) {
 
 // Prompt portions as sandy_attention_8bit (attention_8bit.cu) takes them, without splits.  bfloat16, heads of 64 and 128, pages of a multiple
 // of 16 keys, rows of q and out on 16 bytes, a positive scale, no bias by distance; SANDY_ERR_UNSUPPORTED for everything else, which the
-// other kernel takes.  The scales of values are powers of two here (what appending gives), or not finite.
+// other kernel takes.
 SANDY_API int sandy_prefill_attention_8bit_tc(const SandyAttend8* r, cudaStream_t stream) {
     if (!r) return SANDY_ERR_ARGUMENT;
     const SandyCache8& c = r->cache;
@@ -601,6 +626,7 @@ SANDY_API int sandy_prefill_attention_8bit_tc(const SandyAttend8* r, cudaStream_
     a.scale_stride = c.scale_stride;
     a.max_blocks = c.max_blocks;
     a.n_rows = r->n_rows;
+    a.max_n = r->max_n;
     a.n_heads = r->n_heads;
     a.n_kv_heads = c.n_kv_heads;
     a.group = r->n_heads / c.n_kv_heads;

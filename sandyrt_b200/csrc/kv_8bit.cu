@@ -100,14 +100,15 @@ __global__ void __launch_bounds__(WARPS * 32)
 append_kernel(const T* __restrict__ k_src, const T* __restrict__ v_src, long long ld_k, long long ld_v, Planes cache,
               const int* __restrict__ block_table, int max_blocks, const int* __restrict__ q_start,
               const int* __restrict__ kv_before, int n_rows, int n_kv_heads, int head_dim, int page_size, int num_pages,
-              int page_shift, int row_shift, int* __restrict__ status) {
+              int page_shift, int row_shift, int max_len, int* __restrict__ status) {
     pdl_launch_dependents();
     pdl_wait();
     const int s = blockIdx.z, nth = blockIdx.x;                     // which of the request's touched pages
     const int unit = blockIdx.y * WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int first_row = q_start[s], n = q_start[s + 1] - first_row, before = kv_before[s];
     if (unit >= 2 * n_kv_heads || n <= 0) return;
-    if (first_row < 0 || n > n_rows - first_row) {                  // rows that are not there
+    // rows that are not there, or more than max_len said: then there may be no block for the last pages
+    if (first_row < 0 || n > n_rows - first_row || n > max_len) {
         if (lane == 0 && status) atomicOr(status, 8);
         return;
     }
@@ -216,14 +217,14 @@ template <typename T, int CODE>
 __global__ void __launch_bounds__(READ_THREADS)
 read_kernel(Planes cache, const int* __restrict__ block_table, int max_blocks, const int* __restrict__ first,
             const int* __restrict__ out_start, T* __restrict__ k_out, T* __restrict__ v_out, long long ld_k, long long ld_v,
-            int n_rows, int n_kv_heads, int head_dim, int page_size, int num_pages, bool aligned, int* __restrict__ status) {
+            int n_rows, int max_len, int n_kv_heads, int head_dim, int page_size, int num_pages, bool aligned, int* __restrict__ status) {
     pdl_launch_dependents();
     pdl_wait();
     const int s = blockIdx.y;
     const int row0 = out_start[s], n = out_start[s + 1] - row0, from = first[s];
     const int r0 = blockIdx.x * READ_ROWS, rows = min(READ_ROWS, n - r0);
     if (rows <= 0) return;
-    if (row0 < 0 || n > n_rows - row0) {                            // rows that are not there
+    if (row0 < 0 || n > n_rows - row0 || n > max_len) {             // rows that are not there, or more than max_len said
         if (threadIdx.x == 0 && status) atomicOr(status, 16);
         return;
     }
@@ -281,7 +282,7 @@ SANDY_API int sandy_kv_append_8bit(const SandyRows8* r, cudaStream_t stream) {
     return sandy_launch(on_16_bytes<T>(*r) ? append_kernel<T, CODE, true> : append_kernel<T, CODE, false>, grid, block, 0, stream, \
                         (const T*)r->k_rows, (const T*)r->v_rows, r->ld_k, r->ld_v, cache, c.block_table, c.max_blocks, r->start, \
                         r->first, r->n_rows, c.n_kv_heads, c.head_dim, c.page_size, c.num_pages, shift(c.page_size), \
-                        shift(c.head_dim / 8), c.status)
+                        shift(c.head_dim / 8), r->max_len, c.status)
     if (c.dtype == SANDY_F32 && c.code == SANDY_E4M3) APPEND(float, SANDY_E4M3);
     if (c.dtype == SANDY_F32 && c.code == SANDY_INT8) APPEND(float, SANDY_INT8);
     if (c.dtype == SANDY_BF16 && c.code == SANDY_E4M3) APPEND(bf16, SANDY_E4M3);
@@ -300,7 +301,7 @@ SANDY_API int sandy_kv_read_8bit(const SandyRows8* r, cudaStream_t stream) {
     const dim3 grid((r->max_len - 1) / READ_ROWS + 1, c.n_seqs), block(READ_THREADS);
 #define READ(T, CODE)                                                                                                           \
     return sandy_launch(read_kernel<T, CODE>, grid, block, 0, stream, cache, c.block_table, c.max_blocks, r->first, r->start,    \
-                        (T*)r->k_rows, (T*)r->v_rows, r->ld_k, r->ld_v, r->n_rows, c.n_kv_heads, c.head_dim, c.page_size,        \
+                        (T*)r->k_rows, (T*)r->v_rows, r->ld_k, r->ld_v, r->n_rows, r->max_len, c.n_kv_heads, c.head_dim, c.page_size, \
                         c.num_pages, on_16_bytes<T>(*r), c.status)
     if (c.dtype == SANDY_F32 && c.code == SANDY_E4M3) READ(float, SANDY_E4M3);
     if (c.dtype == SANDY_F32 && c.code == SANDY_INT8) READ(float, SANDY_INT8);

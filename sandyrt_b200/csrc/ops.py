@@ -547,6 +547,7 @@ def _status_word(index: int) -> int:
         if torch.cuda.is_current_stream_capturing():
             raise KernelError("the device's status word is made by its first kernel call; call once before capturing a graph")
         t = kernel_status(torch.device("cuda", index))
+        torch.cuda.synchronize(index)                   # it is zeros before a kernel of whichever stream raises a bit
     return t.data_ptr()
 
 
@@ -662,14 +663,16 @@ def kv_append_8bit(k_src, v_src, cache: Cache8, block_table, q_start, kv_before,
     kv_before[s] on (int32 [S]); max_q_len: the most that one request brings.  A block's scale is the smallest power of two by
     which its largest value fits the code; a block that held earlier positions keeps its scale or, where the new values need a
     larger one, has its earlier codes rounded again.  A block that is given a value that is not finite gets a scale of NaN.
-    Requests must not share a page that they write.  Rows in front of the first request and behind the last one are not read."""
+    Requests must not share a page that they write.  Rows in front of the first request and behind the last one are not read.  A request
+    that brings more rows than max_q_len, or rows that are not there, or positions without a page, is reported (check_kernel_status) and
+    not written.  The first call on a device must not be a recorded one."""
     _rows_call8("kv_append_8bit", "sandy_kv_append_8bit", cache, k_src, v_src, block_table, q_start, kv_before, max_q_len, "max_q_len")
 
 
 def kv_read_8bit(cache: Cache8, block_table, first, out_start, k_out, v_out, *, max_len: int) -> None:
     """Cached rows back as numbers: rows out_start[s] .. out_start[s + 1] - 1 (int32 [S + 1]) of k_out and v_out ([N, Hkv * D], float32
     or bfloat16, a row pitch each) become positions first[s] on (int32 [S]) of the block table's request s; max_len: the
-    most rows of one request.  Exact in both types.  Rows of no request, and of positions without a page, are left as they were."""
+    most rows of one request.  Exact in both types.  Rows of no request, and of positions without a page (reported), are left as they were."""
     _rows_call8("kv_read_8bit", "sandy_kv_read_8bit", cache, k_out, v_out, block_table, out_start, first, max_len, "max_len")
 
 
@@ -774,7 +777,8 @@ def decode_attention_8bit(q, cache: Cache8, block_table, token_seq, positions, o
     token_seq[t] at positions[t] (int32 [T]) sees that request's cached positions up to its own, which kv_append_8bit has written.
     Head sizes 16..256 in steps of 16, any page size.  num_splits: blocks that share a request's keys (0: the kernel's choice).
     rules: window, keep_first, softcap, chunk, sink, out_gate, dist_bias, elem_gate as in paged_attention.  A token at a negative
-    position (a padded one) or of no visible key gets zeros."""
+    position (a padded one), of no visible key or with scores of minus infinity alone gets zeros; a visible key without a page is
+    reported (check_kernel_status) and left out."""
     what, T = "decode_attention_8bit", q.shape[0]
     width = _tokens8(what, T, _layout(block_table), _layout(token_seq), _layout(positions))
     _attention_8bit(what, q, cache, block_table, width, token_seq, positions, None, out, T, 1, n_heads, scale, num_splits, False, rules)

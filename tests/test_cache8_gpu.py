@@ -307,6 +307,14 @@ def test_single_tokens(code, dtype, H, hkv, d, ps):
     _check_attention(code, dtype, H, hkv, d, ps, [(0, 1), (1, 1), (15, 1), (16, 1), (63, 1), (130, 1), (257, 1), (700, 1)], True)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("code", list(CODES))
+@pytest.mark.parametrize("hkv,group,rules", [(25, 1, {}), (25, 4, dict(window=20, keep_first=3, sink=True))])
+def test_single_tokens_of_very_many_requests(code, dtype, hkv, group, rules):
+    """Thousands of (token, key/value head) pairs: blocks of two warps."""
+    _check_attention(code, dtype, hkv * group, hkv, 64, 16, [((7 * i) % 90 if i % 9 else 0, 1) for i in range(100)], True, **rules)
+
+
 @pytest.mark.parametrize("splits", [1, 2, 3, 7, 16, 40])
 def test_single_tokens_in_so_many_splits(splits):
     _check_attention("e4m3", "bf16", 6, 2, 64, 16, [(0, 1), (300, 1), (511, 1), (640, 1)], True, splits=splits)
@@ -409,6 +417,102 @@ def test_values_of_blocks_far_apart_in_size(dtype, decode):
         # P is a half-precision number beside its largest term: what is 2^-25 below that is gone
         tol = tol + (w[:, None] * vv[:p + 1, 0].abs().amax(1, keepdim=True)).max() * 2.0 ** -18
         assert bool(((out[i].cpu().double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("path", ["decode", "prompt", "tcgen05"])
+@pytest.mark.parametrize("code", list(CODES))
+@pytest.mark.parametrize("kind", ["any numbers", "zeros", "zeros beside large ones"])
+def test_scales_that_are_no_power_of_two(code, path, kind):
+    """Scales as another program might have them: any numbers, zero for a block of zeros.  And blocks of zeros (2^-100 by appending) beside
+    values of 2^50, whose weights must not be missing in the denominator."""
+    from sandyrt_b200.csrc import ops
+
+    rng = np.random.default_rng(17)
+    hkv, d, ps, H, n = 2, 64, 16, 4, 150
+    lists, table, pages = _tables(rng, [-(-n // ps)])
+    plain = PlainCache(pages, hkv, ps, d, CODES[code])
+    k, v = (_values(rng, n, hkv, d, torch.float64) for _ in range(2))
+    if kind != "any numbers":
+        k[32:48], v[64:80], v[96:112] = 0.0, 0.0, 0.0
+    if kind == "zeros beside large ones":
+        v[16:32] *= 2.0 ** 50
+        k[16:32] = 0.0
+        k[16:32, :, 0] = -20.0                                   # 20 below the others: a weight of e^-20 on values of 2^50
+    plain.append(k, v, lists, [0, n], [0])
+    if kind != "zeros beside large ones":
+        for w in range(2):
+            plain.scales[w] = (plain.scales[w] * torch.from_numpy(rng.uniform(0.6, 1.7, plain.scales[w].shape))).float().double()
+            plain.scales[w] = torch.where(plain.scales[w] < 2.0 ** -90, torch.zeros(()).double(), plain.scales[w])
+    dev = _device_cache(plain)
+    q = torch.from_numpy(rng.standard_normal((n, H, d)))
+    q[:, :, 0] = 8.0
+    q = q.to(torch.bfloat16).reshape(n, -1)
+    out = torch.empty(n, H * d, dtype=torch.bfloat16, device=DEV)
+    if path == "decode":
+        ops.decode_attention_8bit(q.to(DEV), dev, table, _i32([0] * n), _i32(list(range(n))), out, n_heads=H, scale=0.125)
+    else:
+        ops.prefill_attention_8bit(q.to(DEV), dev, table, _i32([0, n]), _i32([0]), out, n_heads=H, max_q_len=n, scale=0.125, tc=path == "tcgen05")
+    ops.check_kernel_status(DEV)
+    kk, vv = (plain.values(w, lists[0], n) for w in range(2))
+    qq = q.double().reshape(n, H, d)
+    want = attention(qq, kk, vv, list(range(n)), scale=0.125)
+    # a sum of terms, each off by 2^-11 twice (the weight, and a value times what its scale is beside a power of two); weights below 2^-25
+    # of the largest term are gone
+    far = attention(qq, kk, vv.abs(), list(range(n)), scale=0.125)
+    tol = want.abs() * 2.0 ** -8 + far * 2.0 ** -9 + far.amax(dim=2, keepdim=True) * 2.0 ** -16
+    assert bool(((out.cpu().double().reshape(n, H, d) - want).abs() <= tol).all())
+
+
+def test_positions_behind_the_block_table():
+    """Far behind: reported, and nothing is walked for them.  A longest portion that was said too short is reported too."""
+    from sandyrt_b200.csrc import ops
+    from sandyrt_b200.errors import KernelError
+
+    rng = np.random.default_rng(3)
+    hkv, d, ps, H = 2, 64, 16, 4
+    plain, lists, table = _filled(rng, "e4m3", hkv, d, ps, [64])
+    dev = _device_cache(plain)
+    q = torch.randn(4, H * d, device=DEV)
+    want, got = torch.empty_like(q), torch.empty_like(q)
+    ops.decode_attention_8bit(q, dev, table, _i32([0] * 4), _i32([63] * 4), want, n_heads=H, scale=0.1)
+    ops.check_kernel_status(DEV)
+    ops.decode_attention_8bit(q, dev, table, _i32([0] * 4), _i32([64, 1000, 2 ** 31 - 17, 2 ** 30]), got, n_heads=H, scale=0.1)
+    with pytest.raises(KernelError, match="status 16"):
+        ops.check_kernel_status(DEV)
+    assert torch.equal(got, want)
+    for rules in (dict(window=30), dict(window=30, keep_first=2 ** 30), dict(window=30, keep_first=40)):
+        ops.decode_attention_8bit(q, dev, table, _i32([0] * 4), _i32([2 ** 31 - 17] * 4), got, n_heads=H, scale=0.1, **rules)
+        with pytest.raises(KernelError, match="status 16"):
+            ops.check_kernel_status(DEV)
+        assert bool((got == 0).all()) if "keep_first" not in rules else bool(torch.isfinite(got).all())
+    b = q.to(torch.bfloat16)
+    for tc in (True, False):
+        outs = []
+        for before in (60, 2 ** 31 - 40):                        # rows at 60..63, and far behind
+            o = torch.full_like(b, 3.0)
+            ops.prefill_attention_8bit(b, dev, table, _i32([0, 4]), _i32([before]), o, n_heads=H, max_q_len=4, scale=0.1, tc=tc)
+            if before > 60:
+                with pytest.raises(KernelError, match="status 16"):
+                    ops.check_kernel_status(DEV)
+            ops.check_kernel_status(DEV)
+            outs.append(o)
+        assert bool(torch.isfinite(outs[0]).all()) and bool(torch.isfinite(outs[1]).all())
+        o = torch.full_like(b, 3.0)
+        ops.prefill_attention_8bit(b, dev, table, _i32([0, 4]), _i32([60]), o, n_heads=H, max_q_len=3, scale=0.1, tc=tc)
+        with pytest.raises(KernelError, match="status 16"):
+            ops.check_kernel_status(DEV)
+        assert bool((o == 3).all())
+    was = _bits(dev)
+    rows = torch.randn(4, hkv * d, device=DEV)
+    ops.kv_append_8bit(rows, rows, dev, table, _i32([0, 4]), _i32([0]), max_q_len=3)
+    with pytest.raises(KernelError, match="status 8"):
+        ops.check_kernel_status(DEV)
+    assert all(torch.equal(a, c) for a, c in zip(was, _bits(dev)))
+    k, v = torch.full_like(rows, 3.0), torch.full_like(rows, 3.0)
+    ops.kv_read_8bit(dev, table, _i32([0]), _i32([0, 4]), k, v, max_len=3)
+    with pytest.raises(KernelError, match="status 16"):
+        ops.check_kernel_status(DEV)
+    assert bool((k == 3).all()) and bool((v == 3).all())
 
 
 @pytest.mark.parametrize("code", list(CODES))
