@@ -21,7 +21,11 @@
 //
 // What bounds it: 32,768 exponentials a pair of tiles are 2,048 cycles of the special-function units, the products at heads of 128
 // as much of the tensor cores; converting 32,768 codes is some 700 (int8) issue slots of each SM quarter.  256 rows a block halve the
-// conversion's share and the reads of the cache.  One block an SM (213 KB of shared memory at heads of 128).
+// conversion's share and the reads of the cache.  One block an SM (193 KB of shared memory at heads of 128).
+// Measured: 2,048 tokens behind 6,000, 32 heads of 128 reading 8 (int8): 307 us, 46% of the 1.67 PFLOP/s that a matrix product gets;
+// four prompts of 500 to 950 tokens, 12 heads of 64 (e4m3): 39 us.  A pair of tiles takes some 5,000 cycles: what a tile waits for is the
+// chain of its softmax (reading, exponentials, writing), the issuing warp's wake-up and the products, of which the two tiles overlap
+// about half; and 256 blocks on 148 SMs are two rounds.  Blocks with the most keys start first, over all requests.
 //
 // Every wait on an mbarrier is bounded; one that runs out raises bit 8 of the status word and the block ends without waiting again.
 #include <atomic>

@@ -778,7 +778,8 @@ def decode_attention_8bit(q, cache: Cache8, block_table, token_seq, positions, o
     Head sizes 16..256 in steps of 16, any page size.  num_splits: blocks that share a request's keys (0: the kernel's choice).
     rules: window, keep_first, softcap, chunk, sink, out_gate, dist_bias, elem_gate as in paged_attention.  A token at a negative
     position (a padded one), of no visible key or with scores of minus infinity alone gets zeros; a visible key without a page is
-    reported (check_kernel_status) and left out."""
+    reported (check_kernel_status) and left out.  Values of a block whose largest is below 2^-53 (in magnitude) count with fewer bits,
+    below 2^-77 as zeros."""
     what, T = "decode_attention_8bit", q.shape[0]
     width = _tokens8(what, T, _layout(block_table), _layout(token_seq), _layout(positions))
     _attention_8bit(what, q, cache, block_table, width, token_seq, positions, None, out, T, 1, n_heads, scale, num_splits, False, rules)
