@@ -111,8 +111,8 @@ append_kernel(const T* __restrict__ k_src, const T* __restrict__ v_src, long lon
     const int unit = blockIdx.y * WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int first_row = q_start[s], n = q_start[s + 1] - first_row, before = kv_before[s];
     if (unit >= 2 * n_kv_heads || n <= 0) return;
-    // rows that are not there, or more than max_len said: then there may be no block for the last pages
-    if (first_row < 0 || n > n_rows - first_row || n > max_len) {
+    // rows that are not there, or more than max_len said: then there may be no block for the last pages; positions that are no int
+    if (first_row < 0 || n > n_rows - first_row || n > max_len || (long long)before + n + page_size > 0x7fffffffll) {
         if (lane == 0 && status) atomicOr(status, 8);
         return;
     }

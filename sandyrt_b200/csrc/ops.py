@@ -647,8 +647,8 @@ def _rows_call8(what: str, name: str, cache: Cache8, k_rows, v_rows, block_table
     at, (pitch, hkv, d, ps, pages, code) = _cache8(what, cache)
     ld, n_rows, dtype = _rows8(what, hkv, d, _layout(k_rows), _layout(v_rows))
     S, width = _requests8(what, _layout(block_table), _layout(starts), _layout(firsts))
-    if max_len < 0:
-        raise KernelError(f"{what}: {longest} is negative")
+    if not 0 <= max_len < 1 << 31:
+        raise KernelError(f"{what}: {longest} is negative or no 32-bit number")
     index = _one_device(what, k_rows, v_rows, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, starts, firsts)
     if S == 0 or max_len == 0 or n_rows == 0:
         return
@@ -795,8 +795,8 @@ def prefill_attention_8bit(q, cache: Cache8, block_table, q_start, kv_before, ou
     mma.sync one, None picks; num_splits is the latter's."""
     what = "prefill_attention_8bit"
     S, width = _requests8(what, _layout(block_table), _layout(q_start), _layout(kv_before))
-    if max_q_len < 0:
-        raise KernelError(f"{what}: max_q_len is negative")
+    if not 0 <= max_q_len < 1 << 31:
+        raise KernelError(f"{what}: max_q_len is negative or no 32-bit number")
     _attention_8bit(what, q, cache, block_table, width, None, kv_before, q_start, out, S, max_q_len, n_heads, scale, num_splits, tc, rules)
 
 

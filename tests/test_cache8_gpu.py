@@ -515,6 +515,31 @@ def test_positions_behind_the_block_table():
     assert bool((k == 3).all()) and bool((v == 3).all())
 
 
+def test_appending_at_the_last_positions_there_are():
+    """Positions up to and past 2^31: no page, reported, nothing written."""
+    from sandyrt_b200.csrc import ops
+    from sandyrt_b200.errors import KernelError
+
+    for ps in (16, 5):
+        plain, lists, table = _filled(np.random.default_rng(4), "int8", 2, 64, ps, [20])
+        dev = _device_cache(plain)
+        was, rows = _bits(dev), torch.randn(4, 128, device=DEV)
+        for before in (2 ** 31 - 1, 2 ** 31 - 3, 2 ** 31 - 20, 2 ** 31 - 200, -1, -2 ** 31):
+            ops.kv_append_8bit(rows, rows, dev, table, _i32([0, 4]), _i32([before]), max_q_len=4)
+            with pytest.raises(KernelError, match="status 8"):
+                ops.check_kernel_status(DEV)
+            if before != -1:                                         # its second row would be position 0
+                out = torch.full_like(rows, 3.0)
+                ops.kv_read_8bit(dev, table, _i32([before]), _i32([0, 2]), out, out.clone(), max_len=2)
+                with pytest.raises(KernelError, match="status 16"):
+                    ops.check_kernel_status(DEV)
+                assert bool((out == 3).all())
+        with pytest.raises(KernelError, match="32-bit"):
+            ops.kv_append_8bit(rows, rows, dev, table, _i32([0, 4]), _i32([0]), max_q_len=2 ** 31)
+        ops.check_kernel_status(DEV)
+        assert all(torch.equal(x, y) for x, y in zip(was, _bits(dev)))
+
+
 @pytest.mark.parametrize("code", list(CODES))
 @pytest.mark.parametrize("decode", [True, False])
 def test_blocks_that_are_not_finite(code, decode):
