@@ -28,11 +28,16 @@
 // about half; and 256 blocks on 148 SMs are two rounds.  Blocks with the most keys start first, over all requests.
 //
 // Every wait on an mbarrier is bounded; one that runs out raises bit 8 of the status word and the block ends without waiting again.
+#include <algorithm>
 #include <atomic>
+
+#include <cooperative_groups.h>
 
 #include "cache8.h"
 #include "kv_8bit.cuh"
 #include "tcgen05.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -40,6 +45,7 @@ constexpr int BN = 128;                  // keys of a tile
 constexpr int THREADS = 416;
 constexpr int FIRST_PRODUCER = 256, ISSUE_WARP = 12;
 constexpr int STAGES = 2;
+constexpr int SPLIT_ROOM = 1;            // rounds of blocks that splits of the keys may make
 constexpr int CONSTS = 8;                // key tiles whose scales and pages are kept
 constexpr float RESCALE = 8.0f;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -58,7 +64,7 @@ struct Args {
     const bf16* elem_gate;
     long long ld_q, ld_out, page_stride, scale_stride;
     int max_blocks, n_rows, max_n, n_heads, n_kv_heads, group, page_size, page_shift, num_pages;
-    int window, keep_first, chunk, ld_elem_gate, gate_dim;
+    int window, keep_first, chunk, ld_elem_gate, gate_dim, splits;
     float scale, softcap;
 };
 
@@ -126,7 +132,8 @@ __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-template <int CODE, int HD>
+// SPLIT: a cluster of a.splits blocks shares a block's rows, each with a run of their key tiles.
+template <int CODE, int HD, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_constant__ Args a) {
     constexpr int SUBS = HD / 64;                        // runs of 64 dims: 128-byte rows
     constexpr uint32_t Q_BYTES = SUBS * HALF_TILE, KV_BYTES = SUBS * HALF_TILE;
@@ -140,13 +147,15 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
     __shared__ unsigned s_runs[CONSTS];                  // the tile's runs: bit i, it has a page; bit 8 + i, its values' scale is not 2^ev
     __shared__ float s_rest[CONSTS][BN / 16];            // of these: the scale over 2^ev
     __shared__ uint64_t q_ready[2], first_k, k_empty[STAGES], v_empty[STAGES], s_full[2], go[2][2], o_full[2], c_full[CONSTS];
+    __shared__ float2 s_ml[SPLIT ? 256 : 1];             // M and l of the rows
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int s_failed;
 
     pdl_launch_dependents();
     pdl_wait();
     // tiles in the slowest dimension: all requests' blocks with the most keys start first, and what is left for the end is small
-    const int z = blockIdx.y, kvh = blockIdx.x, nth = blockIdx.z;
+    const int z = blockIdx.y, kvh = SPLIT ? blockIdx.x / a.splits : blockIdx.x, nth = blockIdx.z;
+    const int rank = SPLIT ? blockIdx.x - kvh * a.splits : 0;
     const int row0 = a.q_start[z], n = a.q_start[z + 1] - row0, before = a.kv_before[z];
     const bool there = row0 >= 0 && n <= a.n_rows - row0 && n <= a.max_n;      // the portion's rows, and blocks for them
     if (!there && n > 0 && threadIdx.x == 0 && a.status) atomicOr(a.status, 16);
@@ -168,8 +177,13 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
     if (key_last < pos_last && threadIdx.x == 0 && a.status) atomicOr(a.status, 16);
     const int kt_window = lo_first / BN;
     const int kept_tiles = lo_first > 0 ? min((int)((min((long long)a.keep_first, in_table) + BN - 1) / BN), kt_window) : 0;
-    const int n_it = pos_last >= 0 ? kept_tiles + max(key_last / BN - kt_window + 1, 0) : 0;
-    auto first_of = [&](int t) { return (t < kept_tiles ? t : t - kept_tiles + kt_window) * BN; };
+    const int n_all = pos_last >= 0 ? kept_tiles + max(key_last / BN - kt_window + 1, 0) : 0;
+    const int share = SPLIT ? (n_all + a.splits - 1) / a.splits : n_all, begin = SPLIT ? min(n_all, rank * share) : 0;
+    const int n_it = SPLIT ? min(share, n_all - begin) : n_all;
+    auto first_of = [&](int it) {
+        const int t = begin + it;
+        return (t < kept_tiles ? t : t - kept_tiles + kt_window) * BN;
+    };
     const int tid = threadIdx.x, warp = tid >> 5;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
 
@@ -219,22 +233,23 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
         if (g < groups) {
             // the row of q, scaled, as the first operand: 16-byte piece c of its 128-byte rows at piece c ^ (r & 7)
             const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(row0 + token) * a.ld_q + (size_t)h * HD);
+            uint4 w[HD / 8];
+#pragma unroll
+            for (int c = 0; c < HD / 8; c++) w[c] = mine ? src[c] : make_uint4(0u, 0u, 0u, 0u);
             uint32_t amax = 0;
-#pragma unroll 4
+#pragma unroll
             for (int c = 0; c < HD / 8; c++) {
-                const uint4 w = mine ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-                const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+                const uint32_t m = __vmaxu2(__vmaxu2(w[c].x & 0x7fff7fffu, w[c].y & 0x7fff7fffu), __vmaxu2(w[c].z & 0x7fff7fffu, w[c].w & 0x7fff7fffu));
                 amax = max(amax, max(m & 0xffffu, m >> 16));
             }
             const int e2 = max(-100, min(120, (int)(amax >> 7) - 127));
             const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
             factor = __uint_as_float((uint32_t)(127 + e2) << 23) * a.scale * (a.softcap > 0.0f ? 1.0f : LOG2E);
             const uint32_t to = base + g * Q_BYTES + r * 128;
-#pragma unroll 4
+#pragma unroll
             for (int c = 0; c < HD / 8; c++) {
-                const uint4 w = mine ? src[c] : make_uint4(0u, 0u, 0u, 0u);
                 auto two = [&](uint32_t x) { return pack_half(__uint_as_float(x << 16) * down, __uint_as_float(x & 0xffff0000u) * down); };
-                sts128(to + (c >> 3) * HALF_TILE + (((c & 7) ^ (r & 7)) << 4), two(w.x), two(w.y), two(w.z), two(w.w));
+                sts128(to + (c >> 3) * HALF_TILE + (((c & 7) ^ (r & 7)) << 4), two(w[c].x), two(w[c].y), two(w[c].z), two(w[c].w));
             }
             fence_async_proxy();
             warp_arrive(&q_ready[g]);
@@ -353,7 +368,25 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             tc_fence_before();
             warp_arrive(&go[g][it & 1]);
         }
-        if (g < groups) {
+        if (SPLIT && g < groups) {
+            // this block's sums where its keys and values lay, 4 dims of a row in a piece, a row's pieces 256 pieces apart
+            if (n_it > 0) {
+                wait_for(&o_full[0], 0);                             // of both: nothing reads keys and values any more
+                if (groups == 2) wait_for(&o_full[1], 0);
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; c++) {
+                    uint32_t o[32];
+                    tmem_ld_32x32(lanes + o_col(g) + 32 * c, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        sts128(base + OFF_K + ((8 * c + e) * 256 + tid) * 16, o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                }
+            }
+            s_ml[tid] = make_float2(M, l);
+        }
+        if (!SPLIT && g < groups) {
             if (n_it > 0) {
                 wait_for(&o_full[g], 0);
                 tc_fence_after();
@@ -391,39 +424,56 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
         const int p = tid - FIRST_PRODUCER, piece = p % PIECES, my_row = p / PIECES;
         const int* table = a.block_table + (size_t)z * a.max_blocks;
         auto seen = [&](int j) { return j <= pos_last && (j >= lo_first || j < a.keep_first); };
-        // Threads 0..7: page and scales of a run of tile `it`, two tiles before the tile is brought, so that no one waits for the
-        // chain from the table to the scales.  A run whose values' scale is not finite takes a key scale of NaN: rows that see it
-        // become NaN.  The tile's slot is free: whoever is two tiles behind has stored a tile whose stage the products had left.
-        auto look_up = [&](int it) {
-            if (p >= BN / 16 || it >= n_it) return;
-            const int j = first_of(it) + 16 * p;
-            bool good = false, odd = false;
+        // Pages and scales of four tiles' runs, a lane of the first warp each: the pages are asked for four tiles ahead, the scales a
+        // tile later, and noted another tile later, so that no one waits for the chain from the table to the scales.  A run whose values'
+        // scale is not finite takes a key scale of NaN: rows that see it become NaN.
+        int run_page = -1;
+        float run_ks = 0.0f, run_vs = 0.0f;
+        auto run_key = [&](int it) { return first_of(it + (p >> 3)) + 16 * (p & 7); };
+        auto run_seen = [&](int it) {
+            const int j = run_key(it);
+            return it + (p >> 3) < n_it && j <= pos_last && (j + 15 >= lo_first || j < a.keep_first);
+        };
+        auto block_of = [&](int j) { return a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size; };
+        auto ask_pages = [&](int it) {
+            run_page = -1;
+            if (run_seen(it)) {
+                const int b = block_of(run_key(it));
+                if (b < a.max_blocks) run_page = table[b];
+                if (run_page >= a.num_pages) run_page = -1;
+            }
+        };
+        auto ask_scales = [&]() {
+            if (run_page < 0) return;
+            run_vs = a.v_scale[(size_t)run_page * a.scale_stride + kvh];
+            run_ks = a.k_scale[(size_t)run_page * a.scale_stride + kvh];
+        };
+        // The tiles' slots are free: two tiles before the first of them the products have left the tile eight before the last.
+        auto note = [&](int it) {
             RunConsts c = {0.0f, -INFINITY, 0.0f, 0.0f};             // keys of no page weigh nothing
             long long off = 0;
-            if (j <= pos_last && (j + 15 >= lo_first || j < a.keep_first)) {
-                const int b = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
-                const int page = b < a.max_blocks ? table[b] : -1;
-                if (page >= 0 && page < a.num_pages) {
-                    good = true;
-                    off = page * a.page_stride + ((long long)kvh * a.page_size + (j - b * a.page_size)) * HD;
-                    const float vs = a.v_scale[(size_t)page * a.scale_stride + kvh];
-                    c.ks = a.k_scale[(size_t)page * a.scale_stride + kvh];
-                    const int biased = (int)(__float_as_uint(vs) >> 23) & 255, e = biased == 255 ? 127 : max(biased, 127 - 60);
-                    c.ev = (float)(e - 127);                         // at least -60: see attention_8bit.cu
-                    c.inv = __uint_as_float((unsigned)max(254 - e, 0) << 23);
-                    if (biased == 255) c.ks = __uint_as_float(0x7fffffffu);
-                    else odd = __float_as_uint(vs) != (unsigned)e << 23;
-                    s_rest[it % CONSTS][p] = vs * c.inv;
-                } else if (a.status) {
-                    atomicOr(a.status, 16);
-                }
+            float rest = 1.0f;
+            bool odd = false;
+            const int slot = (it + (p >> 3)) % CONSTS;
+            if (run_page >= 0) {
+                const int j = run_key(it), biased = (int)(__float_as_uint(run_vs) >> 23) & 255, e = biased == 255 ? 127 : max(biased, 127 - 60);
+                off = run_page * a.page_stride + ((long long)kvh * a.page_size + (j - block_of(j) * a.page_size)) * HD;
+                c.ks = biased == 255 ? __uint_as_float(0x7fffffffu) : run_ks;
+                c.ev = (float)(e - 127);                             // at least -60: see attention_8bit.cu
+                c.inv = __uint_as_float((unsigned)max(254 - e, 0) << 23);
+                odd = biased != 255 && __float_as_uint(run_vs) != (unsigned)e << 23;
+                rest = run_vs * c.inv;
+            } else if (run_seen(it) && a.status) {
+                atomicOr(a.status, 16);
             }
-            s_consts[it % CONSTS][p] = c;
-            s_off[it % CONSTS][p] = off;
-            const unsigned all = __ballot_sync(0xffu, good);
-            const unsigned odds = __ballot_sync(0xffu, odd);
-            if (p == 0) s_runs[it % CONSTS] = all | odds << 8;
-            mbar_arrive(&c_full[it % CONSTS]);
+            const unsigned good = __ballot_sync(0xffffffffu, run_page >= 0), odds = __ballot_sync(0xffffffffu, odd);
+            if (it + (p >> 3) < n_it) {
+                s_consts[slot][p & 7] = c;
+                s_off[slot][p & 7] = off;
+                s_rest[slot][p & 7] = rest;
+                if ((p & 7) == 0) s_runs[slot] = ((good >> p) & 0xff) | ((odds >> p) & 0xff) << 8;
+                mbar_arrive(&c_full[slot]);
+            }
         };
         // A thread's pieces of a tile; bit i of the result: piece i is one that counts.  The others are read from where something is, so
         // that no load hangs on a condition, and become zeros when stored.
@@ -486,14 +536,24 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             }
         };
         uint4 kw[EACH], vw[EACH];
-        look_up(0);
-        look_up(1);
+        if (p < 32) {
+            ask_pages(0);
+            ask_scales();
+            note(0);
+        }
         asm volatile("bar.sync 1, 128;" ::: "memory");
         unsigned k_counts = load(a.k, 0, kw), v_counts = load(a.v, 0, vw);
         for (int it = 0; it < n_it; it++) {
             const int stage = it % STAGES;
-            look_up(it + 2);
-            asm volatile("bar.sync 1, 128;" ::: "memory");           // the producers: tile it + 1 has been looked up
+            const int next = (it & ~3) + 4;                          // the four tiles after these
+            if (next < n_it) {
+                if (p < 32) {
+                    if ((it & 3) == 0) ask_pages(next);
+                    if ((it & 3) == 1) ask_scales();
+                    if ((it & 3) == 2) note(next);
+                }
+                if ((it & 3) == 2) asm volatile("bar.sync 1, 128;" ::: "memory");      // the producers: they have been noted
+            }
             if (it >= STAGES) wait_for(&k_empty[stage], (it / STAGES - 1) & 1);
             store(base + OFF_K + stage * KV_BYTES, kw, k_counts);
             fence_async_proxy();
@@ -565,6 +625,47 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
         }
         __syncwarp();
     }
+    if constexpr (SPLIT) {
+        // ---- the cluster's sums, joined in its blocks' order: each block does its share of the rows, a row in a.splits pieces ------------
+        const cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        const int rows = 256 / a.splits, row = rank * rows + (tid & (rows - 1)), width = HD / a.splits, d0 = tid / rows * width;
+        if (tid < 256 && row < n_valid) {
+            const int token = (first + row) / a.group, h = kvh * a.group + (first + row - token * a.group);
+            const float4* sums = reinterpret_cast<const float4*>(smem_raw + (base - smem_u32(smem_raw)) + OFF_K);
+            float m = -INFINITY, L = 0.0f;
+            for (int k = 0; k < a.splits; k++) m = fmaxf(m, cluster.map_shared_rank(s_ml, k)[row].x);
+            // a block that saw no key has no maximum and nothing to add; what is NaN has no maximum either, and counts
+            auto factor_of = [&](float2 ml) { return ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : ex2(ml.x - m); };
+            for (int k = 0; k < a.splits; k++) {
+                const float2 ml = cluster.map_shared_rank(s_ml, k)[row];
+                L = fmaf(ml.y, factor_of(ml), L);
+            }
+            if (a.sink && m > -INFINITY) L += ex2(fmaf(a.sink[h], LOG2E, -m));
+            float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;        // no visible key: zeros
+            if (a.out_gate) inv *= a.out_gate[(size_t)(row0 + token) * a.n_heads + h];
+            bf16* dst = a.out + (size_t)(row0 + token) * a.ld_out + (size_t)h * HD;
+            for (int d = d0; d < d0 + width; d += 8) {
+                float y[8] = {};
+                for (int k = 0; k < a.splits; k++) {
+                    const float f = factor_of(cluster.map_shared_rank(s_ml, k)[row]);
+                    if (f == 0.0f) continue;
+                    const float4* from = cluster.map_shared_rank(sums, k);
+                    const float4 u = from[d / 4 * 256 + row], v = from[(d / 4 + 1) * 256 + row];
+                    const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int i = 0; i < 8; i++) y[i] = fmaf(x[i], f, y[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    y[i] *= inv;
+                    if (a.elem_gate) y[i] *= elem_gate_of(a.elem_gate, a.ld_elem_gate, a.gate_dim, row0 + token, h, d + i);
+                }
+                *reinterpret_cast<uint4*>(dst + d) = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+            }
+        }
+        cluster.sync();                                              // no block leaves while another reads its sums
+    }
     tc_fence_before();
     __syncthreads();
     if (warp == ISSUE_WARP) {
@@ -573,8 +674,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
     }
 }
 
-template <int CODE, int HD>
-int launch(const Args& a, int n_seqs, int max_q_len, cudaStream_t stream) {
+template <int CODE, int HD, bool SPLIT>
+int launch(const Args& a, int n_seqs, long long tiles, cudaStream_t stream) {
     constexpr int SMEM = (2 + 2 * STAGES) * (HD / 64) * (int)HALF_TILE + 1024;
     static std::atomic<unsigned long long> told{0};
     int device = 0;
@@ -582,12 +683,33 @@ int launch(const Args& a, int n_seqs, int max_q_len, cudaStream_t stream) {
     if (e != cudaSuccess) return (int)e;
     const unsigned long long bit = 1ull << (device & 63);
     if (!(told.load() & bit) || device > 63) {
-        e = cudaFuncSetAttribute(prefill_8bit_kernel<CODE, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        e = cudaFuncSetAttribute(prefill_8bit_kernel<CODE, HD, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return (int)e;
         told.fetch_or(bit);
     }
-    const dim3 grid(a.n_kv_heads, n_seqs, (unsigned)(((long long)max_q_len * a.group + 255) / 256));
-    return sandy_launch(prefill_8bit_kernel<CODE, HD>, grid, dim3(THREADS), SMEM, stream, a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.n_kv_heads * a.splits, n_seqs, (unsigned)tiles);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int na = 0;
+    if (SPLIT) {
+        attr[na].id = cudaLaunchAttributeClusterDimension;
+        attr[na].val.clusterDim.x = a.splits;
+        attr[na].val.clusterDim.y = 1;
+        attr[na].val.clusterDim.z = 1;
+        na++;
+    }
+    if (sandy_pdl_enabled()) {
+        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[na].val.programmaticStreamSerializationAllowed = 1;
+        na++;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = na;
+    e = cudaLaunchKernelEx(&cfg, prefill_8bit_kernel<CODE, HD, SPLIT>, a);
+    return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
 }  // namespace
@@ -608,7 +730,7 @@ SANDY_API int sandy_prefill_attention_8bit_tc(const SandyAttend8* r, cudaStream_
         return SANDY_ERR_UNSUPPORTED;
     if ((c.head_dim != 64 && c.head_dim != 128) || c.page_size % 16 || c.n_kv_heads < 1 || r->n_heads % c.n_kv_heads) return SANDY_ERR_UNSUPPORTED;
     if (c.page_stride % 16 || (((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)r->q | (uintptr_t)r->out) & 15) || r->ld_q % 8 || r->ld_out % 8 ||
-        r->n_z > 65535 || (long long)r->max_n * (r->n_heads / c.n_kv_heads) > 65535 * 256ll)
+        r->n_z > 65535 || r->num_splits < 0 || r->num_splits > 8 || (r->num_splits & (r->num_splits - 1)) || (long long)r->max_n * (r->n_heads / c.n_kv_heads) > 65535 * 256ll)
         return SANDY_ERR_UNSUPPORTED;
     Args a = {};
     a.q = (const bf16*)r->q;
@@ -644,9 +766,18 @@ SANDY_API int sandy_prefill_attention_8bit_tc(const SandyAttend8* r, cudaStream_
     a.gate_dim = rules.gate_dim;
     a.scale = r->scale;
     a.softcap = rules.softcap;
-    if (c.code == SANDY_E4M3 && c.head_dim == 64) return launch<SANDY_E4M3, 64>(a, r->n_z, r->max_n, stream);
-    if (c.code == SANDY_E4M3 && c.head_dim == 128) return launch<SANDY_E4M3, 128>(a, r->n_z, r->max_n, stream);
-    if (c.code == SANDY_INT8 && c.head_dim == 64) return launch<SANDY_INT8, 64>(a, r->n_z, r->max_n, stream);
-    if (c.code == SANDY_INT8 && c.head_dim == 128) return launch<SANDY_INT8, 128>(a, r->n_z, r->max_n, stream);
+    const long long tiles = ((long long)r->max_n * a.group + 255) / 256, blocks = tiles * c.n_kv_heads * r->n_z;
+    a.splits = r->num_splits;
+    if (!a.splits) {
+        a.splits = 1;
+        while (a.splits < 8 && blocks * a.splits * 2 <= SPLIT_ROOM * sandy_sm_count() && r->max_keys >= a.splits * 2 * BN) a.splits *= 2;
+    }
+#define LAUNCH(CODE, HD) \
+    return a.splits > 1 ? launch<CODE, HD, true>(a, r->n_z, tiles, stream) : launch<CODE, HD, false>(a, r->n_z, tiles, stream)
+    if (c.code == SANDY_E4M3 && c.head_dim == 64) LAUNCH(SANDY_E4M3, 64);
+    if (c.code == SANDY_E4M3 && c.head_dim == 128) LAUNCH(SANDY_E4M3, 128);
+    if (c.code == SANDY_INT8 && c.head_dim == 64) LAUNCH(SANDY_INT8, 64);
+    if (c.code == SANDY_INT8 && c.head_dim == 128) LAUNCH(SANDY_INT8, 128);
+#undef LAUNCH
     return SANDY_ERR_UNSUPPORTED;
 }

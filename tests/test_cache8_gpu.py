@@ -348,6 +348,15 @@ def test_prompt_portions_on_tcgen05(code, H, hkv, d, ps, seqs):
     _check_attention(code, "bf16", H, hkv, d, ps, seqs, False, tc=True)
 
 
+@pytest.mark.parametrize("code", list(CODES))
+@pytest.mark.parametrize("splits", [1, 2, 4, 8])
+@pytest.mark.parametrize("H,hkv,d,ps", [(2, 2, 64, 16), (8, 2, 128, 32)])
+@pytest.mark.parametrize("seqs,rules", [([(0, 1), (0, 128), (0, 3)], {}), ([(0, 300), (700, 140), (3, 0), (1500, 1)], {}), ([(0, 1000)], {}),
+                                        ([(900, 200), (5, 60)], dict(window=200, keep_first=3, sink=True)), ([(400, 260)], dict(chunk=96, out_gate=True, elem_gate=8))])
+def test_prompt_portions_on_tcgen05_in_so_many_splits(code, splits, H, hkv, d, ps, seqs, rules):
+    _check_attention(code, "bf16", H, hkv, d, ps, seqs, False, splits=splits, tc=True, **rules)
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("rules", [r for r in RULES if "dist_bias" not in r], ids=lambda r: "-".join(r))
 def test_rules_on_tcgen05(d, rules):
