@@ -277,18 +277,16 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                     const int j = j0 + 64 * half;
                     const int last = pos - j, from = lo - j, kept = a.keep_first - j;      // this row sees e <= last, e >= from or e < kept
                     read(half);
+                    if (a.softcap > 0.0f) {
+#pragma unroll
+                        for (int e = 0; e < 64; e++)
+                            s[e] = __float_as_uint(a.softcap * LOG2E * tanh_fast(__fdividef(__uint_as_float(s[e]) * (consts[4 * half + e / 16].ks * factor), a.softcap)));
+                    }
 #pragma unroll
                     for (int u = 0; u < 4; u++) {
-                        const float f = consts[4 * half + u].ks * factor, ev = consts[4 * half + u].ev;
-                        if (a.softcap > 0.0f) {
+                        const float f = a.softcap > 0.0f ? 1.0f : consts[4 * half + u].ks * factor, ev = consts[4 * half + u].ev;
 #pragma unroll
-                            for (int e = 16 * u; e < 16 * u + 16; e++)
-                                s[e] = __float_as_uint(
-                                    fmaf(a.softcap * LOG2E, tanh_fast(__fdividef(__uint_as_float(s[e]) * f, a.softcap)), ev));
-                        } else {
-#pragma unroll
-                            for (int e = 16 * u; e < 16 * u + 16; e++) s[e] = __float_as_uint(fmaf(__uint_as_float(s[e]), f, ev));
-                        }
+                        for (int e = 16 * u; e < 16 * u + 16; e++) s[e] = __float_as_uint(fmaf(__uint_as_float(s[e]), f, ev));
                     }
 #pragma unroll
                     for (int e = 0; e < 64; e++)
@@ -391,6 +389,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                 wait_for(&o_full[g], 0);
                 tc_fence_after();
             }
+            const bool nothing = M == -INFINITY && l == 0.0f;        // no visible key
             if (a.sink && M > -INFINITY) l += ex2(fmaf(a.sink[h], LOG2E, -M));
             float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;        // no visible key: zeros
             if (a.out_gate && mine) inv *= a.out_gate[(size_t)(row0 + token) * a.n_heads + h];
@@ -403,18 +402,18 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                     tmem_wait_ld();
                 }
                 if (mine) {
+                    float y[32];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        float y[8];
+                    for (int e = 0; e < 32; e++) y[e] = nothing ? 0.0f : __uint_as_float(o[e]) * inv;
+                    // one branch around all of it: a test at each element, and the code it jumps over, made the write-back three times as long
+                    if (a.elem_gate) {
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            y[i] = M == -INFINITY && l == 0.0f ? 0.0f : __uint_as_float(o[e + i]) * inv;
-                            if (a.elem_gate)
-                                y[i] *= elem_gate_of(a.elem_gate, a.ld_elem_gate, a.gate_dim, row0 + token, h, 32 * c + e + i);
-                        }
-                        *reinterpret_cast<uint4*>(dst + 32 * c + e) =
-                            make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+                        for (int e = 0; e < 32; e++) y[e] *= elem_gate_of(a.elem_gate, a.ld_elem_gate, a.gate_dim, row0 + token, h, 32 * c + e);
                     }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                        *reinterpret_cast<uint4*>(dst + 32 * c + e) = make_uint4(pack_bf16(y[e], y[e + 1]), pack_bf16(y[e + 2], y[e + 3]),
+                                                                                 pack_bf16(y[e + 4], y[e + 5]), pack_bf16(y[e + 6], y[e + 7]));
                 }
             }
         }
@@ -657,9 +656,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                     for (int i = 0; i < 8; i++) y[i] = fmaf(x[i], f, y[i]);
                 }
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    y[i] *= inv;
-                    if (a.elem_gate) y[i] *= elem_gate_of(a.elem_gate, a.ld_elem_gate, a.gate_dim, row0 + token, h, d + i);
+                for (int i = 0; i < 8; i++) y[i] *= inv;
+                if (a.elem_gate) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) y[i] *= elem_gate_of(a.elem_gate, a.ld_elem_gate, a.gate_dim, row0 + token, h, d + i);
                 }
                 *reinterpret_cast<uint4*>(dst + d) = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
             }
