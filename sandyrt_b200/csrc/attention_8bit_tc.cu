@@ -92,6 +92,13 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t* r)
         "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
@@ -256,6 +263,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
         }
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         float M = -INFINITY, l = 0.0f;
+        // of the warp's rows: the first and the last position, the first visible key behind the kept ones
+        const int pos_min = __reduce_min_sync(0xffffffffu, mine ? pos : 0x7fffffff), pos_max = __reduce_max_sync(0xffffffffu, pos);
+        const int lo_min = __reduce_min_sync(0xffffffffu, mine ? lo : 0x7fffffff), lo_max = __reduce_max_sync(0xffffffffu, mine ? lo : 0);
         for (int it = 0; it < n_it && g < groups; it++) {
             const int j0 = first_of(it);
             wait_for(&c_full[it % CONSTS], (it / CONSTS) & 1);       // long there
@@ -268,54 +278,58 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                 tmem_ld_32x32(lanes + s_col(g) + 64 * half + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
                 tmem_wait_ld();
             };
-            // A tile that every row of the block sees whole needs no mask.  In any other the scores become x where they lie.
+            // A tile that every row of the block sees whole needs no mask.  In any other the scores become x where they lie, 32 keys at a
+            // time: not those that none of the warp's rows sees, and with a test a key only where some see it and some don't.
             const bool whole = j0 + BN - 1 <= pos_first && j0 >= lo_last && a.softcap == 0.0f;
-            if (!whole) {
-                const bool ranged = a.window > 0 || a.chunk > 0;
+            unsigned hidden = 0;                         // which 32 keys no row of the warp sees
+            float top = -INFINITY;
+            if (whole) {
 #pragma unroll 1
                 for (int half = 0; half < 2; half++) {
-                    const int j = j0 + 64 * half;
-                    const int last = pos - j, from = lo - j, kept = a.keep_first - j;      // this row sees e <= last, e >= from or e < kept
                     read(half);
-                    if (a.softcap > 0.0f) {
-#pragma unroll
-                        for (int e = 0; e < 64; e++)
-                            s[e] = __float_as_uint(a.softcap * LOG2E * tanh_fast(__fdividef(__uint_as_float(s[e]) * (consts[4 * half + e / 16].ks * factor), a.softcap)));
-                    }
 #pragma unroll
                     for (int u = 0; u < 4; u++) {
-                        const float f = a.softcap > 0.0f ? 1.0f : consts[4 * half + u].ks * factor, ev = consts[4 * half + u].ev;
+                        float m0 = __uint_as_float(s[16 * u]), m1 = __uint_as_float(s[16 * u + 1]);
 #pragma unroll
-                        for (int e = 16 * u; e < 16 * u + 16; e++) s[e] = __float_as_uint(fmaf(__uint_as_float(s[e]), f, ev));
+                        for (int e = 2; e < 16; e += 2) {
+                            m0 = fmaxf(m0, __uint_as_float(s[16 * u + e]));
+                            m1 = fmaxf(m1, __uint_as_float(s[16 * u + e + 1]));
+                        }
+                        top = fmaxf(top, fmaf(fmaxf(m0, m1), consts[4 * half + u].ks * factor, consts[4 * half + u].ev));
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (int q = 0; q < 4; q++) {
+                    const int j = j0 + 32 * q;
+                    if (j > pos_max || (j + 31 < lo_min && j >= a.keep_first)) {
+                        hidden |= 1u << q;
+                        continue;
+                    }
+                    uint32_t x[32];
+                    tmem_ld_32x32(lanes + s_col(g) + 32 * q, x);
+                    tmem_wait_ld();
+                    const RunConsts c0 = consts[2 * q], c1 = consts[2 * q + 1];
+                    float f0 = c0.ks * factor, f1 = c1.ks * factor;
+                    if (a.softcap > 0.0f) {
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            x[e] = __float_as_uint(a.softcap * LOG2E * tanh_fast(__fdividef(__uint_as_float(x[e]) * (e < 16 ? f0 : f1), a.softcap)));
+                        f0 = f1 = 1.0f;
                     }
 #pragma unroll
-                    for (int e = 0; e < 64; e++)
-                        if (e > last) s[e] = 0xff800000u;
-                    if (ranged) {
+                    for (int e = 0; e < 32; e++) x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), e < 16 ? f0 : f1, e < 16 ? c0.ev : c1.ev));
+                    if (j + 31 > pos_min || j < lo_max) {
+                        const int last = pos - j, from = lo - j, kept = a.keep_first - j;      // this row sees e <= last, e >= from or e < kept
 #pragma unroll
-                        for (int e = 0; e < 64; e++)
-                            if (e < from && e >= kept) s[e] = 0xff800000u;
+                        for (int e = 0; e < 32; e++)
+                            if (e > last || (e < from && e >= kept)) x[e] = 0xff800000u;
                     }
-                    tmem_st_32x32(lanes + s_col(g) + 64 * half, s);
-                    tmem_st_32x32(lanes + s_col(g) + 64 * half + 32, s + 32);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) top = fmaxf(top, __uint_as_float(x[e]));
+                    tmem_st_32x32(lanes + s_col(g) + 32 * q, x);
                 }
                 tmem_wait_st();
-            }
-            float top = -INFINITY;
-#pragma unroll 1
-            for (int half = 0; half < 2; half++) {
-                read(half);
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    float m0 = __uint_as_float(s[16 * u]), m1 = __uint_as_float(s[16 * u + 1]);
-#pragma unroll
-                    for (int e = 2; e < 16; e += 2) {
-                        m0 = fmaxf(m0, __uint_as_float(s[16 * u + e]));
-                        m1 = fmaxf(m1, __uint_as_float(s[16 * u + e + 1]));
-                    }
-                    m0 = fmaxf(m0, m1);
-                    top = fmaxf(top, whole ? fmaf(m0, consts[4 * half + u].ks * factor, consts[4 * half + u].ev) : m0);
-                }
             }
             const bool move = top > M + RESCALE;
             if (__any_sync(0xffffffffu, move)) {
@@ -328,12 +342,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                         tmem_wait_ld();
 #pragma unroll
                         for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                        asm volatile(
-                            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-                            "%15, %16};" ::"r"(lanes + o_col(g) + 16 * c),
-                            "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]), "r"(o[8]), "r"(o[9]),
-                            "r"(o[10]), "r"(o[11]), "r"(o[12]), "r"(o[13]), "r"(o[14]), "r"(o[15])
-                            : "memory");
+                        tmem_st_32x16(lanes + o_col(g) + 16 * c, o);
                     }
                     tmem_wait_st();
                 }
@@ -341,26 +350,53 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                 if (move) M = top;
             }
             const float m_use = M == -INFINITY ? 0.0f : M;           // no key yet: weights are 2^-inf
+            if (whole) {
 #pragma unroll 1
-            for (int half = 0; half < 2; half++) {
-                read(half);
+                for (int half = 0; half < 2; half++) {
+                    read(half);
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const RunConsts c = consts[4 * half + u];
-                    const float f = whole ? c.ks * factor : 1.0f, off = (whole ? c.ev : 0.0f) - m_use;
-                    float2 sum = {0.0f, 0.0f};
+                    for (int u = 0; u < 4; u++) {
+                        const RunConsts c = consts[4 * half + u];
+                        const float f = c.ks * factor, off = c.ev - m_use;
+                        float2 sum = {0.0f, 0.0f};
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        float2 x = fma2(make_float2(__uint_as_float(s[16 * u + e]), __uint_as_float(s[16 * u + e + 1])), make_float2(f, f), make_float2(off, off));
-                        x.x = ex2(x.x);
-                        x.y = ex2(x.y);
-                        sum = add2(sum, x);
-                        s[8 * u + e / 2] = pack_half(x.x, x.y);
+                        for (int e = 0; e < 16; e += 2) {
+                            float2 x = fma2(make_float2(__uint_as_float(s[16 * u + e]), __uint_as_float(s[16 * u + e + 1])), make_float2(f, f), make_float2(off, off));
+                            x.x = ex2(x.x);
+                            x.y = ex2(x.y);
+                            sum = add2(sum, x);
+                            s[8 * u + e / 2] = pack_half(x.x, x.y);
+                        }
+                        l = fmaf(sum.x + sum.y, c.inv, l);
                     }
-                    l = fmaf(sum.x + sum.y, c.inv, l);
+                    // over columns whose scores have been read: 0..31 of the tile's 128, then 32..63
+                    tmem_st_32x32(lanes + s_col(g) + 32 * half, s);
                 }
-                // over columns whose scores have been read: 0..31 of the tile's 128, then 32..63
-                tmem_st_32x32(lanes + s_col(g) + 32 * half, s);
+            } else {
+                // 32 keys' weights over 16 columns, whose scores have been read
+#pragma unroll 1
+                for (int q = 0; q < 4; q++) {
+                    uint32_t x[32];
+                    if ((hidden >> q) & 1) {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) x[e] = 0u;
+                    } else {
+                        tmem_ld_32x32(lanes + s_col(g) + 32 * q, x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            float2 sum = {0.0f, 0.0f};
+#pragma unroll
+                            for (int e = 16 * u; e < 16 * u + 16; e += 2) {
+                                const float2 w = {ex2(__uint_as_float(x[e]) - m_use), ex2(__uint_as_float(x[e + 1]) - m_use)};
+                                sum = add2(sum, w);
+                                x[e / 2] = pack_half(w.x, w.y);
+                            }
+                            l = fmaf(sum.x + sum.y, consts[2 * q + u].inv, l);
+                        }
+                    }
+                    tmem_st_32x16(lanes + s_col(g) + 16 * q, x);
+                }
             }
             tmem_wait_st();
             tc_fence_before();
