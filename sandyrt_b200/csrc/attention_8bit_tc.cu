@@ -22,10 +22,14 @@
 // What bounds it: 32,768 exponentials a pair of tiles are 2,048 cycles of the special-function units, the products at heads of 128
 // as much of the tensor cores; converting 32,768 codes is some 700 (int8) issue slots of each SM quarter.  256 rows a block halve the
 // conversion's share and the reads of the cache.  One block an SM (193 KB of shared memory at heads of 128).
-// Measured: 2,048 tokens behind 6,000, 32 heads of 128 reading 8 (int8): 307 us, 46% of the 1.67 PFLOP/s that a matrix product gets;
-// four prompts of 500 to 950 tokens, 12 heads of 64 (e4m3): 39 us.  A pair of tiles takes some 5,000 cycles: what a tile waits for is the
-// chain of its softmax (reading, exponentials, writing), the issuing warp's wake-up and the products, of which the two tiles overlap
-// about half; and 256 blocks on 148 SMs are two rounds.  Blocks with the most keys start first, over all requests.
+// Measured: 2,048 tokens behind 6,000, 32 heads of 128 reading 8 (int8): 288 us, 49% of the 1.67 PFLOP/s that a matrix product gets;
+// four prompts of 500 to 950 tokens, 12 heads of 64 (e4m3): 32.6 us.  At heads of 64 a pair of tiles takes 3,300 cycles: 2,200 of softmax,
+// and 1,100 from the weights to the next scores (the issuing warp's wake-up, two products, the way back), of which the two tiles
+// overlap about half.  A block needs 6,500 cycles to its first scores (page, scale, codes, each a trip to memory) and 2,000 for its
+// write-back; 256 blocks on 148 SMs are two rounds.  Blocks with the most keys start first, over all requests.
+//
+// Where blocks are fewer than SMs, clusters of 2, 4 or 8 share the key tiles of a block of rows.  Each block leaves its O (in the place of
+// its keys and values) and its rows' M and l in its shared memory; then each joins its share of the rows, in the blocks' order.
 //
 // Every wait on an mbarrier is bounded; one that runs out raises bit 8 of the status word and the block ends without waiting again.
 #include <algorithm>
@@ -45,7 +49,6 @@ constexpr int BN = 128;                  // keys of a tile
 constexpr int THREADS = 416;
 constexpr int FIRST_PRODUCER = 256, ISSUE_WARP = 12;
 constexpr int STAGES = 2;
-constexpr int SPLIT_ROOM = 1;            // rounds of blocks that splits of the keys may make
 constexpr int CONSTS = 8;                // key tiles whose scales and pages are kept
 constexpr float RESCALE = 8.0f;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -805,8 +808,11 @@ SANDY_API int sandy_prefill_attention_8bit_tc(const SandyAttend8* r, cudaStream_
     const long long tiles = ((long long)r->max_n * a.group + 255) / 256, blocks = tiles * c.n_kv_heads * r->n_z;
     a.splits = r->num_splits;
     if (!a.splits) {
+        // As many blocks as fit the SMs at once, each with a key tile at least.  256 tokens behind 6,000, 32 heads of 128 on 8: one block
+        // for all keys 135 us, two 80, four 51, eight (two rounds) 112; behind 20,000, 8 heads: 430, 228, 125, 75; a prompt of 950
+        // tokens, 12 heads of 64: 27, 20, 33, 65.
         a.splits = 1;
-        while (a.splits < 8 && blocks * a.splits * 2 <= SPLIT_ROOM * sandy_sm_count() && r->max_keys >= a.splits * 2 * BN) a.splits *= 2;
+        while (a.splits < 8 && blocks * a.splits * 2 <= sandy_sm_count() && r->max_keys >= a.splits * 2 * BN) a.splits *= 2;
     }
 #define LAUNCH(CODE, HD) \
     return a.splits > 1 ? launch<CODE, HD, true>(a, r->n_z, tiles, stream) : launch<CODE, HD, false>(a, r->n_z, tiles, stream)
