@@ -223,13 +223,13 @@ __device__ __forceinline__ unsigned power_of(float vs, float& ev, float& inv) {
 // WARPS: of a block; DMAX: 64, 128 or 256, the head size rounded up; DK: the head size, or 0 where it is known at run time only; NT: column tiles of
 // 8; KT: key tiles of 16 that a warp takes at a time; RUN: 16 or 8, pages are a multiple of it, so that a tile or half a tile lies in
 // one page; 0: every row is looked up by itself.
-template <typename T, int CODE, int WARPS, int DMAX, int DK, int NT, int KT, int RUN>
+template <typename T, int CODE, int WARPS, int DMAX, int DK, int NT, int KT, int RUN, bool ONE = false>
 __global__ void __launch_bounds__(WARPS * 32, NT == 1 && DMAX < 256 ? 16 / WARPS : 1)
 attention_8bit_kernel(const __grid_constant__ Args a) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1;            // pieces a number is split into
     constexpr int QT = 8 * NT / P;                       // queries of a block
     constexpr int CH = DMAX / 64;                        // runs of 64 dims
-    constexpr int Q2 = 2 / P;                            // queries in a lane's two columns of a tile
+    constexpr int Q2 = P == 2 || ONE ? 1 : 2;                            // queries in a lane's two columns of a tile
     constexpr int STAGES = stages_of(DMAX, KT), STAGE = 2 * KT * 16 * DMAX;
     // a warp's stages [STAGES][keys | values][KT * 16 rows of DMAX bytes]; at the end the warps' sums in the same place
     extern __shared__ __align__(128) uint8_t smem[];
@@ -562,7 +562,7 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     // 2^(x - M) is the weight times the value's scale, where that is a power of two: what appending gives
-                    float w[2];
+                    float w[2] = {0.0f, 0.0f};
 #pragma unroll
                     for (int e = 0; e < Q2; e++) {
                         const float x = sc[kt][n][P == 2 ? 2 * r : 2 * r + e];
@@ -773,12 +773,13 @@ template <typename T, int CODE>
 int launch(const Args& a, int n_z, int max_queries, int max_n, cudaStream_t stream) {
     constexpr int P = sizeof(T) == 4 ? 2 : 1;
     const bool wide = is_wide(max_queries, a.head_dim, sizeof(T) == 4 ? SANDY_F32 : SANDY_BF16);
+    const bool one = P == 1 && max_queries == 1;
     int e;
-#define LAUNCH(WARPS, DMAX, DK, NT, KT, RUN)                                                                                     \
+#define LAUNCH(WARPS, DMAX, DK, NT, KT, RUN, ...)                                                                                \
     do {                                                                                                                         \
         constexpr int QT = 8 * NT / P, ring = WARPS * stages_of(DMAX, KT) * 2 * KT * 16 * DMAX, sums = WARPS * QT * (DMAX + 1) * 4; \
         constexpr int alone = std::max(ring, sums), together = std::max(ring, sums + MAX_CLUSTER * QT * (DMAX + 2) * 4);          \
-        e = start<attention_8bit_kernel<T, CODE, WARPS, DMAX, DK, NT, KT, RUN>>(                                                 \
+        e = start<attention_8bit_kernel<T, CODE, WARPS, DMAX, DK, NT, KT, RUN __VA_OPT__(,) __VA_ARGS__>>(                                                 \
             a, dim3((unsigned)((max_queries + QT - 1) / QT * a.num_splits), a.n_kv_heads, n_z), WARPS * 32,                      \
             a.in_cluster ? together : alone, NT == 1 ? together : alone, stream);                                                \
     } while (0)
@@ -788,10 +789,13 @@ int launch(const Args& a, int n_z, int max_queries, int max_n, cudaStream_t stre
         else LAUNCH(4, 256, 0, 1, 1, 0);
     } else if (a.page_size % 16 == 0 && a.head_dim == 64) {
         if (wide) LAUNCH(4, 64, 64, 4, 1, 16);
+        else if (a.two_warps && one) LAUNCH(2, 64, 64, 1, 2, 16, P == 1);
         else if (a.two_warps) LAUNCH(2, 64, 64, 1, 2, 16);
+        else if (one) LAUNCH(4, 64, 64, 1, 2, 16, P == 1);
         else LAUNCH(4, 64, 64, 1, 2, 16);
     } else if (a.page_size % 16 == 0 && a.head_dim == 128) {
         if (wide) LAUNCH(4, 128, 128, 2, 1, 16);
+        else if (one) LAUNCH(4, 128, 128, 1, 1, 16, P == 1);
         else LAUNCH(4, 128, 128, 1, 1, 16);
     } else if (a.head_dim <= 64) {
         if (wide) LAUNCH(4, 64, 0, 4, 1, 8);
