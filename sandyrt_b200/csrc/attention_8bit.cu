@@ -34,10 +34,11 @@
 // What bounds it.  Single tokens: the codes' bytes.  16 warps an SM (in blocks of four, or two where there are very many) with
 // three stages of 4 KB each keep 190 KB on their way.  Where there are few requests `num_splits` blocks share one's keys: up to 8 are a
 // cluster, whose first block takes the others' results over its shared memory; more leave theirs in scratch, which a second kernel joins
-// in a fixed order.  Measured (e4m3, bfloat16): 8 tokens x 12 heads of 64 behind some 1,000 keys 7.5 us, of which half is the launch, the
-// lookup and the join; 64 x 25 heads behind 64 to 1,000 (int8) 37 us, 2.8 TB/s of codes: blocks of unlike length, 14 us with 64 keys each;
-// behind 8,000 keys each 266 us, 94% of 6.57 TB/s (int8 293); 4 requests of 8 heads of 128, each read by 4, behind 30,000 to 100,000
-// keys 119 us, 81%.
+// in a fixed order.  Measured (bfloat16): 8 tokens x 12 heads of 64 behind 100 to 900 keys (e4m3) 6.9 us, of which half is the launch, the
+// lookup and the join; 64 x 25 heads behind 64 to 1,000 (int8) 32.4 us, 3.3 TB/s of codes: 13 us with 64 keys each, what a block's
+// beginning and end cost in 2.7 rounds; behind 8,000 keys each 266 us, 94% of 6.57 TB/s; 4 requests of 8 heads of 128 (e4m3), each read by 4,
+// behind 30,000 to 100,000 keys 118 us, 81%.  Where a key/value head has one query head, bfloat16 kernels keep one column a lane instead of
+// two (ONE): a tenth of the instructions, 32.4 us instead of 36.9 above.
 // Prompt portions: the tensor cores' warp-level instructions; the tcgen05 kernel takes over from 64 query rows on where it can.
 #include <algorithm>
 #include <atomic>
@@ -174,10 +175,11 @@ constexpr float RESCALE = 8.0f;          // how far (in the exponent) a score ma
 // What a warp has looked up about a run of keys in one page: where its rows start (page 0's, if it has no page), its block's scales
 // and what is made of them: ev = log2 of the value's scale, inv = 2^-ev.
 struct __align__(16) Run {
-    long long off;
-    float ks, ev;
-    float inv, vs;
-    unsigned flags, unused;
+    long long off;                       // what copying reads
+    unsigned flags;
+    float vs;
+    float ks, ev, inv;                   // what the products read
+    unsigned again;                      // the flags once more
 };
 constexpr unsigned HAS_PAGE = 1;         // there is a page
 constexpr unsigned NO_POWER = 2;         // vs is not 2^ev: the weights are multiplied by it
@@ -222,7 +224,7 @@ __device__ __forceinline__ unsigned power_of(float vs, float& ev, float& inv) {
 
 // WARPS: of a block; DMAX: 64, 128 or 256, the head size rounded up; DK: the head size, or 0 where it is known at run time only; NT: column tiles of
 // 8; KT: key tiles of 16 that a warp takes at a time; RUN: 16 or 8, pages are a multiple of it, so that a tile or half a tile lies in
-// one page; 0: every row is looked up by itself.
+// one page; 0: every row is looked up by itself.  ONE: a block has one query, in column 0.
 template <typename T, int CODE, int WARPS, int DMAX, int DK, int NT, int KT, int RUN, bool ONE = false>
 __global__ void __launch_bounds__(WARPS * 32, NT == 1 && DMAX < 256 ? 16 / WARPS : 1)
 attention_8bit_kernel(const __grid_constant__ Args a) {
@@ -296,7 +298,7 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
         __syncwarp();
         const int in = group_at * KT + lane / HALVES, half = lane % HALVES;
         const int nth = nth_of(in / KT, in % KT), key0 = first_of(nth), j = key0 + 8 * half;
-        Run run = {0, 0.0f, 0.0f, 0.0f, 0.0f, 0, 0};
+        Run run = {};
         run.flags = (key0 + 15 <= pos_first && key0 >= lo_last && plain ? SEEN_BY_ALL : 0) |
                     (key0 + 15 <= pos_last && key0 >= lo_first ? SEEN_BY_ONE : 0);
         if (lane < 16 && nth < tile_end && j <= pos_last && (j + RUN - 1 >= lo_first || j < a.keep_first)) {
@@ -311,6 +313,7 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                 atomicOr(a.status, 16);
             }
         }
+        run.again = run.flags;
         if (lane < 16) known[warp][(HALVES * in + half) % 32] = run;
         __syncwarp();
     };
@@ -333,14 +336,16 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
     constexpr int PIECES = DMAX / 16, STEP = 32 / PIECES;            // of a row; rows that a warp copies at a time
     const int my_piece = lane % PIECES, my_row = lane / PIECES;
     const uint32_t my_place = my_row * DMAX + swizzled<DMAX>(my_row, my_piece) * 16;      // of rows my_row + a multiple of 4
+    const uint8_t *my_k = a.k + (my_row * D + my_piece * 16), *my_v = a.v + (my_row * D + my_piece * 16);
     auto copy = [&](int group_at, int stage) {
 #pragma unroll
         for (int kt = 0; kt < KT; kt++) {
             const uint32_t to = ring + stage * STAGE + kt * 16 * DMAX;
             if constexpr (RUN == 16) {
-                const Run& run = known[warp][(group_at * KT + kt) % 32];
-                if ((run.flags & (HAS_PAGE | SEEN_BY_ONE)) == (HAS_PAGE | SEEN_BY_ONE)) {      // all of the tile, as it lies
-                    const uint8_t *k = a.k + (run.off + my_row * D + my_piece * 16), *v = a.v + (run.off + my_row * D + my_piece * 16);
+                const uint4 run = *reinterpret_cast<const uint4*>(&known[warp][(group_at * KT + kt) % 32]);
+                if ((run.z & (HAS_PAGE | SEEN_BY_ONE)) == (HAS_PAGE | SEEN_BY_ONE)) {          // all of the tile, as it lies
+                    const long long off = (long long)((unsigned long long)run.y << 32 | run.x);
+                    const uint8_t *k = my_k + off, *v = my_v + off;
 #pragma unroll
                     for (int i = 0; i < 16 / STEP; i++) {
                         copy16(to + my_place + i * STEP * DMAX, k + i * STEP * D);
@@ -439,12 +444,11 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 if constexpr (RUN != 0) {
-                    const Run& run = known[warp][(HALVES * (it * KT + kt) + r) % 32];
-                    ks[kt][r] = run.ks;
-                    ev[kt][r] = run.ev;
-                    inv[kt][r] = run.inv;
-                    vs[kt][r] = run.vs;
-                    flags[kt][r] = run.flags;
+                    const float4 run = *reinterpret_cast<const float4*>(&known[warp][(HALVES * (it * KT + kt) + r) % 32].ks);
+                    ks[kt][r] = run.x;
+                    ev[kt][r] = run.y;
+                    inv[kt][r] = run.z;
+                    flags[kt][r] = __float_as_uint(run.w);
                 } else {
                     size_t off = 0;
                     int page = 0;
@@ -455,6 +459,7 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                 }
             }
 
+        auto vs_of = [&](int kt, int r) { return RUN != 0 ? known[warp][(HALVES * (it * KT + kt) + r) % 32].vs : vs[kt][r]; };
         unsigned every = HAS_PAGE | SEEN_BY_ALL, some = 0;          // flags that all of the group's keys have, that one has
 #pragma unroll
         for (int kt = 0; kt < KT; kt++)
@@ -568,7 +573,7 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                         const float x = sc[kt][n][P == 2 ? 2 * r : 2 * r + e];
                         w[e] = ex2(x - m_use[n][e]);
                         l[n][e] = fmaf(w[e], inv[kt][r % R], l[n][e]);
-                        if (some & NO_POWER) w[e] = x == -INFINITY ? 0.0f : w[e] * inv[kt][r % R] * vs[kt][r % R];
+                        if (some & NO_POWER) w[e] = x == -INFINITY ? 0.0f : w[e] * inv[kt][r % R] * vs_of(kt, r % R);
                     }
                     if (P == 2) w[1] = w[0] - __half2float(__float2half_rn(w[0]));
                     pf[n][r] = turn(pack_half(w[0], w[1]));
