@@ -680,6 +680,15 @@ _RULES8 = {"window": 0, "keep_first": 0, "softcap": 0.0, "chunk": 0, "sink": Non
 _NO_RULES8 = (0, 0, 0.0, 0, 0, 0, 0, 0, 0, 0, 0)
 
 
+def _plain_rules8(rules: dict) -> bool:
+    """Whether every given rule is one that changes nothing, as it is when a caller hands its settings on."""
+    for name, v in rules.items():
+        default = _RULES8.get(name, rules)
+        if v is not default and (default is None or v.__class__ not in (int, float) or v != default):
+            return False
+    return True
+
+
 def _rules8(what: str, q, n_heads: int, rules: dict) -> tuple:
     """The rules as SandyAttentionRules lays them out, and their tensors."""
     for name in rules:
@@ -731,7 +740,7 @@ TC_ROWS_8BIT = 64
 def _attention_8bit(what, q, cache, block_table, width, token_seq, positions, q_start, out, n_z, max_n, n_heads, scale, num_splits, tc, rules) -> None:
     at, (pitch, hkv, d, ps, pages, code) = _cache8(what, cache)
     ld, T, dtype = _queries8(what, n_heads, hkv, d, _layout(q), _layout(out))
-    laid, extra = _rules8(what, q, n_heads, rules) if rules else (_NO_RULES8, ())
+    laid, extra = (_NO_RULES8, ()) if _plain_rules8(rules) else _rules8(what, q, n_heads, rules)
     if num_splits < 0 or num_splits > 256:
         raise KernelError(f"{what}: num_splits must lie in 0 .. 256 (0: the kernel's choice)")
     index = _one_device(what, q, out, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, token_seq, positions, q_start, *extra)
