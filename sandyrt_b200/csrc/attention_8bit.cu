@@ -39,7 +39,7 @@
 // beginning and end cost in 2.7 rounds; behind 8,000 keys each 266 us, 94% of 6.57 TB/s; 4 requests of 8 heads of 128 (e4m3), each read by 4,
 // behind 30,000 to 100,000 keys 118 us, 81%.  Where a key/value head has one query head, bfloat16 kernels keep one column a lane instead of
 // two (ONE): a tenth of the instructions, 32.4 us instead of 36.9 above.
-// Prompt portions: the tensor cores' warp-level instructions; the tcgen05 kernel takes over from 64 query rows on where it can.
+// Prompt portions: the tensor cores' warp-level instructions; the tcgen05 kernel takes over from 33 query rows on where it can.
 #include <algorithm>
 #include <atomic>
 

@@ -733,8 +733,10 @@ def _splits8(*sizes) -> tuple:
     return splits, floats.value
 
 
-# From so many rows (tokens x heads of a group) of the longest portion on, 8-bit prompt attention goes to the tcgen05 kernel.
-TC_ROWS_8BIT = 64
+# From so many rows (tokens x heads of a group) of the longest portion on, 8-bit prompt attention goes to the tcgen05 kernel: the mma.sync
+# one takes up to 32 at a time.  64 rows: 26 us against 28 (one request behind 6,000, 8 heads of 128), 22 against 38 (16 requests behind
+# 300, 12 heads of 64); 32 rows: 22 against 26 (8 requests behind 1,000, 8 heads of 128), 21 against 20; 16 rows: 20 against 16.
+TC_ROWS_8BIT = 33
 
 
 def _attention_8bit(what, q, cache, block_table, width, token_seq, positions, q_start, out, n_z, max_n, n_heads, scale, num_splits, tc, rules) -> None:
