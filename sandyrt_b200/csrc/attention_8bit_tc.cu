@@ -1,5 +1,5 @@
 // Causal attention of prompt portions over the paged cache in 8 bits (kv_8bit.cuh) on the tcgen05 tensor cores: bfloat16 queries,
-// heads of 64 and 128, pages of a multiple of 16 keys.
+// heads of up to 128 (in the place of 64 or 128), pages of a multiple of 16 keys.
 //
 // Formula and scales as in attention_8bit.cu; the products are half-precision ones here too: codes are half-precision numbers without
 // rounding, a query row is scaled by a power of two so that its largest element lies in [1, 2), and the scales of keys and values, which
@@ -16,6 +16,8 @@
 //                    bytes in the 128-byte swizzle, V likewise (an MN-major operand); rows past the portion's last key are zeros;
 //   warp 12          issues the products: S of one tile while the other's softmax runs.  P lies where S lay, so that S of the next
 //                    key tile follows P V of this one; both tiles' S and O fill the 512 columns of tensor memory at heads of 128.
+// Head sizes between are the next of 64 and 128 with zeros behind their dims, in shared memory alone: 12 requests of 800 tokens behind
+// 1,000, 9 heads of 48, 105 us (the mma.sync kernel 492); 12 prompts of 400, 12 heads of 80, 33 (173); 8 heads of 16, 500 tokens, 13 (24).
 // The accumulators stay in tensor memory over all tiles and are rescaled there only when a row's maximum has run ahead of its reference
 // by more than 2^8 (P stays below 256).  When S of a tile is there, the products before it are complete: O is at rest then.
 //
@@ -67,7 +69,7 @@ struct Args {
     const bf16* elem_gate;
     long long ld_q, ld_out, page_stride, scale_stride;
     int max_blocks, n_rows, max_n, n_heads, n_kv_heads, group, page_size, page_shift, num_pages;
-    int window, keep_first, chunk, ld_elem_gate, gate_dim, splits;
+    int window, keep_first, chunk, ld_elem_gate, gate_dim, splits, head_dim;
     float scale, softcap;
 };
 
@@ -142,9 +144,11 @@ __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// HD: 64 or 128, the head size, or (FULL false) the next of the two above it: what is behind the head's dims is zeros in shared memory.
 // SPLIT: a cluster of a.splits blocks shares a block's rows, each with a run of their key tiles.
-template <int CODE, int HD, bool SPLIT>
+template <int CODE, int HD, bool FULL, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_constant__ Args a) {
+    const int D = FULL ? HD : a.head_dim;
     constexpr int SUBS = HD / 64;                        // runs of 64 dims: 128-byte rows
     constexpr uint32_t Q_BYTES = SUBS * HALF_TILE, KV_BYTES = SUBS * HALF_TILE;
     constexpr uint32_t OFF_K = 2 * Q_BYTES, OFF_V = OFF_K + STAGES * KV_BYTES;
@@ -242,10 +246,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
         float factor = 0.0f;
         if (g < groups) {
             // the row of q, scaled, as the first operand: 16-byte piece c of its 128-byte rows at piece c ^ (r & 7)
-            const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(row0 + token) * a.ld_q + (size_t)h * HD);
+            const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(row0 + token) * a.ld_q + (size_t)h * D);
             uint4 w[HD / 8];
 #pragma unroll
-            for (int c = 0; c < HD / 8; c++) w[c] = mine ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+            for (int c = 0; c < HD / 8; c++) w[c] = mine && (FULL || 8 * c < D) ? src[c] : make_uint4(0u, 0u, 0u, 0u);
             uint32_t amax = 0;
 #pragma unroll
             for (int c = 0; c < HD / 8; c++) {
@@ -432,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             if (a.sink && M > -INFINITY) l += ex2(fmaf(a.sink[h], LOG2E, -M));
             float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;        // no visible key: zeros
             if (a.out_gate && mine) inv *= a.out_gate[(size_t)(row0 + token) * a.n_heads + h];
-            bf16* dst = a.out + (size_t)(row0 + token) * a.ld_out + (size_t)h * HD;
+            bf16* dst = a.out + (size_t)(row0 + token) * a.ld_out + (size_t)h * D;
 #pragma unroll 1
             for (int c = 0; c < HD / 32; c++) {
                 uint32_t o[32];
@@ -451,7 +455,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                     }
 #pragma unroll
                     for (int e = 0; e < 32; e += 8)
-                        *reinterpret_cast<uint4*>(dst + 32 * c + e) = make_uint4(pack_bf16(y[e], y[e + 1]), pack_bf16(y[e + 2], y[e + 3]),
+                        if (FULL || 32 * c + e < D) *reinterpret_cast<uint4*>(dst + 32 * c + e) = make_uint4(pack_bf16(y[e], y[e + 1]), pack_bf16(y[e + 2], y[e + 3]),
                                                                                  pack_bf16(y[e + 4], y[e + 5]), pack_bf16(y[e + 6], y[e + 7]));
                 }
             }
@@ -495,7 +499,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             const int slot = (it + (p >> 3)) % CONSTS;
             if (run_page >= 0) {
                 const int j = run_key(it), biased = (int)(__float_as_uint(run_vs) >> 23) & 255, e = biased == 255 ? 127 : max(biased, 127 - 60);
-                off = run_page * a.page_stride + ((long long)kvh * a.page_size + (j - block_of(j) * a.page_size)) * HD;
+                off = run_page * a.page_stride + ((long long)kvh * a.page_size + (j - block_of(j) * a.page_size)) * D;
                 c.ks = biased == 255 ? __uint_as_float(0x7fffffffu) : run_ks;
                 c.ev = (float)(e - 127);                             // at least -60: see attention_8bit.cu
                 c.inv = __uint_as_float((unsigned)max(254 - e, 0) << 23);
@@ -530,9 +534,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
 #pragma unroll
             for (int i = 0; i < EACH; i++) {
                 const int row = i * STEP + my_row;
-                w[i] = __ldg(reinterpret_cast<const uint4*>(from + s_off[at][row >> 4] + ((row & 15) * HD + piece * 16)));
+                w[i] = __ldg(reinterpret_cast<const uint4*>(from + s_off[at][row >> 4] + ((row & 15) * D + (FULL || piece * 16 < D ? piece * 16 : 0))));
             }
-            return counts;
+            return FULL || piece * 16 < D ? counts : 0u;
         };
         // 16 codes of row i * STEP + my_row: two pieces of eight half-precision numbers
         auto store = [&](uint32_t to, uint4 (&w)[EACH], unsigned counts) {
@@ -682,8 +686,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             if (a.sink && m > -INFINITY) L += ex2(fmaf(a.sink[h], LOG2E, -m));
             float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;        // no visible key: zeros
             if (a.out_gate) inv *= a.out_gate[(size_t)(row0 + token) * a.n_heads + h];
-            bf16* dst = a.out + (size_t)(row0 + token) * a.ld_out + (size_t)h * HD;
-            for (int d = d0; d < d0 + width; d += 8) {
+            bf16* dst = a.out + (size_t)(row0 + token) * a.ld_out + (size_t)h * D;
+            for (int d = d0; d < (FULL ? d0 + width : min(d0 + width, D)); d += 8) {
                 float y[8] = {};
                 for (int k = 0; k < a.splits; k++) {
                     const float f = factor_of(cluster.map_shared_rank(s_ml, k)[row]);
@@ -713,7 +717,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
     }
 }
 
-template <int CODE, int HD, bool SPLIT>
+template <int CODE, int HD, bool FULL, bool SPLIT>
 int launch(const Args& a, int n_seqs, long long tiles, cudaStream_t stream) {
     constexpr int SMEM = (2 + 2 * STAGES) * (HD / 64) * (int)HALF_TILE + 1024;
     static std::atomic<unsigned long long> told{0};
@@ -722,7 +726,7 @@ int launch(const Args& a, int n_seqs, long long tiles, cudaStream_t stream) {
     if (e != cudaSuccess) return (int)e;
     const unsigned long long bit = 1ull << (device & 63);
     if (!(told.load() & bit) || device > 63) {
-        e = cudaFuncSetAttribute(prefill_8bit_kernel<CODE, HD, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        e = cudaFuncSetAttribute(prefill_8bit_kernel<CODE, HD, FULL, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return (int)e;
         told.fetch_or(bit);
     }
@@ -747,13 +751,13 @@ int launch(const Args& a, int n_seqs, long long tiles, cudaStream_t stream) {
     }
     cfg.attrs = attr;
     cfg.numAttrs = na;
-    e = cudaLaunchKernelEx(&cfg, prefill_8bit_kernel<CODE, HD, SPLIT>, a);
+    e = cudaLaunchKernelEx(&cfg, prefill_8bit_kernel<CODE, HD, FULL, SPLIT>, a);
     return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
 }  // namespace
 
-// Prompt portions as sandy_attention_8bit (attention_8bit.cu) takes them, without splits.  bfloat16, heads of 64 and 128, pages of a multiple
+// Prompt portions as sandy_attention_8bit (attention_8bit.cu) takes them, without splits.  bfloat16, heads of up to 128, pages of a multiple
 // of 16 keys, rows of q and out on 16 bytes, a positive scale, no bias by distance; SANDY_ERR_UNSUPPORTED for everything else, which the
 // other kernel takes.
 SANDY_API int sandy_prefill_attention_8bit_tc(const SandyAttend8* r, cudaStream_t stream) {
@@ -767,7 +771,7 @@ SANDY_API int sandy_prefill_attention_8bit_tc(const SandyAttend8* r, cudaStream_
     if (c.dtype != SANDY_BF16 || rules.dist_bias || rules.window < 0 || rules.keep_first < 0 || rules.chunk < 0 || !(rules.softcap >= 0.0f) ||
         (rules.keep_first > 0 && rules.chunk > 0) || (rules.elem_gate && rules.gate_dim < 1) || !(r->scale > 0.0f))
         return SANDY_ERR_UNSUPPORTED;
-    if ((c.head_dim != 64 && c.head_dim != 128) || c.page_size % 16 || c.n_kv_heads < 1 || r->n_heads % c.n_kv_heads) return SANDY_ERR_UNSUPPORTED;
+    if (c.head_dim < 16 || c.head_dim > 128 || c.head_dim % 16 || c.page_size % 16 || c.n_kv_heads < 1 || r->n_heads % c.n_kv_heads) return SANDY_ERR_UNSUPPORTED;
     if (c.page_stride % 16 || (((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)r->q | (uintptr_t)r->out) & 15) || r->ld_q % 8 || r->ld_out % 8 ||
         r->n_z > 65535 || r->num_splits < 0 || r->num_splits > 8 || (r->num_splits & (r->num_splits - 1)) || (long long)r->max_n * (r->n_heads / c.n_kv_heads) > 65535 * 256ll)
         return SANDY_ERR_UNSUPPORTED;
@@ -798,6 +802,7 @@ SANDY_API int sandy_prefill_attention_8bit_tc(const SandyAttend8* r, cudaStream_
     a.page_size = c.page_size;
     a.page_shift = (c.page_size & (c.page_size - 1)) == 0 ? __builtin_ctz(c.page_size) : -1;
     a.num_pages = c.num_pages;
+    a.head_dim = c.head_dim;
     a.window = rules.window;
     a.keep_first = rules.keep_first;
     a.chunk = rules.chunk;
@@ -814,12 +819,18 @@ SANDY_API int sandy_prefill_attention_8bit_tc(const SandyAttend8* r, cudaStream_
         a.splits = 1;
         while (a.splits < 8 && blocks * a.splits * 2 <= sandy_sm_count() && r->max_keys >= a.splits * 2 * BN) a.splits *= 2;
     }
-#define LAUNCH(CODE, HD) \
-    return a.splits > 1 ? launch<CODE, HD, true>(a, r->n_z, tiles, stream) : launch<CODE, HD, false>(a, r->n_z, tiles, stream)
-    if (c.code == SANDY_E4M3 && c.head_dim == 64) LAUNCH(SANDY_E4M3, 64);
-    if (c.code == SANDY_E4M3 && c.head_dim == 128) LAUNCH(SANDY_E4M3, 128);
-    if (c.code == SANDY_INT8 && c.head_dim == 64) LAUNCH(SANDY_INT8, 64);
-    if (c.code == SANDY_INT8 && c.head_dim == 128) LAUNCH(SANDY_INT8, 128);
+#define LAUNCH(CODE, HD, FULL) \
+    return a.splits > 1 ? launch<CODE, HD, FULL, true>(a, r->n_z, tiles, stream) : launch<CODE, HD, FULL, false>(a, r->n_z, tiles, stream)
+#define SIZES(CODE)                                         \
+    do {                                                    \
+        if (c.head_dim == 64) LAUNCH(CODE, 64, true);       \
+        if (c.head_dim == 128) LAUNCH(CODE, 128, true);     \
+        if (c.head_dim < 64) LAUNCH(CODE, 64, false);       \
+        LAUNCH(CODE, 128, false);                           \
+    } while (0)
+    if (c.code == SANDY_E4M3) SIZES(SANDY_E4M3);
+    if (c.code == SANDY_INT8) SIZES(SANDY_INT8);
+#undef SIZES
 #undef LAUNCH
     return SANDY_ERR_UNSUPPORTED;
 }

@@ -754,7 +754,7 @@ def _attention_8bit(what, q, cache, block_table, width, token_seq, positions, q_
     if q_start is None:
         tc = False
     elif tc is None:
-        tc = not num_splits and max_n * n_heads >= TC_ROWS_8BIT * hkv and dtype == BF16 and d in (64, 128) and ps % 16 == 0 and scale > 0 \
+        tc = not num_splits and max_n * n_heads >= TC_ROWS_8BIT * hkv and dtype == BF16 and d <= 128 and ps % 16 == 0 and scale > 0 \
             and not laid[6] and not (q_at | out_at) % 16 and not (ld[0] | ld[1]) % 8
     max_keys = min(width * ps, window + laid[1] + max_n if window else 1 << 30)
     splits, floats = (num_splits, 0) if tc else _splits8(T, n_z, max_n, n_heads, hkv, d, max_keys, dtype, num_splits)
@@ -801,7 +801,7 @@ def prefill_attention_8bit(q, cache: Cache8, block_table, q_start, kv_before, ou
     """Attention of prompt portions over a cache in 8 bits: request s of the block table's rows brings rows q_start[s] ..
     q_start[s + 1] - 1 (int32 [S + 1]) at its positions kv_before[s] on (int32 [S]), whose keys and values kv_append_8bit has
     written; max_q_len: the most that one request brings.  Types, sizes and rules as in decode_attention_8bit; portions of one
-    token are allowed.  Rows of no request are left as they were.  tc: True asks for the tcgen05 kernel (bfloat16, heads of 64 or 128,
+    token are allowed.  Rows of no request are left as they were.  tc: True asks for the tcgen05 kernel (bfloat16, heads of up to 128,
     pages of a multiple of 16 keys, rows of q and out on 16-byte boundaries, a positive scale, no bias by distance), False for the
     mma.sync one, None picks (the latter where num_splits is given; the tcgen05 kernel takes 1, 2, 4 and 8)."""
     what = "prefill_attention_8bit"

@@ -357,6 +357,15 @@ def test_prompt_portions_on_tcgen05_in_so_many_splits(code, splits, H, hkv, d, p
     _check_attention(code, "bf16", H, hkv, d, ps, seqs, False, splits=splits, tc=True, **rules)
 
 
+@pytest.mark.parametrize("code", list(CODES))
+@pytest.mark.parametrize("splits", [0, 1, 4, 8])
+@pytest.mark.parametrize("H,hkv,d,ps", [(3, 3, 16, 16), (6, 2, 32, 16), (8, 2, 48, 32), (4, 4, 80, 16), (5, 1, 96, 16), (2, 2, 112, 48)])
+def test_prompt_portions_on_tcgen05_of_other_head_sizes(code, splits, H, hkv, d, ps):
+    """The last page of the cache is used, whose rows' ends are the memory's."""
+    _check_attention(code, "bf16", H, hkv, d, ps, [(0, 300), (130, 40), (0, 1)], False, splits=splits, tc=True)
+    _check_attention(code, "bf16", H, hkv, d, ps, [(700, 90)], False, splits=splits, tc=True, window=100, keep_first=5, sink=True, elem_gate=11)
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("rules", [r for r in RULES if "dist_bias" not in r], ids=lambda r: "-".join(r))
 def test_rules_on_tcgen05(d, rules):
@@ -366,7 +375,7 @@ def test_rules_on_tcgen05(d, rules):
 def test_calls_the_tcgen05_kernel_does_not_take():
     from sandyrt_b200.errors import UnsupportedShape
 
-    for H, hkv, d, ps, dtype, rules in ((2, 2, 64, 8, "bf16", {}), (2, 2, 96, 16, "bf16", {}), (2, 2, 64, 16, "bf16", dict(dist_bias=True))):
+    for H, hkv, d, ps, dtype, rules in ((2, 2, 64, 8, "bf16", {}), (2, 2, 256, 16, "bf16", {}), (2, 2, 64, 16, "bf16", dict(dist_bias=True))):
         with pytest.raises(UnsupportedShape):
             _check_attention("int8", dtype, H, hkv, d, ps, [(0, 70)], False, tc=True, **rules)
     with pytest.raises(UnsupportedShape):
