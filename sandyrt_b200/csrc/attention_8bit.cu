@@ -27,7 +27,10 @@
 // Roundings.  q is scaled by a power of two (2^eq) so that its largest element lies in [1, 2) and rounded to half precision:
 // exact for bfloat16 elements above 2^-14 of the largest, off by 2^-25 of it at most.  P rounds to 11 bits, the row sum is taken
 // before.  For float32 both are split into two half-precision pieces (22 bits), which lie in neighbouring columns; the two
-// columns' results are in the same lane and are added there.
+// columns' results are in the same lane and are added there.  The second piece is held times 2^11 (SECOND), so that it has its 11 bits
+// wherever the first has one: a number is off by 2^-22 of itself or 2^-36 of the largest, whichever is more.  At its own size it would end
+// where half precision does, at 2^-25 of the largest, and a hundred thousand weights of e^-18 beside one of 1 were missing in
+// the result, though not in the denominator.
 //
 // The maximum that a column refers to moves only when a score runs ahead of it by more than 2^8 (RESCALE); weights stay below 256.
 //
@@ -55,6 +58,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float SECOND = 2048.0f;        // what the second piece of a float32 number is multiplied by
 
 struct Args {
     const void* q;
@@ -409,8 +413,8 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
             for (int w = 0; w < 8; w++) {                // word w: dims 64 c + 16 t + 2 w, + 1; k-step w / 2
                 float x0 = x[c][2 * w] * down, x1 = x[c][2 * w + 1] * down;
                 if (P == 2 && (g & 1)) {                 // the second piece: what the first one leaves
-                    x0 -= __half2float(__float2half_rn(x0));
-                    x1 -= __half2float(__float2half_rn(x1));
+                    x0 = (x0 - __half2float(__float2half_rn(x0))) * SECOND;
+                    x1 = (x1 - __half2float(__float2half_rn(x1))) * SECOND;
                 }
                 qf[n][c * 4 + (w >> 1)][w & 1] = pack_half(x0, x1);
             }
@@ -508,7 +512,7 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int e = 0; e < Q2; e++) {
-                        float x = P == 2 ? sc[kt][n][2 * r] + sc[kt][n][2 * r + 1] : sc[kt][n][2 * r + e];
+                        float x = P == 2 ? fmaf(sc[kt][n][2 * r + 1], 1.0f / SECOND, sc[kt][n][2 * r]) : sc[kt][n][2 * r + e];
                         if (plainly) {
                             x = fmaf(x, ks[kt][r % R] * factor[n][e], ev[kt][r % R]);
                         } else {
@@ -575,7 +579,7 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                         l[n][e] = fmaf(w[e], inv[kt][r % R], l[n][e]);
                         if (some & NO_POWER) w[e] = x == -INFINITY ? 0.0f : w[e] * inv[kt][r % R] * vs_of(kt, r % R);
                     }
-                    if (P == 2) w[1] = w[0] - __half2float(__float2half_rn(w[0]));
+                    if (P == 2) w[1] = (w[0] - __half2float(__float2half_rn(w[0]))) * SECOND;
                     pf[n][r] = turn(pack_half(w[0], w[1]));
                 }
 #pragma unroll
@@ -634,7 +638,7 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                 for (int j = 0; j < CH * 4; j++)
 #pragma unroll
                     for (int r = 0; r < 2; r++)          // product j of a run of 64: dims 8 g + 2 j, + 1
-                        sm_o[warp][i][(j >> 2) * 64 + 8 * g + 2 * (j & 3) + r] = P == 2 ? o[j][n][2 * r] + o[j][n][2 * r + 1] : o[j][n][2 * r + e];
+                        sm_o[warp][i][(j >> 2) * 64 + 8 * g + 2 * (j & 3) + r] = P == 2 ? fmaf(o[j][n][2 * r + 1], 1.0f / SECOND, o[j][n][2 * r]) : o[j][n][2 * r + e];
             }
         }
     __syncthreads();
