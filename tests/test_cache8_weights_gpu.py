@@ -36,14 +36,14 @@ def _one_key_above(code, first_value, ps):
     return _made[key]
 
 
-def _check(code, dtype, first_value, path, n, H, splits, ps, tolerance):
+def _check(code, dtype, first_value, path, n, H, splits, ps, tolerance, above=True):
     from sandyrt_b200.csrc import ops
 
     plain, table, k, v = _one_key_above(code, first_value, ps)
     dev = _device_cache(plain)
     rng = np.random.default_rng(22)
     q = torch.from_numpy(rng.standard_normal((n, H, D))).to(TYPES[dtype])
-    q[:, :, 0] = 8.0
+    q[:, :, 0] = 8.0 if above else 0.0
     out = torch.empty(n, H * D, dtype=TYPES[dtype], device=DEV)
     pos = list(range(BEFORE, BEFORE + n))
     if path == "decode":
@@ -77,3 +77,11 @@ def test_float32_values_of_many_small_weights_at_heads_of_every_kernel():
     """The same through the kernels of odd pages (rows looked up one by one)."""
     _check("int8", "f32", 0.0, "decode", 2, 3, 0, 37, lambda want, v: 1e-4 * want.abs())
     _check("int8", "f32", 0.0, "prompt", 9, 2, 2, 37, lambda want, v: 1e-4 * want.abs())
+
+
+@pytest.mark.parametrize("code", list(CODES))
+@pytest.mark.parametrize("above", [True, False])
+@pytest.mark.parametrize("path,n,H", [("decode", 3, 4), ("decode", 2, 1), ("prompt", 40, 1)])
+def test_sums_over_many_keys_in_float32(code, path, n, H, above):
+    """100,000 keys walked by one block, so that a warp sums 25,000: small weights are not lost beside what the sums already hold."""
+    _check(code, "f32", 1.0, path, n, H, 1, 64, lambda want, v: _tolerance(torch.float32, want, v), above)
