@@ -436,7 +436,7 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
     // rows of the first product and columns of the second: key `my_key` (+ 8) of a tile for lane group g, see row_key()
     const int my_key = row_key(g);
     // float32: the sums of the groups before the last FOLD ones, and what they are to be multiplied by since.  The tensor cores cut what they
-    // add to a sum, and do not round it: 100,000 keys in one split were off by 1.4e-4 of the largest value.
+    // add to a sum, and do not round it: 100,000 keys in one split were off by 1.4e-4 of the largest value.  Costs 1 to 5%.
     float o_all[P == 2 ? CH * 4 : 1][NT][4], l_all[NT][Q2], since[NT][Q2];
     if (P == 2) {
 #pragma unroll
@@ -454,203 +454,203 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
         }
     };
     while (it < n_groups) {
-    for (const int stop = P == 2 ? min(n_groups, it + FOLD) : n_groups; it < stop; it++) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");      // group `it` has landed (a lane's own copies),
-        __syncwarp();                                                                  // and every lane's
-        const uint32_t k_at = ring + stage * STAGE, v_at = k_at + KT * 16 * DMAX;
-        // of keys my_key and my_key + 8 (RUN 16: of both) of the group's tiles: scales and what is made of them, flags
-        constexpr int R = RUN == 16 ? 1 : 2;
-        float ks[KT][R], ev[KT][R], inv[KT][R], vs[KT][R];
-        unsigned flags[KT][R];
+        for (const int stop = P == 2 ? min(n_groups, it + FOLD) : n_groups; it < stop; it++) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");      // group `it` has landed (a lane's own copies),
+            __syncwarp();                                                                  // and every lane's
+            const uint32_t k_at = ring + stage * STAGE, v_at = k_at + KT * 16 * DMAX;
+            // of keys my_key and my_key + 8 (RUN 16: of both) of the group's tiles: scales and what is made of them, flags
+            constexpr int R = RUN == 16 ? 1 : 2;
+            float ks[KT][R], ev[KT][R], inv[KT][R], vs[KT][R];
+            unsigned flags[KT][R];
 #pragma unroll
-        for (int kt = 0; kt < KT; kt++)
+            for (int kt = 0; kt < KT; kt++)
 #pragma unroll
-            for (int r = 0; r < R; r++) {
-                if constexpr (RUN != 0) {
-                    const float4 run = *reinterpret_cast<const float4*>(&known[warp][(HALVES * (it * KT + kt) + r) % 32].ks);
-                    ks[kt][r] = run.x;
-                    ev[kt][r] = run.y;
-                    inv[kt][r] = run.z;
-                    flags[kt][r] = __float_as_uint(run.w);
-                } else {
-                    size_t off = 0;
-                    int page = 0;
-                    const bool ok = row_of(nth_of(it, kt), first_of(nth_of(it, kt)) + my_key + 8 * r, off, page);
-                    ks[kt][r] = ok ? a.k_scale[(size_t)page * a.scale_stride + kvh] : 0.0f;
-                    vs[kt][r] = ok ? a.v_scale[(size_t)page * a.scale_stride + kvh] : 0.0f;
-                    flags[kt][r] = power_of(vs[kt][r], ev[kt][r], inv[kt][r]) | (ok ? HAS_PAGE : 0u);
+                for (int r = 0; r < R; r++) {
+                    if constexpr (RUN != 0) {
+                        const float4 run = *reinterpret_cast<const float4*>(&known[warp][(HALVES * (it * KT + kt) + r) % 32].ks);
+                        ks[kt][r] = run.x;
+                        ev[kt][r] = run.y;
+                        inv[kt][r] = run.z;
+                        flags[kt][r] = __float_as_uint(run.w);
+                    } else {
+                        size_t off = 0;
+                        int page = 0;
+                        const bool ok = row_of(nth_of(it, kt), first_of(nth_of(it, kt)) + my_key + 8 * r, off, page);
+                        ks[kt][r] = ok ? a.k_scale[(size_t)page * a.scale_stride + kvh] : 0.0f;
+                        vs[kt][r] = ok ? a.v_scale[(size_t)page * a.scale_stride + kvh] : 0.0f;
+                        flags[kt][r] = power_of(vs[kt][r], ev[kt][r], inv[kt][r]) | (ok ? HAS_PAGE : 0u);
+                    }
+                }
+
+            auto vs_of = [&](int kt, int r) { return RUN != 0 ? known[warp][(HALVES * (it * KT + kt) + r) % 32].vs : vs[kt][r]; };
+            unsigned every = HAS_PAGE | SEEN_BY_ALL, some = 0;          // flags that all of the group's keys have, that one has
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    every &= flags[kt][r];
+                    some |= flags[kt][r];
+                }
+            const bool plainly = RUN && every == (HAS_PAGE | SEEN_BY_ALL);       // no mask, no rule
+
+            // ---- S ----------------------------------------------------------------------------------------------------
+            float sc[KT][NT][4];
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++) {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[kt][n][e] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < CH; c++) {
+                    unsigned w0[4], w1[4];                    // 16 dims of keys my_key, my_key + 8
+                    lds128(w0, k_at + (kt * 16 + my_key) * DMAX + swizzled<DMAX>(my_key, 4 * c + t) * 16);
+                    lds128(w1, k_at + (kt * 16 + my_key + 8) * DMAX + swizzled<DMAX>(my_key, 4 * c + t) * 16);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        unsigned a0, a1, a2, a3;
+                        decode4<CODE>(w0[i], a0, a2);
+                        decode4<CODE>(w1[i], a1, a3);
+#pragma unroll
+                        for (int n = 0; n < NT; n++) mma_f16(sc[kt][n], a0, a1, a2, a3, qf[n][c * 4 + i][0], qf[n][c * 4 + i][1]);
+                    }
                 }
             }
 
-        auto vs_of = [&](int kt, int r) { return RUN != 0 ? known[warp][(HALVES * (it * KT + kt) + r) % 32].vs : vs[kt][r]; };
-        unsigned every = HAS_PAGE | SEEN_BY_ALL, some = 0;          // flags that all of the group's keys have, that one has
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                every &= flags[kt][r];
-                some |= flags[kt][r];
-            }
-        const bool plainly = RUN && every == (HAS_PAGE | SEEN_BY_ALL);       // no mask, no rule
-
-        // ---- S ----------------------------------------------------------------------------------------------------
-        float sc[KT][NT][4];
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++) {
+            // ---- x = score + log2 of the value's scale, -inf where the key is not seen ------------------------------------
+            float top[NT][Q2];
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) sc[kt][n][e] = 0.0f;
+                for (int e = 0; e < Q2; e++) top[n][e] = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < CH; c++) {
-                unsigned w0[4], w1[4];                    // 16 dims of keys my_key, my_key + 8
-                lds128(w0, k_at + (kt * 16 + my_key) * DMAX + swizzled<DMAX>(my_key, 4 * c + t) * 16);
-                lds128(w1, k_at + (kt * 16 + my_key + 8) * DMAX + swizzled<DMAX>(my_key, 4 * c + t) * 16);
+            for (int kt = 0; kt < KT; kt++) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    unsigned a0, a1, a2, a3;
-                    decode4<CODE>(w0[i], a0, a2);
-                    decode4<CODE>(w1[i], a1, a3);
+                for (int r = 0; r < 2; r++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++) mma_f16(sc[kt][n], a0, a1, a2, a3, qf[n][c * 4 + i][0], qf[n][c * 4 + i][1]);
-                }
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < Q2; e++) {
+                            float x = P == 2 ? fmaf(sc[kt][n][2 * r + 1], 1.0f / SECOND, sc[kt][n][2 * r]) : sc[kt][n][2 * r + e];
+                            if (plainly) {
+                                x = fmaf(x, ks[kt][r % R] * factor[n][e], ev[kt][r % R]);
+                            } else {
+                                const int j = first_of(nth_of(it, kt)) + my_key + 8 * r;
+                                const bool visible = (flags[kt][r % R] & HAS_PAGE) && j <= pos[n][e] && (j >= lo[n][e] || j < a.keep_first);
+                                x *= ks[kt][r % R] * factor[n][e];
+                                if (!plain) {
+                                    if (a.softcap > 0.0f) x = a.softcap * (P == 2 ? tanhf(x / a.softcap) : tanh_fast(x / a.softcap));
+                                    if (a.dist_bias && visible)
+                                        x += a.dist_bias[(size_t)head_of(tile * QT + (n * 8 + 2 * t) / P + e) * a.n_dist + min(pos[n][e] - j, a.n_dist - 1)];
+                                    x *= LOG2E;
+                                }
+                                x = visible ? x + ev[kt][r % R] : -INFINITY;
+                            }
+                            sc[kt][n][P == 2 ? 2 * r : 2 * r + e] = x;
+                            top[n][e] = fmaxf(top[n][e], x);
+                        }
             }
-        }
-
-        // ---- x = score + log2 of the value's scale, -inf where the key is not seen ------------------------------------
-        float top[NT][Q2];
+            // The column's reference moves when a score has run far ahead of it (always on the first keys), for the whole warp together.
+            bool move = false;
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < Q2; e++) top[n][e] = -INFINITY;
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++) {
-#pragma unroll
-            for (int r = 0; r < 2; r++)
+                for (int e = 0; e < Q2; e++) move |= top[n][e] > M[n][e] + RESCALE;
+            if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int e = 0; e < Q2; e++) {
-                        float x = P == 2 ? fmaf(sc[kt][n][2 * r + 1], 1.0f / SECOND, sc[kt][n][2 * r]) : sc[kt][n][2 * r + e];
-                        if (plainly) {
-                            x = fmaf(x, ks[kt][r % R] * factor[n][e], ev[kt][r % R]);
-                        } else {
-                            const int j = first_of(nth_of(it, kt)) + my_key + 8 * r;
-                            const bool visible = (flags[kt][r % R] & HAS_PAGE) && j <= pos[n][e] && (j >= lo[n][e] || j < a.keep_first);
-                            x *= ks[kt][r % R] * factor[n][e];
-                            if (!plain) {
-                                if (a.softcap > 0.0f) x = a.softcap * (P == 2 ? tanhf(x / a.softcap) : tanh_fast(x / a.softcap));
-                                if (a.dist_bias && visible)
-                                    x += a.dist_bias[(size_t)head_of(tile * QT + (n * 8 + 2 * t) / P + e) * a.n_dist + min(pos[n][e] - j, a.n_dist - 1)];
-                                x *= LOG2E;
+                        const float m = fmaxf(M[n][e], max_over_groups(top[n][e]));
+                        const float shrink = m == -INFINITY ? 1.0f : ex2(M[n][e] - m);
+                        M[n][e] = m;
+                        l[n][e] *= shrink;
+                        if (P == 2) since[n][e] *= shrink;
+#pragma unroll
+                        for (int j = 0; j < CH * 4; j++) {
+                            o[j][n][e] *= shrink;
+                            o[j][n][e + 2] *= shrink;
+                            if (P == 2) {
+                                o[j][n][1] *= shrink;
+                                o[j][n][3] *= shrink;
                             }
-                            x = visible ? x + ev[kt][r % R] : -INFINITY;
                         }
-                        sc[kt][n][P == 2 ? 2 * r : 2 * r + e] = x;
-                        top[n][e] = fmaxf(top[n][e], x);
                     }
-        }
-        // The column's reference moves when a score has run far ahead of it (always on the first keys), for the whole warp together.
-        bool move = false;
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int e = 0; e < Q2; e++) move |= top[n][e] > M[n][e] + RESCALE;
-        if (__any_sync(0xffffffffu, move)) {
+            }
+            float m_use[NT][Q2];                              // a column that has seen no key yet: its weights are 2^-inf
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int e = 0; e < Q2; e++) {
-                    const float m = fmaxf(M[n][e], max_over_groups(top[n][e]));
-                    const float shrink = m == -INFINITY ? 1.0f : ex2(M[n][e] - m);
-                    M[n][e] = m;
-                    l[n][e] *= shrink;
-                    if (P == 2) since[n][e] *= shrink;
+                for (int e = 0; e < Q2; e++) m_use[n][e] = M[n][e] == -INFINITY ? 0.0f : M[n][e];
+            // ---- weights, as the second operand; O ---------------------------------------------------------------------
 #pragma unroll
-                    for (int j = 0; j < CH * 4; j++) {
-                        o[j][n][e] *= shrink;
-                        o[j][n][e + 2] *= shrink;
-                        if (P == 2) {
-                            o[j][n][1] *= shrink;
-                            o[j][n][3] *= shrink;
+            for (int kt = 0; kt < KT; kt++) {
+                unsigned pf[NT][2];
+#pragma unroll
+                for (int r = 0; r < 2; r++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        // 2^(x - M) is the weight times the value's scale, where that is a power of two: what appending gives
+                        float w[2] = {0.0f, 0.0f};
+#pragma unroll
+                        for (int e = 0; e < Q2; e++) {
+                            const float x = sc[kt][n][P == 2 ? 2 * r : 2 * r + e];
+                            w[e] = ex2(x - m_use[n][e]);
+                            l[n][e] = fmaf(w[e], inv[kt][r % R], l[n][e]);
+                            if (some & NO_POWER) w[e] = x == -INFINITY ? 0.0f : w[e] * inv[kt][r % R] * vs_of(kt, r % R);
                         }
+                        if (P == 2) w[1] = (w[0] - __half2float(__float2half_rn(w[0]))) * SECOND;
+                        pf[n][r] = turn(pack_half(w[0], w[1]));
                     }
-                }
-        }
-        float m_use[NT][Q2];                              // a column that has seen no key yet: its weights are 2^-inf
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+                for (int c = 0; c < CH; c++) {
+                    unsigned vw[4][2];                        // dims 64 c + 8 g .. of the keys of the second product's columns 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-            for (int e = 0; e < Q2; e++) m_use[n][e] = M[n][e] == -INFINITY ? 0.0f : M[n][e];
-        // ---- weights, as the second operand; O ---------------------------------------------------------------------
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++) {
-            unsigned pf[NT][2];
-#pragma unroll
-            for (int r = 0; r < 2; r++)
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    // 2^(x - M) is the weight times the value's scale, where that is a power of two: what appending gives
-                    float w[2] = {0.0f, 0.0f};
-#pragma unroll
-                    for (int e = 0; e < Q2; e++) {
-                        const float x = sc[kt][n][P == 2 ? 2 * r : 2 * r + e];
-                        w[e] = ex2(x - m_use[n][e]);
-                        l[n][e] = fmaf(w[e], inv[kt][r % R], l[n][e]);
-                        if (some & NO_POWER) w[e] = x == -INFINITY ? 0.0f : w[e] * inv[kt][r % R] * vs_of(kt, r % R);
+                    for (int r = 0; r < 4; r++) {
+                        const int low = r & 1 ? 7 - t : t, row = low + 8 * (r >> 1);
+                        lds64(vw[r], v_at + (kt * 16 + row) * DMAX + swizzled<DMAX>(low, 4 * c + (g >> 1)) * 16 + (g & 1) * 8);
                     }
-                    if (P == 2) w[1] = (w[0] - __half2float(__float2half_rn(w[0]))) * SECOND;
-                    pf[n][r] = turn(pack_half(w[0], w[1]));
-                }
 #pragma unroll
-            for (int c = 0; c < CH; c++) {
-                unsigned vw[4][2];                        // dims 64 c + 8 g .. of the keys of the second product's columns 2t, 2t + 1, 2t + 8, 2t + 9
+                    for (int half = 0; half < 2; half++) {
+                        unsigned w[4];
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int low = r & 1 ? 7 - t : t, row = low + 8 * (r >> 1);
-                    lds64(vw[r], v_at + (kt * 16 + row) * DMAX + swizzled<DMAX>(low, 4 * c + (g >> 1)) * 16 + (g & 1) * 8);
-                }
+                        for (int r = 0; r < 4; r++) w[r] = vw[r][half];
+                        // bytes of two keys side by side: dims d, d + 1 and d + 2, d + 3 of the piece's four
+                        const unsigned e0 = __byte_perm(w[0], w[1], 0x5140), e1 = __byte_perm(w[0], w[1], 0x7362);
+                        const unsigned f0 = __byte_perm(w[2], w[3], 0x5140), f1 = __byte_perm(w[2], w[3], 0x7362);
+                        unsigned a0, a1, a2, a3;
+                        decode4<CODE>(e0, a0, a1);
+                        decode4<CODE>(f0, a2, a3);
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    unsigned w[4];
+                        for (int n = 0; n < NT; n++) mma_f16(o[c * 4 + half * 2][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+                        decode4<CODE>(e1, a0, a1);
+                        decode4<CODE>(f1, a2, a3);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) w[r] = vw[r][half];
-                    // bytes of two keys side by side: dims d, d + 1 and d + 2, d + 3 of the piece's four
-                    const unsigned e0 = __byte_perm(w[0], w[1], 0x5140), e1 = __byte_perm(w[0], w[1], 0x7362);
-                    const unsigned f0 = __byte_perm(w[2], w[3], 0x5140), f1 = __byte_perm(w[2], w[3], 0x7362);
-                    unsigned a0, a1, a2, a3;
-                    decode4<CODE>(e0, a0, a1);
-                    decode4<CODE>(f0, a2, a3);
-#pragma unroll
-                    for (int n = 0; n < NT; n++) mma_f16(o[c * 4 + half * 2][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
-                    decode4<CODE>(e1, a0, a1);
-                    decode4<CODE>(f1, a2, a3);
-#pragma unroll
-                    for (int n = 0; n < NT; n++) mma_f16(o[c * 4 + half * 2 + 1][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+                        for (int n = 0; n < NT; n++) mma_f16(o[c * 4 + half * 2 + 1][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+                    }
                 }
             }
+            __syncwarp();                                     // the stage may be written again
+            if (it + STAGES < n_groups) {
+                if constexpr (RUN != 0)
+                    if ((it + STAGES) * KT % BATCH == 0) look_up(it + STAGES);
+                copy(it + STAGES, stage);
+            }
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
+            asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        __syncwarp();                                     // the stage may be written again
-        if (it + STAGES < n_groups) {
-            if constexpr (RUN != 0)
-                if ((it + STAGES) * KT % BATCH == 0) look_up(it + STAGES);
-            copy(it + STAGES, stage);
+        if (P == 2 && n_groups > FOLD) {
+            fold();
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int j = 0; j < CH * 4; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[j][n][e] = it < n_groups ? 0.0f : o_all[P == 2 ? j : 0][n][e];
+                l[n][0] = it < n_groups ? 0.0f : l_all[n][0];
+                since[n][0] = 1.0f;
+            }
         }
-        stage = stage == STAGES - 1 ? 0 : stage + 1;
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    if (P == 2 && n_groups > FOLD) {
-        fold();
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-#pragma unroll
-            for (int j = 0; j < CH * 4; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[j][n][e] = it < n_groups ? 0.0f : o_all[P == 2 ? j : 0][n][e];
-            l[n][0] = it < n_groups ? 0.0f : l_all[n][0];
-            since[n][0] = 1.0f;
-        }
-    }
     }
     __syncthreads();                                      // no stage is in use any more
     if (a.in_cluster) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
