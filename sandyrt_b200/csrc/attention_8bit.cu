@@ -19,10 +19,12 @@
 // quarter warp's reads of keys and half a warp's of values meet all banks.  Pages and scales of the next 16 tiles are looked up at
 // once, a run of keys a lane, so that the chain from the block table over the scale to the copy is not walked for every tile.
 //
-// Scales.  A score is S * sk * (2^eq * scale), a factor a key.  A value's scale joins the weight: with M the running maximum of
-// s_j + log2(sv_j) (s in units of log 2), p_j = 2^(s_j - M) is summed for the denominator and p_j * sv_j <= 1 (2 if the scale is
-// no power of two) is rounded to half precision for the product.  No block's values are out of half precision's range
-// this way, and nothing is lost that would count beside the largest term.
+// Scales.  A score is S * sk * (2^eq * scale), a factor a key.  A value's scale joins the weight: with x_j = s_j + log2(sv_j) (s in units of
+// log 2) and a reference M near the largest x so far, 2^(x_j - M) / sv_j is summed for the denominator and 2^(x_j - M) is rounded to
+// half precision for the product.  No block's values are out of half precision's range this way.
+// M moves to HEADROOM = 7 below the largest x, and only when an x is above M + RESCALE = 14: weights stay below 2^14 (2^15 where a scale is no
+// power of two), and what is 2^-32 of the largest still rounds to something.  With the largest at 1, all of e^-18 and
+// below was nothing: 100,000 such keys were missing in the result, though not in the denominator.
 //
 // Roundings.  q is scaled by a power of two (2^eq) so that its largest element lies in [1, 2) and rounded to half precision:
 // exact for bfloat16 elements above 2^-14 of the largest, off by 2^-25 of it at most.  P rounds to 11 bits, the row sum is taken
@@ -31,8 +33,6 @@
 // wherever the first has one: a number is off by 2^-22 of itself or 2^-36 of the largest, whichever is more.  At its own size it would end
 // where half precision does, at 2^-25 of the largest, and a hundred thousand weights of e^-18 beside one of 1 were missing in
 // the result, though not in the denominator.
-//
-// The maximum that a column refers to moves only when a score runs ahead of it by more than 2^8 (RESCALE); weights stay below 256.
 //
 // What bounds it.  Single tokens: the codes' bytes.  16 warps an SM (in blocks of four, or two where there are very many) with
 // three stages of 4 KB each keep 190 KB on their way.  Where there are few requests `num_splits` blocks share one's keys: up to 8 are a
@@ -175,7 +175,8 @@ __device__ __forceinline__ void finish(const Args& a, float O, float L, float M,
     ((T*)a.out)[(size_t)row * a.ld_out + (size_t)h * a.head_dim + d] = from_f32<T>(y);
 }
 
-constexpr float RESCALE = 8.0f;          // how far (in the exponent) a score may run ahead of the maximum its column refers to
+constexpr float RESCALE = 14.0f;         // how far (in the exponent) a score may be above the reference of its column
+constexpr float HEADROOM = 7.0f;         // how far below the largest score the reference is set
 
 // What a warp has looked up about a run of keys in one page: where its rows start (page 0's, if it has no page), its block's scales
 // and what is made of them: ev = log2 of the value's scale, inv = 2^-ev.
@@ -561,7 +562,7 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int e = 0; e < Q2; e++) {
-                        const float m = fmaxf(M[n][e], max_over_groups(top[n][e]));
+                        const float m = fmaxf(M[n][e], max_over_groups(top[n][e]) - HEADROOM);
                         const float shrink = m == -INFINITY ? 1.0f : ex2(M[n][e] - m);
                         M[n][e] = m;
                         l[n][e] *= shrink;

@@ -18,8 +18,8 @@
 //                    key tile follows P V of this one; both tiles' S and O fill the 512 columns of tensor memory at heads of 128.
 // Head sizes between are the next of 64 and 128 with zeros behind their dims, in shared memory alone: 12 requests of 800 tokens behind
 // 1,000, 9 heads of 48, 105 us (the mma.sync kernel 492); 12 prompts of 400, 12 heads of 80, 33 (173); 8 heads of 16, 500 tokens, 13 (24).
-// The accumulators stay in tensor memory over all tiles and are rescaled there only when a row's maximum has run ahead of its reference
-// by more than 2^8 (P stays below 256).  When S of a tile is there, the products before it are complete: O is at rest then.
+// The accumulators stay in tensor memory over all tiles and are rescaled there only when a row's maximum is more than 2^14 above its
+// reference, which then goes to 2^-7 of the maximum (attention_8bit.cu; P stays below 2^14).  When S of a tile is there, the products before it are complete: O is at rest then.
 //
 // What bounds it: 32,768 exponentials a pair of tiles are 2,048 cycles of the special-function units, the products at heads of 128
 // as much of the tensor cores; converting 32,768 codes is some 700 (int8) issue slots of each SM quarter.  256 rows a block halve the
@@ -52,7 +52,7 @@ constexpr int THREADS = 416;
 constexpr int FIRST_PRODUCER = 256, ISSUE_WARP = 12;
 constexpr int STAGES = 2;
 constexpr int CONSTS = 8;                // key tiles whose scales and pages are kept
-constexpr float RESCALE = 8.0f;
+constexpr float RESCALE = 14.0f, HEADROOM = 7.0f;     // of a row's reference, see attention_8bit.cu
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr uint32_t HALF_TILE = 128 * 128;            // 128 rows of 64 half-precision numbers
 
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
             }
             const bool move = top > M + RESCALE;
             if (__any_sync(0xffffffffu, move)) {
-                const float alpha = move ? ex2(M - top) : 1.0f;      // 0 on the row's first keys
+                const float next = top - HEADROOM, alpha = move ? ex2(M - next) : 1.0f;      // 0 on the row's first keys
                 if (it > 0) {
 #pragma unroll 1
                     for (int c = 0; c < HD / 16; c++) {
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
                     tmem_wait_st();
                 }
                 l *= alpha;
-                if (move) M = top;
+                if (move) M = next;
             }
             const float m_use = M == -INFINITY ? 0.0f : M;           // no key yet: weights are 2^-inf
             if (whole) {

@@ -85,3 +85,51 @@ def test_float32_values_of_many_small_weights_at_heads_of_every_kernel():
 def test_sums_over_many_keys_in_float32(code, path, n, H, above):
     """100,000 keys walked by one block, so that a warp sums 25,000: small weights are not lost beside what the sums already hold."""
     _check(code, "f32", 1.0, path, n, H, 1, 64, lambda want, v: _tolerance(torch.float32, want, v), above)
+
+
+def _half_tolerance(want, v):
+    """The result's rounding (2^-8 of it) and its two columns' worth of sums (2^-9), and half a step of half precision's smallest numbers,
+    2^-25 beside a reference of 2^-7 of the largest weight: 2^-32 of the largest value a key."""
+    return want.abs() * (2.0 ** -8 + 2.0 ** -9) + BEFORE * 2.0 ** -32 * float(v.abs().max())
+
+
+@pytest.mark.parametrize("code", list(CODES))
+@pytest.mark.parametrize("first_value", [1.0, 0.0])
+@pytest.mark.parametrize("path,n,H,splits", [("decode", 1, 1, 0), ("decode", 3, 4, 1), ("decode", 2, 8, 40), ("prompt", 5, 2, 0), ("prompt", 40, 1, 1), ("tcgen05", 40, 1, 0),
+                                             ("tcgen05", 33, 4, 1), ("tcgen05", 40, 2, 8)])
+def test_small_weights_together_in_bfloat16(code, first_value, path, n, H, splits):
+    """The same as in float32: where the first key's value is 0, as that of a token that takes what attention is left over, the others'
+    1.5e-3 are all there is."""
+    _check(code, "bf16", first_value, path, n, H, splits, 64, _half_tolerance)
+
+
+def test_small_weights_together_beside_scales_that_are_no_powers_of_two():
+    """The largest weights there are, 2^14 and what a scale is beside its power of two, do not pass half precision's range: scores that
+    rise by a little less than what moves the reference, in every tile."""
+    from sandyrt_b200.csrc import ops
+
+    n, hkv = 400, 1
+    rng = np.random.default_rng(5)
+    k = torch.zeros(n, hkv, D, dtype=torch.float64)
+    k[:, 0, 0] = torch.arange(n) // 16 % 2 * 9.0                 # with q's first element 8 and scale 1/8: 9 nats, 13 in units of log 2
+    v = torch.from_numpy(1.0 + 0.3 * rng.standard_normal((n, hkv, D)))
+    lists, table, pages = _tables(rng, [-(-n // 16)])
+    plain = PlainCache(pages, hkv, 16, D, torch.int8)
+    plain.append(k, v, lists, [0, n], [0])
+    plain.scales[1] = (plain.scales[1] * 1.99).float().double()
+    dev = _device_cache(plain)
+    q = torch.zeros(40, D)
+    q[:, 0] = 8.0
+    q = q.to(torch.bfloat16)
+    kk, vv = (plain.values(w, lists[0], n)[:, 0] for w in range(2))
+    for path in ("decode", "prompt", "tcgen05"):
+        out = torch.empty(40, D, dtype=torch.bfloat16, device=DEV)
+        pos = list(range(n - 40, n))
+        if path == "decode":
+            ops.decode_attention_8bit(q.to(DEV), dev, table, _i32([0] * 40), _i32(pos), out, n_heads=1, scale=SCALE, num_splits=1)
+        else:
+            ops.prefill_attention_8bit(q.to(DEV), dev, table, _i32([0, 40]), _i32([n - 40]), out, n_heads=1, max_q_len=40, scale=SCALE, num_splits=1, tc=path == "tcgen05")
+        ops.check_kernel_status(DEV)
+        want = torch.stack([torch.softmax(kk[:p + 1] @ q[0].double() * SCALE, 0) @ vv[:p + 1] for p in pos])
+        # the weights' rounding, and what a scale is beside its power of two times a code: 2^-11 of each term twice
+        assert bool(((out.cpu().double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -9)).all()), path
