@@ -507,6 +507,7 @@ def prefill_attention_f32(q, k_cache, v_cache, block_table, q_start, kv_before, 
 CODE_CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
 _V, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 _CACHE8 = "PPPPqqPP8i"                              # SandyCache8
+_LARGEST_F32 = torch.finfo(torch.float32).max
 _ROWS8 = struct.Struct("@" + _CACHE8 + "PPqqPPii")  # SandyRows8
 _ATTEND8 = struct.Struct("@" + _CACHE8 + "PPqqPPPP" + "iifiPPPiPii" + "6ifi")       # SandyAttend8
 assert (_ROWS8.size, _ATTEND8.size) == (152, 256)
@@ -677,6 +678,7 @@ def kv_read_8bit(cache: Cache8, block_table, first, out_start, k_out, v_out, *, 
 
 
 _RULES8 = {"window": 0, "keep_first": 0, "softcap": 0.0, "chunk": 0, "sink": None, "out_gate": None, "dist_bias": None, "elem_gate": None}
+MAX_SOFTCAP8 = 1e30               # the kernels divide scores by it
 _NO_RULES8 = (0, 0, 0.0, 0, 0, 0, 0, 0, 0, 0, 0)
 
 
@@ -698,6 +700,8 @@ def _rules8(what: str, q, n_heads: int, rules: dict) -> tuple:
     T = q.shape[0]
     if min(window, keep_first, chunk) < 0 or not softcap >= 0 or (keep_first and chunk):
         raise UnsupportedShape(f"{what}: window, keep_first, softcap and chunk must not be negative, kept first keys and chunks not together")
+    if max(window, keep_first, chunk) >= 1 << 31 or softcap > MAX_SOFTCAP8:
+        raise UnsupportedShape(f"{what}: window, keep_first and chunk are 32-bit numbers, a cap at most {MAX_SOFTCAP8:g} (0: none)")
     if sink is not None and (sink.dtype != torch.float32 or sink.shape != (n_heads,) or not sink.is_contiguous()):
         raise KernelError(f"{what}: a sink is a dense float32 [H]")
     if out_gate is not None and (out_gate.dtype != torch.float32 or out_gate.shape != (T, n_heads) or not out_gate.is_contiguous()):
@@ -745,6 +749,8 @@ def _attention_8bit(what, q, cache, block_table, width, token_seq, positions, q_
     laid, extra = (_NO_RULES8, ()) if _plain_rules8(rules) else _rules8(what, q, n_heads, rules)
     if num_splits < 0 or num_splits > 256:
         raise KernelError(f"{what}: num_splits must lie in 0 .. 256 (0: the kernel's choice)")
+    if not abs(scale) <= _LARGEST_F32:
+        raise KernelError(f"{what}: the scale must be a finite float32 number")
     index = _one_device(what, q, out, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, token_seq, positions, q_start, *extra)
     if n_z == 0 or max_n == 0 or T == 0:
         return
@@ -756,7 +762,7 @@ def _attention_8bit(what, q, cache, block_table, width, token_seq, positions, q_
     elif tc is None:
         tc = not num_splits and max_n * n_heads >= TC_ROWS_8BIT * hkv and dtype == BF16 and d <= 128 and ps % 16 == 0 and scale > 0 \
             and not laid[6] and not (q_at | out_at) % 16 and not (ld[0] | ld[1]) % 8
-    max_keys = min(width * ps, window + laid[1] + max_n if window else 1 << 30)
+    max_keys = min(width * ps, window + laid[1] + max_n if window else 1 << 30, 1 << 30)
     splits, floats = (num_splits, 0) if tc else _splits8(T, n_z, max_n, n_heads, hkv, d, max_keys, dtype, num_splits)
     # partial results of many splits: memory of the stream the call is on, given back to the allocator when it returns
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
