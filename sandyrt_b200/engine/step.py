@@ -215,14 +215,20 @@ class Engine:
             raise StepError("a text to score needs at least one token")
         if portion < 1 or not 0 <= top <= min(ops.MAX_TOP_LOGPROBS, self.vocab_size):
             raise StepError(f"score: a portion is at least one token, top 0 .. {min(ops.MAX_TOP_LOGPROBS, self.vocab_size)}")
+        if min(ids) < 0 or max(ids) >= self.vocab_size:               # the first token of a portion is asked for a portion earlier
+            raise StepError(f"score: a token id is outside the vocabulary of {self.vocab_size}")
         rid, got = ("score", object()), []
-        self.admit(rid)
+        try:
+            self.admit(rid)
+        except BaseException:                                         # no slot is free
+            self.ids.forget(rid)
+            raise
         try:
             for at in range(0, len(ids), portion):
                 part = ids[at:at + portion]
                 n = len(part)
                 logits = self.step([StepEntry(rid, part, want=range(n))])
-                self.check_status()                               # a token outside the vocabulary
+                self.check_status()
                 with torch.cuda.device(logits.device):
                     made = lambda *shape, dtype=torch.float32: torch.empty(*shape, dtype=dtype, device=logits.device)
                     given = torch.tensor((ids[at + 1:at + n + 1] + [-1])[:n], dtype=torch.int32).to(logits.device)

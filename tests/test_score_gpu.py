@@ -72,6 +72,41 @@ def test_score_leaves_other_requests_alone_and_refuses(model_dirs):
     assert np.array_equal(scores[1].logprobs, llm.score(prompt)[0].logprobs)
 
 
+@pytest.mark.parametrize("at", [0, 1, 4, 5, 7, 8])
+@pytest.mark.parametrize("bad", [-1, "vocab", 1 << 31, -(1 << 40)])
+def test_score_names_a_token_outside_the_vocabulary(model_dirs, at, bad):
+    """Wherever in a portion of 4 it stands: the first token of a portion is asked for with the portion before it."""
+    from sandyrt_b200.engine.step import Engine
+    from sandyrt_b200.errors import StepError
+    from sandyrt_b200.models.model import load_model
+
+    engine = Engine(load_model(model_dirs["A"], device="cuda:0", dtype=torch.float32), max_tokens=64, max_requests=2)
+    free, ids = engine.cache.alloc.free_pages(0), _text("A", 9, 2)
+    want = engine.score(ids, portion=4)
+    wrong = list(ids)
+    wrong[at] = TINY["A"]["vocab_size"] if bad == "vocab" else bad
+    with pytest.raises(StepError, match="token id is outside the vocabulary"):
+        engine.score(wrong, portion=4)
+    assert engine.cache.alloc.free_pages(0) == free and not engine.cache.alloc.live()
+    assert np.array_equal(engine.score(ids, portion=4).logprobs, want.logprobs)
+
+
+def test_score_without_a_free_slot_leaves_nothing_behind(model_dirs):
+    from sandyrt_b200.engine.step import Engine
+    from sandyrt_b200.errors import NoFreeSlot
+    from sandyrt_b200.models.model import load_model
+
+    engine = Engine(load_model(model_dirs["A"], device="cuda:0", dtype=torch.float32), max_tokens=64, max_requests=1)
+    engine.admit("mine")
+    known = dict(engine.ids._to_int)
+    for _ in range(3):
+        with pytest.raises(NoFreeSlot):
+            engine.score([1, 2, 3])
+    assert engine.ids._to_int == known
+    engine.release("mine")
+    assert engine.score([1, 2, 3]).logprobs.shape == (2,)
+
+
 def test_score_on_the_command_line(model_dirs, capsys):
     from sandyrt_b200.cli import main
 
