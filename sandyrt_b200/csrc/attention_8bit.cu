@@ -151,7 +151,8 @@ __device__ __forceinline__ Portion portion_of(const Args& a, int z) {
     p.row0 = a.q_start ? a.q_start[z] : z;
     p.n = a.q_start ? a.q_start[z + 1] - p.row0 : 1;
     p.before = a.positions[z];
-    if (p.row0 < 0 || p.n > a.n_rows - p.row0 || p.n > a.max_n) {    // rows that are not there, or no block is there for
+    // rows that are not there, or no block is there for, or whose positions are no int
+    if (p.row0 < 0 || p.n > a.n_rows - p.row0 || p.n > a.max_n || (long long)p.before + p.n - 1 > 0x7fffffffll) {
         if (p.n > 0 && a.status && threadIdx.x == 0) atomicOr(a.status, 16);
         p.n = 0;
     }

@@ -171,7 +171,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_8bit_kernel(const __grid_c
     const int z = blockIdx.y, kvh = SPLIT ? blockIdx.x / a.splits : blockIdx.x, nth = blockIdx.z;
     const int rank = SPLIT ? blockIdx.x - kvh * a.splits : 0;
     const int row0 = a.q_start[z], n = a.q_start[z + 1] - row0, before = a.kv_before[z];
-    const bool there = row0 >= 0 && n <= a.n_rows - row0 && n <= a.max_n;      // the portion's rows, and blocks for them
+    // the portion's rows, blocks for them, and positions that are ints
+    const bool there = row0 >= 0 && n <= a.n_rows - row0 && n <= a.max_n && (long long)before + n - 1 <= 0x7fffffffll;
     if (!there && n > 0 && threadIdx.x == 0 && a.status) atomicOr(a.status, 16);
     const int tiles = there && n > 0 ? (int)(((long long)n * a.group + 255) / 256) : 0;
     if (nth >= tiles) return;

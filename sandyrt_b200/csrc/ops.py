@@ -807,7 +807,8 @@ def prefill_attention_8bit(q, cache: Cache8, block_table, q_start, kv_before, ou
     """Attention of prompt portions over a cache in 8 bits: request s of the block table's rows brings rows q_start[s] ..
     q_start[s + 1] - 1 (int32 [S + 1]) at its positions kv_before[s] on (int32 [S]), whose keys and values kv_append_8bit has
     written; max_q_len: the most that one request brings.  Types, sizes and rules as in decode_attention_8bit; portions of one
-    token are allowed.  Rows of no request are left as they were.  tc: True asks for the tcgen05 kernel (bfloat16, heads of up to 128,
+    token are allowed.  Rows of no request are left as they were, and those of a portion that is longer than max_q_len, that brings rows
+    that are not there or whose positions pass 2^31 - 1, which is reported.  tc: True asks for the tcgen05 kernel (bfloat16, heads of up to 128,
     pages of a multiple of 16 keys, rows of q and out on 16-byte boundaries, a positive scale, no bias by distance), False for the
     mma.sync one, None picks (the latter where num_splits is given; the tcgen05 kernel takes 1, 2, 4 and 8)."""
     what = "prefill_attention_8bit"
