@@ -541,7 +541,7 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                                 const bool visible = (flags[kt][r % R] & HAS_PAGE) && j <= pos[n][e] && (j >= lo[n][e] || j < a.keep_first);
                                 x *= ks[kt][r % R] * factor[n][e];
                                 if (!plain) {
-                                    if (a.softcap > 0.0f) x = a.softcap * (P == 2 ? tanhf(x / a.softcap) : tanh_fast(x / a.softcap));
+                                    if (a.softcap > 0.0f) x = a.softcap * (P == 2 ? tanhf(x / a.softcap) : tanh_capped(x / a.softcap));
                                     if (a.dist_bias && visible)
                                         x += a.dist_bias[(size_t)head_of(tile * QT + (n * 8 + 2 * t) / P + e) * a.n_dist + min(pos[n][e] - j, a.n_dist - 1)];
                                     x *= LOG2E;

@@ -761,7 +761,7 @@ def _attention_8bit(what, q, cache, block_table, width, token_seq, positions, q_
         tc = False
     elif tc is None:
         tc = not num_splits and max_n * n_heads >= TC_ROWS_8BIT * hkv and dtype == BF16 and d <= 128 and ps % 16 == 0 and scale > 0 \
-            and not laid[6] and not (q_at | out_at) % 16 and not (ld[0] | ld[1]) % 8
+            and not laid[6] and laid[2] <= 512 and not (q_at | out_at) % 16 and not (ld[0] | ld[1]) % 8
     max_keys = min(width * ps, window + laid[1] + max_n if window else 1 << 30, 1 << 30)
     splits, floats = (num_splits, 0) if tc else _splits8(T, n_z, max_n, n_heads, hkv, d, max_keys, dtype, num_splits)
     # partial results of many splits: memory of the stream the call is on, given back to the allocator when it returns
@@ -809,7 +809,7 @@ def prefill_attention_8bit(q, cache: Cache8, block_table, q_start, kv_before, ou
     written; max_q_len: the most that one request brings.  Types, sizes and rules as in decode_attention_8bit; portions of one
     token are allowed.  Rows of no request are left as they were, and those of a portion that is longer than max_q_len, that brings rows
     that are not there or whose positions pass 2^31 - 1, which is reported.  tc: True asks for the tcgen05 kernel (bfloat16, heads of up to 128,
-    pages of a multiple of 16 keys, rows of q and out on 16-byte boundaries, a positive scale, no bias by distance), False for the
+    pages of a multiple of 16 keys, rows of q and out on 16-byte boundaries, a positive scale, no bias by distance, no cap above 512), False for the
     mma.sync one, None picks (the latter where num_splits is given; the tcgen05 kernel takes 1, 2, 4 and 8)."""
     what = "prefill_attention_8bit"
     S, width = _requests8(what, _layout(block_table), _layout(q_start), _layout(kv_before))

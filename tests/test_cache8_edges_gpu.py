@@ -30,3 +30,21 @@ def test_portions_past_the_last_position(tc, dtype):
         with pytest.raises(KernelError, match="status 16"):
             ops.check_kernel_status(DEV)
         assert bool((got[:4] == 3).all()) and torch.equal(got[4:], want[4:])
+
+
+@pytest.mark.parametrize("softcap", [0.5, 50.0, 3e3, 1e5, 1e7, 1e30])
+@pytest.mark.parametrize("path", ["decode", "mma", "chosen"])
+def test_caps_of_every_size(softcap, path):
+    """A cap far above the scores changes nothing; its own size does not make their error larger.  Scores of some 30 beside each other."""
+    seqs = [(0, 1), (70, 1), (200, 1)] if path == "decode" else [(0, 60), (150, 40)]
+    _check_attention("int8", "bf16", 4, 2, 64, 16, seqs, path == "decode", q_scale=8.0, softcap=softcap, tc=False if path == "mma" else None)
+    if path != "chosen":
+        _check_attention("e4m3", "f32", 4, 2, 64, 16, seqs, path == "decode", softcap=softcap)
+
+
+def test_caps_that_the_tcgen05_kernel_takes():
+    from sandyrt_b200.errors import UnsupportedShape
+
+    _check_attention("int8", "bf16", 4, 2, 64, 16, [(0, 60), (150, 40)], False, q_scale=8.0, softcap=512.0, tc=True)
+    with pytest.raises(UnsupportedShape):
+        _check_attention("int8", "bf16", 4, 2, 64, 16, [(0, 60)], False, softcap=513.0, tc=True)
