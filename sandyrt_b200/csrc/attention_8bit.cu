@@ -59,6 +59,7 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float SECOND = 2048.0f;        // what the second piece of a float32 number is multiplied by
+constexpr float FAR = 8388608.0f;        // 2^23: the largest score, in units of log 2, under a cap or a bias
 constexpr int FOLD = 32;                 // groups of keys that a float32 warp sums by themselves
 
 struct Args {
@@ -544,7 +545,10 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
                                     if (a.softcap > 0.0f) x = a.softcap * (P == 2 ? tanhf(x / a.softcap) : tanh_capped(x / a.softcap));
                                     if (a.dist_bias && visible)
                                         x += a.dist_bias[(size_t)head_of(tile * QT + (n * 8 + 2 * t) / P + e) * a.n_dist + min(pos[n][e] - j, a.n_dist - 1)];
-                                    x *= LOG2E;
+                                    // far below and above what softmax tells apart (a bias as a mask: -1e30, or the type's lowest number): whole
+                                // numbers of x still add up with the value's log2 there, so that a row of such keys alone is their mean
+                                const float y = x * LOG2E;
+                                x = fabsf(y) > FAR && fabsf(x) < INFINITY ? copysignf(FAR, x) : y;
                                 }
                                 x = visible ? x + ev[kt][r % R] : -INFINITY;
                             }
