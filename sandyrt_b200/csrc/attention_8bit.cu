@@ -38,10 +38,12 @@
 // three stages of 4 KB each keep 190 KB on their way.  Where there are few requests `num_splits` blocks share one's keys: up to 8 are a
 // cluster, whose first block takes the others' results over its shared memory; more leave theirs in scratch, which a second kernel joins
 // in a fixed order.  Measured (bfloat16): 8 tokens x 12 heads of 64 behind 100 to 900 keys (e4m3) 6.9 us, of which half is the launch, the
-// lookup and the join; 64 x 25 heads behind 64 to 1,000 (int8) 32.4 us, 3.3 TB/s of codes: 13 us with 64 keys each, what a block's
+// lookup and the join; 64 x 25 heads behind 64 to 1,000 (int8) 32.6 us, 3.3 TB/s of codes: 13 us with 64 keys each, what a block's
 // beginning and end cost in 2.7 rounds; behind 8,000 keys each 266 us, 94% of 6.57 TB/s; 4 requests of 8 heads of 128 (e4m3), each read by 4,
-// behind 30,000 to 100,000 keys 118 us, 81%.  Where a key/value head has one query head, bfloat16 kernels keep one column a lane instead of
-// two (ONE): a tenth of the instructions, 32.4 us instead of 36.9 above.
+// behind 30,000 to 100,000 keys 120 us, 80% (a call by itself 127: two kernels).  These are tables as wide as the longest request: splits are
+// cut from the table's width, so that a request much shorter than its table is walked by the first of them.
+// Where a key/value head has one query head, bfloat16 kernels keep one column a lane instead of two (ONE): a tenth fewer instructions, 32.4 us
+// instead of 36.9 above.
 // Prompt portions: the tensor cores' warp-level instructions; the tcgen05 kernel takes over from 33 query rows on where it can.
 #include <algorithm>
 #include <atomic>
@@ -194,8 +196,9 @@ constexpr unsigned NO_POWER = 2;         // vs is not 2^ev: the weights are mult
 constexpr unsigned SEEN_BY_ALL = 4;      // every query of the block sees all keys of the tile, and scores are as they are
 constexpr unsigned SEEN_BY_ONE = 8;      // every key of the tile is seen by one query or more
 
-// Stages of KT tiles of 16 keys that a warp has on their way: 12 KB (heads of 256: 24).
-__host__ __device__ constexpr int stages_of(int dmax, int kt) { return 3; }
+// Stages of KT tiles of 16 keys that a warp has on their way: 12 KB at heads of 64 with two tiles a stage and at heads of 128 with one, 24 KB at
+// heads of 256, 6 KB at heads of 64 with one (odd pages, and blocks of 32 columns).
+constexpr int STAGES = 3;
 
 // Where piece p (16 bytes) of row r lies in its row: what a quarter warp reads at a time of the keys (two rows' 64 bytes) and half
 // a warp of the values (four rows' 32 bytes) then comes from different banks.
@@ -240,7 +243,7 @@ attention_8bit_kernel(const __grid_constant__ Args a) {
     constexpr int QT = 8 * NT / P;                       // queries of a block
     constexpr int CH = DMAX / 64;                        // runs of 64 dims
     constexpr int Q2 = P == 2 || ONE ? 1 : 2;                            // queries in a lane's two columns of a tile
-    constexpr int STAGES = stages_of(DMAX, KT), STAGE = 2 * KT * 16 * DMAX;
+    constexpr int STAGE = 2 * KT * 16 * DMAX;
     // a warp's stages [STAGES][keys | values][KT * 16 rows of DMAX bytes]; at the end the warps' sums in the same place
     extern __shared__ __align__(128) uint8_t smem[];
     float (*sm_o)[QT][DMAX + 1] = reinterpret_cast<float (*)[QT][DMAX + 1]>(smem);
@@ -825,7 +828,7 @@ int launch(const Args& a, int n_z, int max_queries, int max_n, cudaStream_t stre
     int e;
 #define LAUNCH(WARPS, DMAX, DK, NT, KT, RUN, ...)                                                                                \
     do {                                                                                                                         \
-        constexpr int QT = 8 * NT / P, ring = WARPS * stages_of(DMAX, KT) * 2 * KT * 16 * DMAX, sums = WARPS * QT * (DMAX + 1) * 4; \
+        constexpr int QT = 8 * NT / P, ring = WARPS * STAGES * 2 * KT * 16 * DMAX, sums = WARPS * QT * (DMAX + 1) * 4; \
         constexpr int alone = std::max(ring, sums), together = std::max(ring, sums + MAX_CLUSTER * QT * (DMAX + 2) * 4);          \
         e = start<attention_8bit_kernel<T, CODE, WARPS, DMAX, DK, NT, KT, RUN __VA_OPT__(,) __VA_ARGS__>>(                                                 \
             a, dim3((unsigned)((max_queries + QT - 1) / QT * a.num_splits), a.n_kv_heads, n_z), WARPS * 32,                      \

@@ -758,7 +758,8 @@ int launch(const Args& a, int n_seqs, long long tiles, cudaStream_t stream) {
 
 }  // namespace
 
-// Prompt portions as sandy_attention_8bit (attention_8bit.cu) takes them, without splits.  bfloat16, heads of up to 128, pages of a multiple
+// Prompt portions as sandy_attention_8bit (attention_8bit.cu) takes them; num_splits 1, 2, 4 or 8 blocks share a block of rows' keys as a cluster,
+// 0: the choice below.  bfloat16, heads of up to 128, pages of a multiple
 // of 16 keys, rows of q and out on 16 bytes, a positive scale, no bias by distance, no cap above 512; SANDY_ERR_UNSUPPORTED for everything else, which the
 // other kernel takes.
 SANDY_API int sandy_prefill_attention_8bit_tc(const SandyAttend8* r, cudaStream_t stream) {

@@ -12,9 +12,10 @@
 // What bounds it.  2 (keys, values) x 2 bytes in and 1 byte out a value: a copy's work.  One warp owns one block and holds the
 // block's new values in registers between the maximum and the rounding (up to 1,024 values; larger blocks are read twice,
 // the second time from the caches), so each value crosses the memory bus once.
-// Measured: 24 prompts of 400 to 930 tokens, bfloat16, 25 heads of 64, appended in 35.5 us, 67% of 6.57 TB/s: a warp's maximum stands
-// between its loads and its stores, and a block's rows are pieces of 128 bytes; a step's 8 tokens in 2.3 us, of which the work is a
-// hundredth.  Reading: 24 requests of 300 to 4,000 rows of 8 heads of 128 in 67 us, 80%; one request's 700 rows in 5 us, a
+// Measured: 24 prompts of 400 to 930 tokens, bfloat16, 25 heads of 64, appended in 35.7 us, 66% of 6.57 TB/s: under ncu 62% of the issue
+// slots are taken (14 instructions for 32 values, the indexes and conversions) and a third of the waiting is for memory, with the 25
+// warps an SM that 64 registers allow; a step's 8 tokens in 2.4 us, of which the work is a hundredth.
+// Reading: 24 requests of 300 to 4,000 rows of 8 heads of 128 in 67 us, 80%; one request's 700 rows in 5 us, a
 // launch and the chain from the table to the scale to the codes.
 #include "cache8.h"
 #include "kv_8bit.cuh"

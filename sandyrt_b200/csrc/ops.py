@@ -795,8 +795,11 @@ def decode_attention_8bit(q, cache: Cache8, block_table, token_seq, positions, o
     Head sizes 16..256 in steps of 16, any page size.  num_splits: blocks that share a request's keys (0: the kernel's choice).
     rules: window, keep_first, softcap, chunk, sink, out_gate, dist_bias, elem_gate as in paged_attention.  A token at a negative
     position (a padded one), of no visible key or with scores of minus infinity alone gets zeros; a visible key without a page is
-    reported (check_kernel_status) and left out.  Values of a block whose largest is below 2^-53 (in magnitude) count with fewer bits,
-    below 2^-77 as zeros."""
+    reported (check_kernel_status) and left out.  A cap is at most 1e30; under a cap or a bias a score counts as 5.8 million (2^23 log 2) at
+    most, and as minus that at least if it is finite.  Weights below 2^-32 of the row's largest (times its value's scale) may count as zeros in
+    bfloat16, 2^-43 in float32.  Values of a block whose largest is below 2^-53 (in magnitude) may count with fewer bits, below 2^-77 as
+    zeros, and weights of such blocks are lost beside values above 2^80.  What bounds the time of few requests is the block
+    table's width: num_splits blocks share that many keys, whatever a request holds of them."""
     what, T = "decode_attention_8bit", q.shape[0]
     width = _tokens8(what, T, _layout(block_table), _layout(token_seq), _layout(positions))
     _attention_8bit(what, q, cache, block_table, width, token_seq, positions, None, out, T, 1, n_heads, scale, num_splits, False, rules)
