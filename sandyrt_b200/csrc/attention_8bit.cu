@@ -38,7 +38,7 @@
 // three stages of 4 KB each keep 190 KB on their way.  Where there are few requests `num_splits` blocks share one's keys: up to 8 are a
 // cluster, whose first block takes the others' results over its shared memory; more leave theirs in scratch, which a second kernel joins
 // in a fixed order.  Measured (bfloat16): 8 tokens x 12 heads of 64 behind 100 to 900 keys (e4m3) 6.9 us, of which half is the launch, the
-// lookup and the join; 64 x 25 heads behind 64 to 1,000 (int8) 32.6 us, 3.3 TB/s of codes: 13 us with 64 keys each, what a block's
+// lookup and the join; 64 x 25 heads behind 64 to 1,000 (int8) 32.8 us, 3.2 TB/s of codes: 13 us with 64 keys each, what a block's
 // beginning and end cost in 2.7 rounds; behind 8,000 keys each 266 us, 94% of 6.57 TB/s; 4 requests of 8 heads of 128 (e4m3), each read by 4,
 // behind 30,000 to 100,000 keys 120 us, 80% (a call by itself 127: two kernels).  These are tables as wide as the longest request: splits are
 // cut from the table's width, so that a request much shorter than its table is walked by the first of them.
